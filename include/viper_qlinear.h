@@ -458,6 +458,137 @@ int viper_hip_clock_stamp(uint64_t* out, void* stream);
  * time the fixed cost of a dispatch. */
 int viper_hip_empty_dispatch(int workgroups, int threads, void* y_bf16, void* stream);
 
+/* ---------------------------------------------------------------- paged key/value cache
+ *
+ * The attention side of a decode / verify step: the newest rows of every
+ * sequence are rotated and stored (viper_hip_kv_append), attend over their
+ * sequence's pages (viper_hip_attention_paged) and, after the head, drafted
+ * tokens are verified (viper_hip_verify_draft).
+ *
+ * A cache is two pools of pages (K and V) of page_size tokens (32, 64, 128 or
+ * 256), [num_pages][kv_heads][page_size / 32] tiles of 32 tokens x head_dim
+ * (64, 128 or 256) values, bf16 or int8, each tile in the order in which the
+ * matrix instructions take it, so that a wave reads whole tiles with
+ * contiguous 1 KiB loads straight into operands.  Token t of its tile and
+ * dimension d of its row are element
+ *   K bf16  512 * (2 * (d / 32) + s) + 8 * (16 * g + m) + d % 8
+ *   K int8  1024 * (2 * (d / 64) + s) + 16 * (16 * g + m) + 8 * (d / 32 % 2) + d % 8
+ *           with s = t / 4 % 2, m = 4 * (t / 8) + t % 4, g = d / 8 % 4;
+ *   V bf16  512 * (d / 16) + 8 * (16 * (t / 8) + d % 16) + t % 8
+ *   V int8  1024 * (d / 32) + 16 * (16 * (t / 8) + d % 16) + 8 * (d / 16 % 2) + t % 8.
+ * int8 rows (the head_dim values of one token and head) have one fp32 scale
+ * each, k_scales and v_scales [num_pages][kv_heads][page_size]:
+ * s = max(amax / 127, 1e-8), code = RNE(x / s), the activation quantizer's
+ * rule over the row.  bf16 caches have no scales (NULL).
+ *
+ * Reference counterparts: the engine's caches and decode attention
+ * (kernels/ops/attn_decode_kernel.cu:35,155,615,727, kernels/ops/q8_kv_cache.cuh)
+ * and rope_q_k_fused (kernels/ops/rope_kernel.cu:74-186); the paged layout,
+ * window, sinks and verification have none. */
+#define VIPER_KV_BF16 0
+#define VIPER_KV_INT8 1
+#define VIPER_KV_TILE 32
+
+typedef struct viper_kv_cache {
+    int32_t kv_type; /* VIPER_KV_BF16 or VIPER_KV_INT8 */
+    int32_t kv_heads;
+    int32_t head_dim;  /* 64, 128 or 256 */
+    int32_t page_size; /* tokens: 32, 64, 128 or 256 */
+    int32_t num_pages;
+    void* k; /* the pools, 16-byte aligned */
+    void* v;
+    float* k_scales; /* int8 only, 16-byte aligned */
+    float* v_scales;
+} viper_kv_cache;
+
+/* The rows of one call.  Sequence b of `batch` holds seq_lens[b] tokens, its
+ * newest rows among them; token j lies on page block_table[b * table_width +
+ * j / page_size].  With row_offsets NULL every sequence has max_rows rows, rows
+ * b * max_rows.. of the row tensors; else sequence b has the rows
+ * row_offsets[b] .. row_offsets[b + 1] - 1 (0 to max_rows of them; the tensors
+ * hold total_rows).  Row r of n sits at position seq_lens[b] - n + r.  Rows at
+ * negative positions are no tokens: they are neither stored nor read, and their
+ * attention is zero (a batch padded with sequences of length 0).  Rows behind
+ * the last sequence are left as they were.  The three arrays are read on the
+ * device at each launch, so a captured graph follows them.
+ * Entries that do not fit (offsets outside 0 .. total_rows or more than max_rows
+ * apart, table entries outside the pool, positions past the table) never reach
+ * memory: such a sequence's rows are left alone (offsets), such a token is not
+ * stored, reads back as zeros, and makes the attention rows that see it NaN.
+ * Table entries of pages that no row sees (behind the window) are not used. */
+typedef struct viper_kv_batch {
+    int32_t batch;
+    int32_t max_rows;
+    int32_t total_rows;
+    int32_t table_width;
+    const int32_t* block_table;
+    const int32_t* seq_lens;
+    const int32_t* row_offsets; /* [batch + 1] or NULL */
+} viper_kv_batch;
+
+/* Stores the batch's rows k and v (bf16, kv_heads * head_dim values a row,
+ * kv_stride elements from row to row) in the cache.  rope_theta > 0: k is
+ * rotated by its position first, x_i, x_(i + D/2) by the angle position *
+ * theta^(-2i/D) (angles and products in 64 bits, rounded to fp32, then bf16), and so
+ * is q (heads * head_dim values a row; may be NULL) into q_out, which may be q;
+ * rope_theta = 0: k is stored as it is, q must be NULL.  Strides are multiples
+ * of 8 elements, all pointers 16-byte aligned.  Two rows of one call must not be
+ * one token. */
+int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* k_bf16,
+                        const void* v_bf16, int64_t kv_stride, const void* q_bf16, int64_t q_stride, int heads,
+                        void* q_out_bf16, int64_t q_out_stride, double rope_theta, void* stream);
+
+/* The batch's rows (any max_rows) back from the cache, k_out and v_out
+ * [total_rows][kv_heads][head_dim] bf16 (int8: bf16_RNE(code * scale)). */
+int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_batch* batch, void* k_out_bf16, void* v_out_bf16,
+                      void* stream);
+
+/* out[row][head] = sum_j w_j v_j, w = softmax(scale * q . k_j) over the tokens j
+ * that the row sees: j <= p (its position) and, with window > 0, j > p - window
+ * or j < sinks.  max_rows <= VIPER_QLINEAR_MAX_M; heads a multiple of kv_heads
+ * (query head h reads key head h / (heads / kv_heads)), at most 64 to one key
+ * head; q and out rows of heads * head_dim bf16 values, strides multiples of 8 elements, 16-byte
+ * aligned; scale finite and > 0.  Values that a row does not see (masked rows,
+ * stale or unwritten places of a page) never reach its output, whatever they
+ * hold.  The cache's length is split over workgroups that meet through
+ * workspace (16-byte aligned, viper_hip_attention_workspace_bytes() bytes, zero
+ * before the first call; every call leaves it fit for the next call of any
+ * shape that it is large enough for; calls in flight on one workspace race); with NULL one
+ * workgroup takes a key head's rows over the whole length. */
+size_t viper_hip_attention_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads);
+int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16,
+                              int64_t q_stride, int heads, float scale, int window, int sinks, void* out_bf16,
+                              int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Verification of drafted tokens (speculative sampling) for B sequences of up to
+ * R - 1 drafted tokens, R <= VIPER_QLINEAR_MAX_M rows of target logits each
+ * (bf16 [B][R][V]; row i follows drafted token i - 1).  With p_i and q_i the
+ * softmax of the target's and the drafter's logits ([B][R-1][V]; NULL: the
+ * drafter was certain, q_i is one at its token) over temperature[b] (fp32 [B],
+ * NULL: 1; 0: all on the first largest logit):
+ *   token i is accepted while uniforms[b][i] * q_i(d_i) < p_i(d_i);
+ *   at the first that is not, the next token is drawn from max(p_i - q_i, 0)
+ *   (p_i where that is all zero), after draft_lens[b] (NULL: R - 1) accepted
+ *   ones from p of the last row: the first j whose cumulated weight exceeds
+ *   uniforms[b][R - 1] times the sum.
+ * out_tokens [B][R]: the accepted tokens, the next one, then -1; out_accepted
+ * [B]: how many were accepted.  accept_probs (fp32 [B][R-1], may be NULL):
+ * min(1, p_i(d_i) / q_i(d_i)), 0 past draft_lens.  uniforms fp32 [B][R] in
+ * [0, 1).  Weights and sums in 64 bits.  NaN logits weigh nothing, a row with
+ * nothing above -inf gives token 0, infinite logits share the mass.  R = 1
+ * samples (draft_tokens may be NULL).  A draft token outside the vocabulary is
+ * rejected; a temperature that is negative or not finite, or a draft_lens[b]
+ * outside 0 .. R - 1, makes out_accepted[b] and the sequence's tokens -1.
+ * B <= 4096, V < 2^26.  workspace: viper_hip_verify_workspace_bytes(B, R, V)
+ * bytes, 16-byte aligned, zero before the first call; every call leaves it fit
+ * for the next call of any shape that it is large enough for; calls in flight
+ * on one workspace race. */
+size_t viper_hip_verify_workspace_bytes(int B, int R, int V);
+int viper_hip_verify_draft(const void* target_bf16, const void* draft_bf16, const int32_t* draft_tokens,
+                           const int32_t* draft_lens, const float* uniforms, const float* temperature, int B, int R,
+                           int V, int32_t* out_tokens, int32_t* out_accepted, float* accept_probs, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,3 +9,5 @@ from .qlinear import (GROUP, MAX_M, Prologue, QType, QuantizedWeight, ScaleEnc, 
                       linear_bf16, rmsnorm_quantize, sampling_greedy, greedy_workspace_bytes, swiglu_quantize,
                       workspace_bytes, workspace_layout, frag_bytes, rmsnorm_quantize_frag, swiglu_quantize_frag,
                       linear_prequantized_frag, linear_fused2_prequantized_frag, frag_workspace_bytes)
+from .decode import (KVBatch, KVCache, KVType, attention_paged, attention_workspace_bytes, kv_append, kv_read,  # noqa: F401
+                     verify_draft, verify_workspace_bytes)

@@ -1,0 +1,429 @@
+// Verification of drafted tokens against the target's probabilities, from given
+// uniforms (speculative sampling): accept token d_i while u_i q_i(d_i) < p_i(d_i),
+// then draw the next token from max(p - q, 0) (or p after the last).
+//
+// Which token comes out depends on comparisons with cumulated sums over the whole
+// vocabulary, so that a sum held in 32 bits would decide some of them by its
+// rounding (166144 terms: a few per cent of the draws of a flat row).  Weights e^((l - M) / T)
+// and their sums are 64-bit.
+//
+// Two launches.  verify_stats_kernel: per row and chunk of 4096 logits the
+// largest value M_c, its first index and sum_c = sum e^((l - M_c) / T).
+// verify_select_kernel, a workgroup per sequence and chunk: every workgroup joins
+// the chunks of the sequence's rows (M, Z = sum_c sum_c e^((M_c - M) / T)), finds
+// how many tokens are accepted, and sums its chunk's weights of the deciding row;
+// the one that counts last finds the chunk and the token where the cumulated
+// weight passes u times the total, in index order.
+
+#include "qlinear_host.h"
+
+namespace vq {
+
+constexpr int VF_NT = 256, VF_PT = 16, VF_CHUNK = VF_NT * VF_PT;
+constexpr int VF_CNT = 4096;  // sequences of a call, a counter each
+
+struct VfStat {
+    double sum;
+    float max;
+    int arg;
+};
+
+struct VerifyArgs {
+    const uint16_t* target;
+    const uint16_t* draft;
+    const int32_t* tokens;
+    const int32_t* lens;
+    const float* uniforms;
+    const float* temperature;
+    int32_t* out;
+    int32_t* accepted;
+    float* ratios;
+    unsigned* cnt;
+    VfStat* stats;  // [B][2R - 1][chunks]: the target's rows, then the drafter's
+    double* sums;   // [B][chunks]
+    int B, R, V, chunks;
+};
+
+// Sequence b's temperature and drafted tokens; false where they do not fit
+__device__ __forceinline__ bool vf_seq(const VerifyArgs& a, int b, float& T, int& n) {
+    T = a.temperature != nullptr ? a.temperature[b] : 1.0f;
+    n = a.lens != nullptr ? a.lens[b] : a.R - 1;
+    return T >= 0.0f && T < __builtin_inff() && n >= 0 && n < a.R;
+}
+
+// 16 logits from index j of a row; past the row NaN, which weighs nothing
+template <bool VEC>
+__device__ __forceinline__ void vf_load(const uint16_t* row, int j, int V, float* l) {
+    if constexpr (VEC) {  // rows of whole octets, 16-byte aligned
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 v = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+            if (j + 8 * h < V) v = *(const u32x4*)(row + j + 8 * h);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) l[8 * h + i] = bf16f((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) l[i] = j + i < V ? bf16f(row[j + i]) : __uint_as_float(0x7fc00000u);
+    }
+}
+
+// e^((l - M) / T): 1 at the maximum (also an infinite one), 0 for NaN
+__device__ __forceinline__ double vf_exp(float l, float M, double iT) {
+    if (l == M) return 1.0;
+    if (!(l < M)) return 0.0;
+    return exp(((double)l - (double)M) * iT);
+}
+
+// What a row's weights need: p(j) = weight(l_j, j)
+struct VfRow {
+    double iz, iT;
+    float M;
+    int arg;
+    bool one;  // all on arg
+    __device__ __forceinline__ double weight(float l, int j) const {
+        if (one) return j == arg ? 1.0 : 0.0;
+        return vf_exp(l, M, iT) * iz;
+    }
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+// Sum over the workgroup, in a fixed order; red holds a value per wave
+__device__ __forceinline__ double wg_sum(double v, double* red) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return ((red[0] + red[1]) + red[2]) + red[3];
+}
+// Inclusive sum over the threads before and at this one
+__device__ __forceinline__ double wg_scan(double v, double* red) {
+    const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
+    for (int off = 1; off < 64; off <<= 1) {
+        const double o = __shfl_up(v, off, 64);
+        if (lane >= off) v += o;
+    }
+    __syncthreads();
+    if (lane == 63) red[wave] = v;
+    __syncthreads();
+    double before = 0.0;
+    for (int w = 0; w < wave; ++w) before += red[w];
+    return before + v;
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(VF_NT)
+verify_stats_kernel(VerifyArgs a) {
+    __shared__ float smax[VF_NT / 64];
+    __shared__ int sarg;
+    __shared__ double red[VF_NT / 64];
+    const int c = (int)blockIdx.x % a.chunks, rid = (int)blockIdx.x / a.chunks;
+    const int per = a.draft != nullptr ? 2 * a.R - 1 : a.R;  // rows of a sequence
+    const int b = rid / per, i = rid % per, tid = (int)threadIdx.x;
+    float T;
+    int n;
+    if (!vf_seq(a, b, T, n)) return;
+    if (i < a.R ? i > n : i - a.R >= n) return;
+    const uint16_t* row = i < a.R ? a.target + ((size_t)b * a.R + i) * a.V : a.draft + ((size_t)b * (a.R - 1) + i - a.R) * a.V;
+    const int j0 = c * VF_CHUNK + tid * VF_PT;
+    float l[VF_PT];
+    vf_load<VEC>(row, j0, a.V, l);
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int k = 0; k < VF_PT; ++k) m = fmaxf(m, l[k]);
+    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    if ((tid & 63) == 0) smax[tid >> 6] = m;
+    if (tid == 0) sarg = 0x7fffffff;
+    __syncthreads();
+    m = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+    int arg = 0x7fffffff;
+#pragma unroll
+    for (int k = VF_PT - 1; k >= 0; --k)
+        if (l[k] == m) arg = j0 + k;
+    if (arg != 0x7fffffff) atomicMin(&sarg, arg);
+    double sum = 0.0;
+    if (T > 0.0f && m > -__builtin_inff()) {
+        const double iT = 1.0 / (double)T;
+#pragma unroll
+        for (int k = 0; k < VF_PT; ++k) sum += vf_exp(l[k], m, iT);
+    }
+    sum = wg_sum(sum, red);  // (and every thread's index)
+    if (tid == 0) a.stats[((size_t)b * (2 * a.R - 1) + i) * a.chunks + c] = VfStat{sum, m, sarg};
+}
+
+template <bool VEC>
+__global__ void __launch_bounds__(VF_NT)
+verify_select_kernel(VerifyArgs a) {
+    __shared__ VfRow rows[2 * VIPER_QLINEAR_MAX_M];
+    __shared__ int taken[VIPER_QLINEAR_MAX_M];
+    __shared__ double red[VF_NT / 64];
+    __shared__ int pick, last_part;
+    __shared__ double before;
+    const int c = (int)blockIdx.x % a.chunks, b = (int)blockIdx.x / a.chunks;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int32_t* out = a.out + (size_t)b * a.R;
+    float T;
+    int n;
+    if (!vf_seq(a, b, T, n)) {
+        if (c == 0) {
+            if (tid < a.R) out[tid] = -1;
+            if (tid == 0) a.accepted[b] = -1;
+            if (a.ratios != nullptr && tid < a.R - 1) a.ratios[(size_t)b * (a.R - 1) + tid] = 0.0f;
+        }
+        return;
+    }
+    const double iT = T > 0.0f ? 1.0 / (double)T : 0.0;
+    const VfStat* stats = a.stats + (size_t)b * (2 * a.R - 1) * a.chunks;
+
+    // the rows' maxima and sums, a wave per row: rows 0 .. n of the target, n of the drafter
+    const int nrows = n + 1 + (a.draft != nullptr ? n : 0);
+    for (int k = wave; k < nrows; k += VF_NT / 64) {
+        const VfStat* s = stats + (size_t)(k <= n ? k : a.R + k - n - 1) * a.chunks;
+        float M = -__builtin_inff();
+        int arg = 0x7fffffff;
+        for (int x = lane; x < a.chunks; x += 64) {
+            const VfStat v = s[x];
+            if (v.max > M) {  // (chunks in index order: the first of equal ones stays)
+                M = v.max;
+                arg = v.arg;
+            }
+        }
+        for (int off = 32; off > 0; off >>= 1) {
+            const float om = __shfl_xor(M, off, 64);
+            const int oa = __shfl_xor(arg, off, 64);
+            if (om > M || (om == M && oa < arg)) {
+                M = om;
+                arg = oa;
+            }
+        }
+        double z = 0.0;
+        for (int x = lane; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, iT);
+        z = wave_sum(z);
+        if (lane == 0) {
+            VfRow r;
+            r.M = M;
+            r.iT = iT;
+            r.iz = 1.0 / z;
+            const bool none = !(M > -__builtin_inff());
+            r.arg = none ? 0 : arg;
+            r.one = none || T == 0.0f;
+            rows[k] = r;
+        }
+    }
+    __syncthreads();
+    const uint16_t* trow = a.target + (size_t)b * a.R * a.V;
+    const uint16_t* drow = a.draft != nullptr ? a.draft + (size_t)b * (a.R - 1) * a.V : nullptr;
+    if (tid < n) {
+        const int d = a.tokens[(size_t)b * (a.R - 1) + tid];
+        double p = 0.0, q = 1.0;
+        if (d >= 0 && d < a.V) {
+            p = rows[tid].weight(bf16f(trow[(size_t)tid * a.V + d]), d);
+            if (drow != nullptr) q = rows[n + 1 + tid].weight(bf16f(drow[(size_t)tid * a.V + d]), d);
+        }
+        taken[tid] = (double)a.uniforms[(size_t)b * a.R + tid] * q < p;
+        if (c == 0 && a.ratios != nullptr)
+            a.ratios[(size_t)b * (a.R - 1) + tid] = p > 0.0 ? (float)fmin(1.0, p / q) : 0.0f;
+    } else if (c == 0 && a.ratios != nullptr && tid < a.R - 1) {
+        a.ratios[(size_t)b * (a.R - 1) + tid] = 0.0f;
+    }
+    __syncthreads();
+    int r = 0;  // the deciding row
+    while (r < n && taken[r]) ++r;
+    const VfRow pr = rows[r];
+    const bool less = r < n;  // a rejected token: what the drafter gave is taken away
+    const bool point = less && drow == nullptr;
+    const int dtok = less ? a.tokens[(size_t)b * (a.R - 1) + r] : -1;
+    VfRow qr = pr;
+    if (less && drow != nullptr) qr = rows[n + 1 + r];
+    const uint16_t* prow = trow + (size_t)r * a.V;
+    const uint16_t* qrow = less && drow != nullptr ? drow + (size_t)r * a.V : nullptr;
+
+    // weights of 16 consecutive tokens; plain: the target's own
+    auto weights = [&](int j, bool plain, double* w) {
+        float l[VF_PT], ld[VF_PT];
+        vf_load<VEC>(prow, j, a.V, l);
+        if (!plain && qrow != nullptr) vf_load<VEC>(qrow, j, a.V, ld);
+#pragma unroll
+        for (int k = 0; k < VF_PT; ++k) {
+            double v = j + k < a.V ? pr.weight(l[k], j + k) : 0.0;
+            if (!plain && less && j + k < a.V) {
+                const double q = point ? (j + k == dtok ? 1.0 : 0.0) : qr.weight(ld[k], j + k);
+                v = fmax(v - q, 0.0);
+            }
+            w[k] = v;
+        }
+    };
+    double w[VF_PT], sum = 0.0;
+    weights(c * VF_CHUNK + tid * VF_PT, false, w);
+#pragma unroll
+    for (int k = 0; k < VF_PT; ++k) sum += w[k];
+    sum = wg_sum(sum, red);
+    double* sums = a.sums + (size_t)b * a.chunks;
+    if (tid == 0) {
+        sums[c] = sum;
+        __threadfence();
+        const unsigned old = __hip_atomic_fetch_add(a.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        last_part = old == (unsigned)(a.chunks - 1);
+        if (last_part) __hip_atomic_store(a.cnt + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last_part) return;
+    __threadfence();
+
+    // the chunk: threads hold consecutive runs of chunk sums
+    const int run = (a.chunks + VF_NT - 1) / VF_NT, x0 = min(tid * run, a.chunks), x1 = min(x0 + run, a.chunks);
+    bool plain = false;
+    double mine = 0.0, scan = 0.0, total = 0.0;
+    auto chunk_sum = [&](int x) {
+        if (!plain) return sums[x];
+        const VfStat v = stats[(size_t)r * a.chunks + x];
+        if (pr.one) return pr.arg / VF_CHUNK == x ? 1.0 : 0.0;
+        return v.sum * vf_exp(v.max, pr.M, iT) * pr.iz;
+    };
+    for (int pass = 0; pass < 2; ++pass) {
+        mine = 0.0;
+        for (int x = x0; x < x1; ++x) mine += chunk_sum(x);
+        scan = wg_scan(mine, red);
+        __syncthreads();
+        if (tid == VF_NT - 1) before = scan;
+        __syncthreads();
+        total = before;
+        if (total > 0.0) break;
+        plain = true;  // nothing left of the target's weights: the target's own
+    }
+    const double u = fmax(0.0, (double)a.uniforms[(size_t)b * a.R + a.R - 1]);
+    double goal = u * total;
+    if (tid == 0) pick = 0x7fffffff;
+    __syncthreads();
+    if (mine > 0.0 && scan > goal) atomicMin(&pick, tid);
+    __syncthreads();
+    if (pick != 0x7fffffff) {
+        if (tid == pick) {
+            // the chunk within this thread's run: its sums are added up again from
+            // what comes before them
+            double acc = scan - mine;
+            for (int x = x0; x < x1; ++x) {
+                const double v = chunk_sum(x);
+                if (!(v > 0.0)) continue;
+                before = acc;
+                last_part = x;
+                acc += v;
+                if (acc > goal) break;
+            }
+        }
+    } else {  // u * total rounded up to the total: the last chunk with a weight
+        if (tid == 0) pick = -1;
+        __syncthreads();
+        int lastx = -1;
+        for (int x = x0; x < x1; ++x)
+            if (chunk_sum(x) > 0.0) lastx = x;
+        if (lastx >= 0) atomicMax(&pick, lastx);
+        __syncthreads();
+        if (tid == 0) {
+            last_part = pick < 0 ? 0 : pick;
+            before = 0.0;
+        }
+        goal = __builtin_inf();
+    }
+    __syncthreads();
+    const int ch = last_part;
+    const double base = before;
+    const int j0 = ch * VF_CHUNK + tid * VF_PT;
+    weights(j0, plain, w);
+    sum = 0.0;
+    int mylast = -1;
+#pragma unroll
+    for (int k = 0; k < VF_PT; ++k) {
+        sum += w[k];
+        if (w[k] > 0.0) mylast = j0 + k;
+    }
+    scan = base + wg_scan(sum, red);
+    __syncthreads();
+    if (tid == 0) pick = 0x7fffffff;
+    __syncthreads();
+    if (mylast >= 0 && scan > goal) {
+        // the first token of this thread that passes; its last one where the
+        // additions' order hides it
+        double acc = scan - sum;
+        int j = mylast;
+#pragma unroll
+        for (int k = 0; k < VF_PT; ++k) {
+            acc += w[k];
+            if (w[k] > 0.0 && acc > goal && j0 + k < j) j = j0 + k;
+        }
+        atomicMin(&pick, j);
+    }
+    __syncthreads();
+    if (pick == 0x7fffffff) {  // the chunk's last token with a weight
+        __syncthreads();
+        if (tid == 0) pick = -1;
+        __syncthreads();
+        if (mylast >= 0) atomicMax(&pick, mylast);
+        __syncthreads();
+    }
+    const int token = pick < 0 ? pr.arg : pick;
+    if (tid < a.R) out[tid] = tid < r ? a.tokens[(size_t)b * (a.R - 1) + tid] : tid == r ? token : -1;
+    if (tid == 0) a.accepted[b] = r;
+}
+
+static int64_t vf_chunks(int V) { return ((int64_t)V + VF_CHUNK - 1) / VF_CHUNK; }
+static bool vf_sizes(int B, int R, int V) {
+    return B > 0 && B <= VF_CNT && R > 0 && R <= VIPER_QLINEAR_MAX_M && V > 0 && V < 1 << 26 &&
+           (int64_t)B * (2 * R - 1) * vf_chunks(V) <= (1 << 24) - 1;
+}
+static size_t vf_bytes(int B, int R, int V) {
+    const size_t ch = (size_t)vf_chunks(V);
+    return VF_CNT * 4 + (size_t)B * (2 * R - 1) * ch * sizeof(VfStat) + (size_t)B * ch * 8;
+}
+
+}  // namespace vq
+
+extern "C" size_t viper_hip_verify_workspace_bytes(int B, int R, int V) {
+    return vq::vf_sizes(B, R, V) ? vq::vf_bytes(B, R, V) : 0;
+}
+
+extern "C" int viper_hip_verify_draft(const void* target_bf16, const void* draft_bf16, const int32_t* draft_tokens,
+                                      const int32_t* draft_lens, const float* uniforms, const float* temperature, int B,
+                                      int R, int V, int32_t* out_tokens, int32_t* out_accepted, float* accept_probs,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+    using namespace vq;
+    if (target_bf16 == nullptr || uniforms == nullptr || out_tokens == nullptr || out_accepted == nullptr)
+        return VIPER_INVALID_ARGUMENT;
+    if (!vf_sizes(B, R, V) || (R > 1 && draft_tokens == nullptr)) return VIPER_INVALID_ARGUMENT;
+    if (misaligned(target_bf16, 2) || misaligned(draft_bf16, 2) || misaligned(draft_tokens, 4) || misaligned(draft_lens, 4) ||
+        misaligned(uniforms, 4) || misaligned(temperature, 4) || misaligned(out_tokens, 4) || misaligned(out_accepted, 4) ||
+        misaligned(accept_probs, 4))
+        return VIPER_INVALID_ARGUMENT;
+    if (workspace == nullptr || misaligned(workspace, 16) || workspace_bytes < vf_bytes(B, R, V)) return VIPER_INVALID_ARGUMENT;
+    VerifyArgs a;
+    a.target = (const uint16_t*)target_bf16;
+    a.draft = R > 1 ? (const uint16_t*)draft_bf16 : nullptr;
+    a.tokens = draft_tokens;
+    a.lens = draft_lens;
+    a.uniforms = uniforms;
+    a.temperature = temperature;
+    a.out = out_tokens;
+    a.accepted = out_accepted;
+    a.ratios = accept_probs;
+    a.B = B;
+    a.R = R;
+    a.V = V;
+    a.chunks = (int)vf_chunks(V);
+    a.cnt = (unsigned*)workspace;
+    a.stats = (VfStat*)((char*)workspace + VF_CNT * 4);
+    a.sums = (double*)(a.stats + (size_t)B * (2 * R - 1) * a.chunks);
+    const bool vec = V % 8 == 0 && !misaligned(target_bf16, 16) && !misaligned(draft_bf16, 16);
+    const unsigned rows = (unsigned)B * (a.draft != nullptr ? 2 * R - 1 : R);
+    void* args[] = {&a};
+    launch(vec ? (const void*)verify_stats_kernel<true> : (const void*)verify_stats_kernel<false>, rows * (unsigned)a.chunks,
+           VF_NT, 0, (hipStream_t)stream, args);
+    const int rc = status_of(hipGetLastError());
+    if (rc != VIPER_OK) return rc;
+    launch(vec ? (const void*)verify_select_kernel<true> : (const void*)verify_select_kernel<false>,
+           (unsigned)B * (unsigned)a.chunks, VF_NT, 0, (hipStream_t)stream, args);
+    return status_of(hipGetLastError());
+}

@@ -145,6 +145,12 @@ _SYMBOLS = (
     "viper_hip_qlinear_fused2_prequantized_frag",
     "viper_hip_qlinear_frag_timeline",
     "viper_hip_qlinear_route",
+    "viper_hip_kv_append",
+    "viper_hip_kv_read",
+    "viper_hip_attention_workspace_bytes",
+    "viper_hip_attention_paged",
+    "viper_hip_verify_workspace_bytes",
+    "viper_hip_verify_draft",
 )
 
 
@@ -228,6 +234,19 @@ def lib():
     L.viper_hip_qlinear_m1_swiglu.argtypes = [i32, i32, i32, i32, i32, vp, vp, C.c_float, vp, vp, vp, vp, vp, i32,
                                               vp, vp, vp, vp]
     L.viper_hip_qlinear_m1_swiglu.restype = i32
+    i64 = C.c_int64
+    L.viper_hip_kv_append.argtypes = [vp, vp, vp, vp, i64, vp, i64, i32, vp, i64, C.c_double, vp]
+    L.viper_hip_kv_append.restype = i32
+    L.viper_hip_kv_read.argtypes = [vp, vp, vp, vp, vp]
+    L.viper_hip_kv_read.restype = i32
+    L.viper_hip_attention_workspace_bytes.argtypes = [vp, vp, i32]
+    L.viper_hip_attention_workspace_bytes.restype = sz
+    L.viper_hip_attention_paged.argtypes = [vp, vp, vp, i64, i32, C.c_float, i32, i32, vp, i64, vp, sz, vp]
+    L.viper_hip_attention_paged.restype = i32
+    L.viper_hip_verify_workspace_bytes.argtypes = [i32, i32, i32]
+    L.viper_hip_verify_workspace_bytes.restype = sz
+    L.viper_hip_verify_draft.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp]
+    L.viper_hip_verify_draft.restype = i32
     _lib = L
     return L
 
