@@ -4,11 +4,21 @@
 
 namespace vq {
 
-const void* attn_kernel_bf16(int D, int qt);
-const void* attn_kernel_int8(int D, int qt);
+AttnFn attn_kernels_bf16(int D, int qt, int W);
+AttnFn attn_kernels_int8(int D, int qt, int W);
+
+// One row of 20 heads over 4 key heads, 128 dims:
+//  * 8 waves a CU (one workgroup, each wave a tile in use and one in flight): 131072
+//    tokens 47.2 us, with 4 waves 52.3, 16 (in two workgroups) 49.5;
+//  * up to 4096 tokens in the table workgroups of 4 waves, one tile each, over more
+//    CUs (a CU reads 0.1 TB/s): 512 tokens 7.1 us, in eights 7.7;
+//  * 80 KB of parts or more of a group of rows are joined by a launch of their own,
+//    below by the workgroup that counts last: 16384 tokens in 64 parts 13.3 us
+//    against 16.1, 512 in 4 parts 8.5 against 7.1 (2 x 16 rows of 8000: 20 against 37).
+constexpr int AT_WAVES = 8, AT_PARTS = 64, AT_SHORT = 4096 / KV_TILE, AT_APART = 80000;
 
 struct AttnPlan {
-    int qt, qgroups, splits, min_tiles;
+    int qt, qgroups, waves, splits, lrows;
     size_t bytes;  // of workspace; 0: one part
 };
 
@@ -18,14 +28,18 @@ static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int 
     const int t16 = (b->max_rows * gqa + 15) / 16;
     p.qgroups = (t16 + most - 1) / most;
     p.qt = (t16 + p.qgroups - 1) / p.qgroups;
-    p.min_tiles = AT_W;  // one per wave
+    p.lrows = b->max_rows * gqa < p.qt * 16 ? b->max_rows * gqa : p.qt * 16;
     const int64_t base = (int64_t)b->batch * c->kv_heads * p.qgroups;
     const int64_t tiles = (int64_t)b->table_width * (c->page_size / KV_TILE);
+    p.waves = at_waves(c->head_dim, p.qt);
+    if (tiles <= AT_SHORT) p.waves = 4;
     int64_t s = 1;
     if (base <= AT_CNT) {
-        s = (2 * (int64_t)device_cus() + base - 1) / base;
-        const int64_t fit = (tiles + p.min_tiles - 1) / p.min_tiles;
+        const int64_t wgs = (int64_t)device_cus() * AT_WAVES / p.waves;
+        s = (wgs + base - 1) / base;
+        const int64_t fit = (tiles + p.waves - 1) / p.waves;
         if (s > fit) s = fit;
+        if (s > AT_PARTS) s = AT_PARTS;
     }
     p.splits = (int)s;
     p.bytes = s > 1 ? AT_CNT * 4 + (size_t)base * s * at_part_floats(c->head_dim, p.qt) * 4 : 0;
@@ -74,17 +88,24 @@ extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const vipe
     a.gqa = heads / cache->kv_heads;
     a.qgroups = p.qgroups;
     a.splits = p.splits;
-    a.min_tiles = p.min_tiles;
+    a.lrows = p.lrows;
     // a window longer than any sequence hides nothing (and p - window stays in 32 bits)
     a.window = window > INT32_MAX - VIPER_QLINEAR_MAX_M ? 0 : window;
     a.sinks = sinks;
     a.scale = scale * 1.44269504088896340736f;
-    const int64_t grid = (int64_t)batch->batch * cache->kv_heads * p.qgroups * p.splits;
-    if (grid > (1 << 24) - 1) return VIPER_INVALID_ARGUMENT;
     const int D = cache->head_dim;
-    const void* fn = cache->kv_type == VIPER_KV_INT8 ? attn_kernel_int8(D, p.qt) : attn_kernel_bf16(D, p.qt);
-    if (fn == nullptr) return VIPER_INTERNAL;
+    const AttnFn fn = cache->kv_type == VIPER_KV_INT8 ? attn_kernels_int8(D, p.qt, p.waves) : attn_kernels_bf16(D, p.qt, p.waves);
+    if (fn.attn == nullptr) return VIPER_INTERNAL;
+    a.by_gqa = (65536u + (unsigned)a.gqa - 1) / (unsigned)a.gqa;
+    a.apart = p.splits > 1 && (int64_t)p.splits * p.lrows * D * 4 >= AT_APART;
     void* args[] = {&a};
-    launch(fn, (unsigned)grid, AT_NT, at_lds_bytes(D, p.qt), (hipStream_t)stream, args);
+    const dim3 grid((unsigned)p.splits, (unsigned)(cache->kv_heads * p.qgroups), (unsigned)batch->batch);
+    (void)hipLaunchKernel(fn.attn, grid, dim3((unsigned)p.waves * 64), args, at_lds_bytes(D, p.qt, p.waves, p.lrows),
+                          (hipStream_t)stream);
+    if (a.apart) {
+        const int rc2 = status_of(hipGetLastError());
+        if (rc2 != VIPER_OK) return rc2;
+        (void)hipLaunchKernel(fn.join, dim3((unsigned)p.lrows, grid.y, grid.z), dim3(AT_JNT), args, 0, (hipStream_t)stream);
+    }
     return status_of(hipGetLastError());
 }

@@ -1,5 +1,5 @@
 // Attention over a bf16 cache.
 #include "attention.h"
 namespace vq {
-const void* attn_kernel_bf16(int D, int qt) { return attn_fn<false>(D, qt); }
+AttnFn attn_kernels_bf16(int D, int qt, int W) { return attn_fn<false>(D, qt, W); }
 }  // namespace vq

@@ -1,5 +1,5 @@
 // Attention over an int8 cache.
 #include "attention.h"
 namespace vq {
-const void* attn_kernel_int8(int D, int qt) { return attn_fn<true>(D, qt); }
+AttnFn attn_kernels_int8(int D, int qt, int W) { return attn_fn<true>(D, qt, W); }
 }  // namespace vq

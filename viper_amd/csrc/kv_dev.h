@@ -40,6 +40,12 @@ __device__ __forceinline__ int v_place(int t, int d) {
     return I8 ? 1024 * (d >> 5) + 16 * lane + 8 * ((d >> 4) & 1) + (t & 7) : 512 * (d >> 4) + 8 * lane + (t & 7);
 }
 
+// Wave-uniform reads of the arrays through the scalar cache (read-only within a
+// launch), so that a page's number is in scalar registers and its wait does not
+// count the vector loads in flight.
+typedef const __attribute__((address_space(4))) int32_t* kv_cptr;
+__device__ __forceinline__ int kv_sload(const int32_t* p, size_t i) { return ((kv_cptr)(uintptr_t)p)[i]; }
+
 // Sequence b's rows: the first, their count (0 where the offsets do not fit)
 // and the sequence's length.
 struct KvSeq {
@@ -47,9 +53,9 @@ struct KvSeq {
 };
 __device__ __forceinline__ KvSeq kv_seq(const KvArgs& a, int b) {
     KvSeq q;
-    q.len = a.lens[b];
+    q.len = kv_sload(a.lens, b);
     if (a.offs != nullptr) {
-        const int o = a.offs[b], e = a.offs[b + 1];
+        const int o = kv_sload(a.offs, b), e = kv_sload(a.offs, b + 1);
         const bool fits = o >= 0 && o <= e && e <= a.total_rows && e - o <= a.max_rows;
         q.row0 = fits ? o : 0;
         q.n = fits ? e - o : 0;
@@ -65,6 +71,12 @@ __device__ __forceinline__ int kv_page(const KvArgs& a, int b, int tile) {
     const int col = tile >> a.tpl;
     if (col >= a.width) return -1;
     const int p = a.table[(size_t)b * a.width + col];
+    return (unsigned)p < (unsigned)a.pages ? p : -1;
+}
+__device__ __forceinline__ int kv_page_uniform(const KvArgs& a, int b, int tile) {
+    const int col = tile >> a.tpl;
+    if (col >= a.width) return -1;
+    const int p = kv_sload(a.table, (size_t)b * a.width + col);
     return (unsigned)p < (unsigned)a.pages ? p : -1;
 }
 // Tile number in the pool (times 32 * D elements; times 32 for the scales).
