@@ -15,6 +15,9 @@ AttnFn attn_kernels_int8(int D, int qt, int W);
 //  * 80 KB of parts or more of a group of rows are joined by a launch of their own,
 //    below by the workgroup that counts last: 16384 tokens in 64 parts 13.3 us
 //    against 16.1, 512 in 4 parts 8.5 against 7.1 (2 x 16 rows of 8000: 20 against 37).
+// Parts of equal steps dealt out over all sequences of a batch, whatever their
+// lengths, were slower (32 x 8192 tokens 92.9 us against 85.7, 256 x 600 76 against
+// 36): a part that ends one sequence and begins another waits at both.
 constexpr int AT_WAVES = 8, AT_PARTS = 64, AT_SHORT = 4096 / KV_TILE, AT_APART = 80000;
 
 struct AttnPlan {
@@ -35,7 +38,8 @@ static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int 
     if (tiles <= AT_SHORT) p.waves = 4;
     int64_t s = 1;
     if (base <= AT_CNT) {
-        const int64_t wgs = (int64_t)device_cus() * AT_WAVES / p.waves;
+        const bool two = b->batch > 1 && at_two(c->head_dim, c->kv_type == VIPER_KV_INT8, p.qt);
+        const int64_t wgs = (int64_t)device_cus() * AT_WAVES * (two ? 2 : 1) / p.waves;
         s = (wgs + base - 1) / base;
         const int64_t fit = (tiles + p.waves - 1) / p.waves;
         if (s > fit) s = fit;
