@@ -10,16 +10,20 @@
 // Two launches.  verify_stats_kernel: per row and chunk of 4096 logits the
 // largest value M_c, its first index and sum_c = sum e^((l - M_c) / T).
 // verify_select_kernel, a workgroup per sequence and chunk: every workgroup joins
-// the chunks of the sequence's rows (M, Z = sum_c sum_c e^((M_c - M) / T)), finds
-// how many tokens are accepted, and sums its chunk's weights of the deciding row;
-// the one that counts last finds the chunk and the token where the cumulated
-// weight passes u times the total, in index order.
+// the chunks of the sequence's rows (M, Z = sum_c sum_c e^((M_c - M) / T)) and finds
+// how many tokens are accepted.  Where the deciding row's weights are p itself
+// (nothing rejected, or a certain drafter: p without its token) the sums of its
+// chunks are known and the first workgroup goes on alone; else each sums
+// max(p - q, 0) over its chunk and the one that counts last goes on: it finds the chunk
+// and the token where the cumulated weight passes u times the total, in index order.
 
 #include "qlinear_host.h"
 
 namespace vq {
 
-constexpr int VF_NT = 256, VF_PT = 16, VF_CHUNK = VF_NT * VF_PT;
+constexpr int VF_CHUNK = 4096;
+constexpr int VF_NT = 256, VF_PT = VF_CHUNK / VF_NT;  // verify_stats_kernel
+constexpr int VS_NT = 512, VS_PT = VF_CHUNK / VS_NT;  // verify_select_kernel
 constexpr int VF_CNT = 4096;  // sequences of a call, a counter each
 
 struct VfStat {
@@ -51,12 +55,12 @@ __device__ __forceinline__ bool vf_seq(const VerifyArgs& a, int b, float& T, int
     return T >= 0.0f && T < __builtin_inff() && n >= 0 && n < a.R;
 }
 
-// 16 logits from index j of a row; past the row NaN, which weighs nothing
-template <bool VEC>
+// N logits from index j of a row; past the row NaN, which weighs nothing
+template <bool VEC, int N>
 __device__ __forceinline__ void vf_load(const uint16_t* row, int j, int V, float* l) {
     if constexpr (VEC) {  // rows of whole octets, 16-byte aligned
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < N / 8; ++h) {
             u32x4 v = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
             if (j + 8 * h < V) v = *(const u32x4*)(row + j + 8 * h);
             const uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -65,15 +69,38 @@ __device__ __forceinline__ void vf_load(const uint16_t* row, int j, int V, float
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) l[i] = j + i < V ? bf16f(row[j + i]) : __uint_as_float(0x7fc00000u);
+        for (int i = 0; i < N; ++i) l[i] = j + i < V ? bf16f(row[j + i]) : __uint_as_float(0x7fc00000u);
     }
 }
 
+// e^x for x <= 0 in 64 bits: 2^n 2^f with n + f = x log2 e, |f| <= 1/2, and the
+// power series of 2^f = e^(f ln 2) to its 12th term ((ln 2 / 2)^13 / 13! =
+// 1.7e-16 is left out).  The rounding of x log2 e is off by |x| 2^-53, which
+// matters only to weights of e^x.  About 20 instructions, where the general
+// exp() with its cases takes three times as many (8 batches of full drafts: see
+// below).
+__device__ __forceinline__ double exp_neg(double x) {
+    const double y = fmax(x * 1.4426950408889634074, -1100.0), n = rint(y), f = y - n;
+    double p = 2.5678435993488196e-11;         // ln2^12 / 12!
+    p = __builtin_fma(p, f, 4.4455382718708101e-10);
+    p = __builtin_fma(p, f, 7.0549116208011209e-09);
+    p = __builtin_fma(p, f, 1.0178086009239696e-07);
+    p = __builtin_fma(p, f, 1.3215486790144305e-06);
+    p = __builtin_fma(p, f, 1.5252733804059838e-05);
+    p = __builtin_fma(p, f, 1.5403530393381606e-04);
+    p = __builtin_fma(p, f, 1.3333558146428441e-03);
+    p = __builtin_fma(p, f, 9.6181291076284770e-03);
+    p = __builtin_fma(p, f, 5.5504108664821576e-02);
+    p = __builtin_fma(p, f, 2.4022650695910070e-01);
+    p = __builtin_fma(p, f, 6.9314718055994531e-01);
+    p = __builtin_fma(p, f, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)n);
+}
 // e^((l - M) / T): 1 at the maximum (also an infinite one), 0 for NaN
 __device__ __forceinline__ double vf_exp(float l, float M, double iT) {
     if (l == M) return 1.0;
     if (!(l < M)) return 0.0;
-    return exp(((double)l - (double)M) * iT);
+    return exp_neg(((double)l - (double)M) * iT);
 }
 
 // What a row's weights need: p(j) = weight(l_j, j)
@@ -93,12 +120,16 @@ __device__ __forceinline__ double wave_sum(double v) {
     return v;
 }
 // Sum over the workgroup, in a fixed order; red holds a value per wave
+template <int NT>
 __device__ __forceinline__ double wg_sum(double v, double* red) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return ((red[0] + red[1]) + red[2]) + red[3];
+    double t = red[0];
+#pragma unroll
+    for (int w = 1; w < NT / 64; ++w) t += red[w];
+    return t;
 }
 // Inclusive sum over the threads before and at this one
 __device__ __forceinline__ double wg_scan(double v, double* red) {
@@ -131,7 +162,7 @@ verify_stats_kernel(VerifyArgs a) {
     const uint16_t* row = i < a.R ? a.target + ((size_t)b * a.R + i) * a.V : a.draft + ((size_t)b * (a.R - 1) + i - a.R) * a.V;
     const int j0 = c * VF_CHUNK + tid * VF_PT;
     float l[VF_PT];
-    vf_load<VEC>(row, j0, a.V, l);
+    vf_load<VEC, VF_PT>(row, j0, a.V, l);
     float m = -__builtin_inff();
 #pragma unroll
     for (int k = 0; k < VF_PT; ++k) m = fmaxf(m, l[k]);
@@ -151,16 +182,17 @@ verify_stats_kernel(VerifyArgs a) {
 #pragma unroll
         for (int k = 0; k < VF_PT; ++k) sum += vf_exp(l[k], m, iT);
     }
-    sum = wg_sum(sum, red);  // (and every thread's index)
+    sum = wg_sum<VF_NT>(sum, red);  // (and every thread's index)
     if (tid == 0) a.stats[((size_t)b * (2 * a.R - 1) + i) * a.chunks + c] = VfStat{sum, m, sarg};
 }
 
 template <bool VEC>
-__global__ void __launch_bounds__(VF_NT)
+__global__ void __launch_bounds__(VS_NT)
 verify_select_kernel(VerifyArgs a) {
+    constexpr int W = VS_NT / 64, RPW = (2 * VIPER_QLINEAR_MAX_M + W - 1) / W;  // rows of a wave
     __shared__ VfRow rows[2 * VIPER_QLINEAR_MAX_M];
     __shared__ int taken[VIPER_QLINEAR_MAX_M];
-    __shared__ double red[VF_NT / 64];
+    __shared__ double red[W];
     __shared__ int pick, last_part;
     __shared__ double before;
     const int c = (int)blockIdx.x % a.chunks, b = (int)blockIdx.x / a.chunks;
@@ -178,14 +210,39 @@ verify_select_kernel(VerifyArgs a) {
     }
     const double iT = T > 0.0f ? 1.0 / (double)T : 0.0;
     const VfStat* stats = a.stats + (size_t)b * (2 * a.R - 1) * a.chunks;
+    const uint16_t* trow = a.target + (size_t)b * a.R * a.V;
+    const uint16_t* drow = a.draft != nullptr ? a.draft + (size_t)b * (a.R - 1) * a.V : nullptr;
+    int dtoken = -1;
+    float dp = 0.0f, dq = 0.0f, du = 0.0f;
+    if (tid < n) {  // (in flight while the rows are joined)
+        dtoken = a.tokens[(size_t)b * (a.R - 1) + tid];
+        du = a.uniforms[(size_t)b * a.R + tid];
+        if (dtoken >= 0 && dtoken < a.V) {
+            dp = bf16f(trow[(size_t)tid * a.V + dtoken]);
+            if (drow != nullptr) dq = bf16f(drow[(size_t)tid * a.V + dtoken]);
+        }
+    }
 
-    // the rows' maxima and sums, a wave per row: rows 0 .. n of the target, n of the drafter
-    const int nrows = n + 1 + (a.draft != nullptr ? n : 0);
-    for (int k = wave; k < nrows; k += VF_NT / 64) {
-        const VfStat* s = stats + (size_t)(k <= n ? k : a.R + k - n - 1) * a.chunks;
-        float M = -__builtin_inff();
-        int arg = 0x7fffffff;
-        for (int x = lane; x < a.chunks; x += 64) {
+    // the rows' maxima and sums: rows 0 .. n of the target, n of the drafter; a wave
+    // has up to RPW rows, a lane every 64th chunk, the first of which is loaded
+    // for all of them at once
+    const int nrows = n + 1 + (drow != nullptr ? n : 0);
+    auto row_stats = [&](int k) { return stats + (size_t)(k <= n ? k : a.R + k - n - 1) * a.chunks; };
+    VfStat head[RPW];
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+        const int k = wave + i * W;
+        head[i] = VfStat{0.0, -__builtin_inff(), 0x7fffffff};
+        if (k < nrows && lane < a.chunks) head[i] = row_stats(k)[lane];
+    }
+#pragma unroll
+    for (int i = 0; i < RPW; ++i) {
+        const int k = wave + i * W;
+        if (k >= nrows) break;
+        const VfStat* s = row_stats(k);
+        float M = head[i].max;
+        int arg = head[i].max > -__builtin_inff() ? head[i].arg : 0x7fffffff;
+        for (int x = lane + 64; x < a.chunks; x += 64) {
             const VfStat v = s[x];
             if (v.max > M) {  // (chunks in index order: the first of equal ones stays)
                 M = v.max;
@@ -200,8 +257,8 @@ verify_select_kernel(VerifyArgs a) {
                 arg = oa;
             }
         }
-        double z = 0.0;
-        for (int x = lane; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, iT);
+        double z = head[i].sum * vf_exp(head[i].max, M, iT);
+        for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, iT);
         z = wave_sum(z);
         if (lane == 0) {
             VfRow r;
@@ -215,16 +272,13 @@ verify_select_kernel(VerifyArgs a) {
         }
     }
     __syncthreads();
-    const uint16_t* trow = a.target + (size_t)b * a.R * a.V;
-    const uint16_t* drow = a.draft != nullptr ? a.draft + (size_t)b * (a.R - 1) * a.V : nullptr;
     if (tid < n) {
-        const int d = a.tokens[(size_t)b * (a.R - 1) + tid];
         double p = 0.0, q = 1.0;
-        if (d >= 0 && d < a.V) {
-            p = rows[tid].weight(bf16f(trow[(size_t)tid * a.V + d]), d);
-            if (drow != nullptr) q = rows[n + 1 + tid].weight(bf16f(drow[(size_t)tid * a.V + d]), d);
+        if (dtoken >= 0 && dtoken < a.V) {
+            p = rows[tid].weight(dp, dtoken);
+            if (drow != nullptr) q = rows[n + 1 + tid].weight(dq, dtoken);
         }
-        taken[tid] = (double)a.uniforms[(size_t)b * a.R + tid] * q < p;
+        taken[tid] = (double)du * q < p;
         if (c == 0 && a.ratios != nullptr)
             a.ratios[(size_t)b * (a.R - 1) + tid] = p > 0.0 ? (float)fmin(1.0, p / q) : 0.0f;
     } else if (c == 0 && a.ratios != nullptr && tid < a.R - 1) {
@@ -236,19 +290,21 @@ verify_select_kernel(VerifyArgs a) {
     const VfRow pr = rows[r];
     const bool less = r < n;  // a rejected token: what the drafter gave is taken away
     const bool point = less && drow == nullptr;
+    const bool alone = !less || point;
+    if (alone && c != 0) return;
     const int dtok = less ? a.tokens[(size_t)b * (a.R - 1) + r] : -1;
     VfRow qr = pr;
     if (less && drow != nullptr) qr = rows[n + 1 + r];
     const uint16_t* prow = trow + (size_t)r * a.V;
     const uint16_t* qrow = less && drow != nullptr ? drow + (size_t)r * a.V : nullptr;
 
-    // weights of 16 consecutive tokens; plain: the target's own
+    // weights of consecutive tokens; plain: the target's own
     auto weights = [&](int j, bool plain, double* w) {
-        float l[VF_PT], ld[VF_PT];
-        vf_load<VEC>(prow, j, a.V, l);
-        if (!plain && qrow != nullptr) vf_load<VEC>(qrow, j, a.V, ld);
+        float l[VS_PT], ld[VS_PT];
+        vf_load<VEC, VS_PT>(prow, j, a.V, l);
+        if (!plain && qrow != nullptr) vf_load<VEC, VS_PT>(qrow, j, a.V, ld);
 #pragma unroll
-        for (int k = 0; k < VF_PT; ++k) {
+        for (int k = 0; k < VS_PT; ++k) {
             double v = j + k < a.V ? pr.weight(l[k], j + k) : 0.0;
             if (!plain && less && j + k < a.V) {
                 const double q = point ? (j + k == dtok ? 1.0 : 0.0) : qr.weight(ld[k], j + k);
@@ -257,29 +313,39 @@ verify_select_kernel(VerifyArgs a) {
             w[k] = v;
         }
     };
-    double w[VF_PT], sum = 0.0;
-    weights(c * VF_CHUNK + tid * VF_PT, false, w);
-#pragma unroll
-    for (int k = 0; k < VF_PT; ++k) sum += w[k];
-    sum = wg_sum(sum, red);
+    double w[VS_PT], sum = 0.0;
     double* sums = a.sums + (size_t)b * a.chunks;
-    if (tid == 0) {
-        sums[c] = sum;
-        __threadfence();
-        const unsigned old = __hip_atomic_fetch_add(a.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        last_part = old == (unsigned)(a.chunks - 1);
-        if (last_part) __hip_atomic_store(a.cnt + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    double without = 0.0;  // the sum of the rejected token's chunk without it
+    const int dchunk = point && dtok >= 0 && dtok < a.V ? dtok / VF_CHUNK : -1;
+    if (!alone || dchunk >= 0) {
+        weights((alone ? dchunk : c) * VF_CHUNK + tid * VS_PT, false, w);
+#pragma unroll
+        for (int k = 0; k < VS_PT; ++k) sum += w[k];
+        without = wg_sum<VS_NT>(sum, red);
     }
-    __syncthreads();
-    if (!last_part) return;
-    __threadfence();
+    if (!alone) {
+        // written through to where every XCD sees it, and counted once it is there
+        if (tid == 0) {
+            __hip_atomic_store((unsigned long long*)sums + c, (unsigned long long)__double_as_longlong(without), __ATOMIC_RELAXED,
+                               __HIP_MEMORY_SCOPE_AGENT);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            const unsigned old = __hip_atomic_fetch_add(a.cnt + b, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            last_part = old == (unsigned)(a.chunks - 1);
+            if (last_part) __hip_atomic_store(a.cnt + b, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        __syncthreads();
+        if (!last_part) return;
+    }
 
     // the chunk: threads hold consecutive runs of chunk sums
-    const int run = (a.chunks + VF_NT - 1) / VF_NT, x0 = min(tid * run, a.chunks), x1 = min(x0 + run, a.chunks);
+    const int run = (a.chunks + VS_NT - 1) / VS_NT, x0 = min(tid * run, a.chunks), x1 = min(x0 + run, a.chunks);
     bool plain = false;
     double mine = 0.0, scan = 0.0, total = 0.0;
     auto chunk_sum = [&](int x) {
-        if (!plain) return sums[x];
+        if (!plain && !alone)
+            return __longlong_as_double((long long)__hip_atomic_load((unsigned long long*)sums + x, __ATOMIC_RELAXED,
+                                                                     __HIP_MEMORY_SCOPE_AGENT));
+        if (!plain && x == dchunk) return without;
         const VfStat v = stats[(size_t)r * a.chunks + x];
         if (pr.one) return pr.arg / VF_CHUNK == x ? 1.0 : 0.0;
         return v.sum * vf_exp(v.max, pr.M, iT) * pr.iz;
@@ -289,7 +355,7 @@ verify_select_kernel(VerifyArgs a) {
         for (int x = x0; x < x1; ++x) mine += chunk_sum(x);
         scan = wg_scan(mine, red);
         __syncthreads();
-        if (tid == VF_NT - 1) before = scan;
+        if (tid == VS_NT - 1) before = scan;
         __syncthreads();
         total = before;
         if (total > 0.0) break;
@@ -316,6 +382,7 @@ verify_select_kernel(VerifyArgs a) {
             }
         }
     } else {  // u * total rounded up to the total: the last chunk with a weight
+        __syncthreads();
         if (tid == 0) pick = -1;
         __syncthreads();
         int lastx = -1;
@@ -332,12 +399,12 @@ verify_select_kernel(VerifyArgs a) {
     __syncthreads();
     const int ch = last_part;
     const double base = before;
-    const int j0 = ch * VF_CHUNK + tid * VF_PT;
+    const int j0 = ch * VF_CHUNK + tid * VS_PT;
     weights(j0, plain, w);
     sum = 0.0;
     int mylast = -1;
 #pragma unroll
-    for (int k = 0; k < VF_PT; ++k) {
+    for (int k = 0; k < VS_PT; ++k) {
         sum += w[k];
         if (w[k] > 0.0) mylast = j0 + k;
     }
@@ -351,7 +418,7 @@ verify_select_kernel(VerifyArgs a) {
         double acc = scan - sum;
         int j = mylast;
 #pragma unroll
-        for (int k = 0; k < VF_PT; ++k) {
+        for (int k = 0; k < VS_PT; ++k) {
             acc += w[k];
             if (w[k] > 0.0 && acc > goal && j0 + k < j) j = j0 + k;
         }
@@ -424,6 +491,6 @@ extern "C" int viper_hip_verify_draft(const void* target_bf16, const void* draft
     const int rc = status_of(hipGetLastError());
     if (rc != VIPER_OK) return rc;
     launch(vec ? (const void*)verify_select_kernel<true> : (const void*)verify_select_kernel<false>,
-           (unsigned)B * (unsigned)a.chunks, VF_NT, 0, (hipStream_t)stream, args);
+           (unsigned)B * (unsigned)a.chunks, VS_NT, 0, (hipStream_t)stream, args);
     return status_of(hipGetLastError());
 }

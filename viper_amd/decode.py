@@ -19,6 +19,8 @@ import math
 from dataclasses import dataclass, field
 from typing import Any, Optional
 
+import torch
+
 from .qlinear import Status, StatusCode, _status, lib, ptr
 
 
@@ -67,12 +69,13 @@ class KVCache:
         self._c = _CCache(int(self.kv_type), self.kv_heads, self.head_dim, self.page_size, self.num_pages, ptr(self.k, size),
                           ptr(self.v, size), ptr(self.k_scales, 4), ptr(self.v_scales, 4))
         self._ref = C.addressof(self._c)
-        self.device = self.k.device
+        self._dev = self.k.get_device()
+        self._width = self.kv_heads * self.head_dim
+        self._scale = 1.0 / math.sqrt(self.head_dim)
 
     @classmethod
     def empty(cls, kv_type, num_pages, page_size, kv_heads, head_dim, device="cuda"):
         """A cache of zeroed pages."""
-        import torch
         i8 = int(kv_type) == KVType.INT8
         shape = (num_pages, kv_heads, page_size // 32, 32 * head_dim)
         pool = lambda: torch.zeros(shape, dtype=torch.int8 if i8 else torch.bfloat16, device=device)
@@ -105,17 +108,23 @@ class KVBatch:
             if t is not None and (t.is_floating_point() or t.element_size() != 4):
                 raise ValueError("KVBatch: int32 arrays")
         _one_device(self.block_table, self.seq_lens, self.row_offsets)
-        self._c = _CBatch(self.batch, self.max_rows, self.total_rows or 0, self.block_table.shape[1], ptr(self.block_table, 4),
-                          ptr(self.seq_lens, 4), ptr(self.row_offsets, 4))
-        self._ref = C.addressof(self._c)
-        self.device = self.seq_lens.device
+        self._views = {}  # C views by the number of rows
+        self._ref = self._view(self.total_rows or 0)
+        self._dev = self.seq_lens.get_device()
 
-    def _rows(self, n):
+    def _rows(self, n, dev):
         """The C view for row tensors of n rows; None where they do not fit."""
+        if dev != self._dev:
+            raise ValueError("viper_amd: tensors on more than one device")
         if self.total_rows is not None:
             return self._ref if n == self.total_rows else None
-        self._c.total_rows = n
-        return self._ref
+        v = self._views.get(n)
+        return C.addressof(v) if v is not None else self._view(n)
+
+    def _view(self, n):
+        v = _CBatch(self.batch, self.max_rows, n, self.block_table.shape[1], ptr(self.block_table, 4), ptr(self.seq_lens, 4),
+                    ptr(self.row_offsets, 4))
+        return C.addressof(self._views.setdefault(n, v))
 
 
 def _one_device(*tensors):
@@ -124,33 +133,58 @@ def _one_device(*tensors):
         raise ValueError("viper_amd: tensors on more than one device")
 
 
-def _row_view(t, width):
-    """(address, row stride in elements, rows) of a bf16 tensor of rows of `width` values: [rows, width] or [rows, heads,
-    head_dim], each row dense, rows any multiple of 8 elements apart (columns of a wider matrix)."""
-    if not t.is_cuda:
-        raise ValueError("viper_amd: tensor arguments must be GPU tensors")
+def _row_view(t, width, dev):
+    """(address, row stride in elements, rows) of a bf16 tensor of rows of `width` values on device number dev: [rows, width]
+    or [rows, heads, head_dim], each row dense, rows any multiple of 8 elements apart (columns of a wider matrix)."""
+    if t.get_device() != dev:
+        raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
     if t.element_size() != 2:
         raise ValueError(f"viper_amd: expected 2-byte elements, got {t.dtype}")
-    s = t.stride()
-    if t.dim() < 2 or t.shape[-1] * (t.shape[1] if t.dim() == 3 else 1) != width or t.dim() > 3 or s[-1] != 1 or \
-            (t.dim() == 3 and t.shape[1] > 1 and s[1] != t.shape[2]):
-        raise ValueError(f"viper_amd: expected rows of {width} dense values, got {tuple(t.shape)} strides {s}")
-    rows = t.shape[0]
-    return t.data_ptr(), s[0] if rows > 1 else max(width, s[0] if s[0] % 8 == 0 else width), rows
+    shape, s = t.shape, t.stride()
+    if len(s) == 2:
+        fine = shape[1] == width and s[1] == 1
+    else:
+        fine = len(s) == 3 and shape[1] * shape[2] == width and s[2] == 1 and (shape[1] == 1 or s[1] == shape[2])
+    if not fine:
+        raise ValueError(f"viper_amd: expected rows of {width} dense values, got {tuple(shape)} strides {s}")
+    rows, stride = shape[0], s[0]
+    if rows == 1 and (stride < width or stride % 8):
+        stride = width
+    return t.data_ptr(), stride, rows
 
 
-def _call(fn, what, device, stream, *args) -> Status:
-    """The launch on the tensors' device, on `stream` or that device's current one."""
-    import torch
-    if stream is None or not isinstance(stream, int):
-        if stream is not None and stream.device != device:
+def _row_width(t):
+    return t.shape[-1] if t.dim() == 2 else t.shape[-1] * t.shape[1]
+
+
+def _flat(t, size, dev, what):
+    """Address of a dense tensor of elements of `size` bytes on device number dev."""
+    if t is None:
+        return None
+    if t.get_device() != dev:
+        raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
+    if not t.is_contiguous():
+        raise ValueError("viper_amd: tensor arguments must be contiguous")
+    if t.element_size() != size:
+        raise ValueError(f"viper_amd: {what}: expected {size}-byte elements, got {t.dtype}")
+    return t.data_ptr()
+
+
+def _call(fn, what, dev, stream, *args) -> Status:
+    """The launch on device number dev, on `stream` or that device's current one."""
+    if stream is not None and not isinstance(stream, int):
+        if stream.device.index != dev:
             return Status(StatusCode.INVALID_ARGUMENT, f"{what}: the stream is on another device")
-        if device.index != torch.cuda.current_device():
-            with torch.cuda.device(device):
-                st = torch.cuda.current_stream() if stream is None else stream
-                return _status(fn(*args, st.cuda_stream), what)
-        stream = (torch.cuda.current_stream() if stream is None else stream).cuda_stream
-    return _status(fn(*args, stream), what)
+        stream = stream.cuda_stream
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream().cuda_stream if stream is None else stream)
+    else:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+    return _OK if rc == 0 else _status(rc, what)
+
+
+_OK = Status()
 
 
 def _mismatch(what, text) -> Status:
@@ -164,37 +198,39 @@ def kv_append(cache: KVCache, batch: KVBatch, k, v, q=None, q_out=None, rope_the
     what = "viper_hip_kv_append"
     if (q is None) != (q_out is None):
         return _mismatch(what, "q and q_out go together")
-    width = cache.kv_heads * cache.head_dim
-    kp, ks, rows = _row_view(k, width)
-    vp, vs, vrows = _row_view(v, width)
+    dev, D = cache._dev, cache.head_dim
+    kp, ks, rows = _row_view(k, cache._width, dev)
+    vp, vs, vrows = _row_view(v, cache._width, dev)
     if rows != vrows or (rows > 1 and ks != vs):
         return _mismatch(what, "k and v are laid out alike")
-    ref = batch._rows(rows)
+    ref = batch._rows(rows, dev)
     if ref is None:
         return _mismatch(what, "the rows do not match the batch")
-    qp = qs = op = os = heads = 0
+    qp = op = None
+    qs = os = heads = 0
     if q is not None:
         if rope_theta is None:
             return Status(StatusCode.INVALID_ARGUMENT, f"{what}: q is taken for its rotation")
-        qw = q.shape[-1] * (q.shape[1] if q.dim() == 3 else 1)
-        heads = qw // cache.head_dim
-        qp, qs, qrows = _row_view(q, heads * cache.head_dim)
-        op, os, orows = _row_view(q_out, heads * cache.head_dim)
+        width = _row_width(q)
+        heads = width // D
+        if heads * D != width:
+            return _mismatch(what, "q rows are not whole heads")
+        qp, qs, qrows = _row_view(q, width, dev)
+        op, os, orows = _row_view(q_out, width, dev)
         if qrows != rows or orows != rows:
             return _mismatch(what, "q rows != k rows")
-    _one_device(cache, batch, k, v, q, q_out)
-    return _call(lib().viper_hip_kv_append, what, cache.device, stream, cache._ref, batch._ref, kp, vp, ks, qp or None, qs, heads,
-                 op or None, os, float(rope_theta or 0.0))
+    return _call(lib().viper_hip_kv_append, what, dev, stream, cache._ref, ref, kp, vp, ks, qp, qs, heads, op, os,
+                 rope_theta or 0.0)
 
 
 def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, stream=None) -> Status:
     """The batch's rows back from the cache: k_out and v_out bf16 [rows, kv_heads, head_dim]."""
     what = "viper_hip_kv_read"
-    width = cache.kv_heads * cache.head_dim
-    if k_out.numel() != v_out.numel() or k_out.numel() % width or batch._rows(k_out.numel() // width) is None:
+    dev, n = cache._dev, k_out.numel()
+    ref = batch._rows(n // cache._width, dev)
+    if v_out.numel() != n or n % cache._width or ref is None:
         return _mismatch(what, "the rows do not match the batch")
-    _one_device(cache, batch, k_out, v_out)
-    return _call(lib().viper_hip_kv_read, what, cache.device, stream, cache._ref, batch._ref, ptr(k_out, 2), ptr(v_out, 2))
+    return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, 2, dev, what), _flat(v_out, 2, dev, what))
 
 
 def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int:
@@ -208,16 +244,22 @@ def attention_paged(cache: KVCache, batch: KVBatch, q, out, scale: Optional[floa
     """out = attention of the rows q ([rows, heads * head_dim], heads a multiple of the cache's) over their sequences' pages:
     causal; with window > 0 the newest `window` tokens and the first `sinks`.  scale defaults to head_dim ** -0.5."""
     what = "viper_hip_attention_paged"
-    heads = q.shape[-1] * (q.shape[1] if q.dim() == 3 else 1) // cache.head_dim
-    qp, qs, rows = _row_view(q, heads * cache.head_dim)
-    op, os, orows = _row_view(out, heads * cache.head_dim)
-    if orows != rows or batch._rows(rows) is None:
+    dev, width = cache._dev, _row_width(q)
+    heads = width // cache.head_dim
+    if heads * cache.head_dim != width:
+        return _mismatch(what, "q rows are not whole heads")
+    qp, qs, rows = _row_view(q, width, dev)
+    op, os, orows = _row_view(out, width, dev)
+    ref = batch._rows(rows, dev)
+    if orows != rows or ref is None:
         return _mismatch(what, "the rows do not match the batch")
-    _one_device(cache, batch, q, out, workspace)
-    ws, nws = (None, 0) if workspace is None or workspace.numel() == 0 else \
-        (ptr(workspace), workspace.numel() * workspace.element_size())
-    return _call(lib().viper_hip_attention_paged, what, cache.device, stream, cache._ref, batch._ref, qp, qs, heads,
-                 1.0 / math.sqrt(cache.head_dim) if scale is None else float(scale), window, sinks, op, os, ws, nws)
+    ws, nws = None, 0
+    if workspace is not None:
+        nws = workspace.numel() * workspace.element_size()
+        if nws:
+            ws = _flat(workspace, workspace.element_size(), dev, what)
+    return _call(lib().viper_hip_attention_paged, what, dev, stream, cache._ref, ref, qp, qs, heads,
+                 cache._scale if scale is None else scale, window, sinks, op, os, ws, nws)
 
 
 def verify_workspace_bytes(B: int, R: int, V: int) -> int:
@@ -234,15 +276,17 @@ def verify_draft(target_logits, draft_tokens, uniforms, out_tokens, out_accepted
     if target_logits.dim() != 3:
         return _mismatch(what, "target_logits is [B, R, V]")
     B, R, V = target_logits.shape
-    for t, n, name in ((draft_tokens, B * (R - 1), "draft_tokens"), (uniforms, B * R, "uniforms"), (out_tokens, B * R, "out_tokens"),
-                       (out_accepted, B, "out_accepted"), (draft_logits, B * (R - 1) * V, "draft_logits"),
-                       (draft_lens, B, "draft_lens"), (temperature, B, "temperature"), (accept_probs, B * (R - 1), "accept_probs")):
-        if t is not None and t.numel() != n:
-            return _mismatch(what, f"{name} does not match target_logits")
-    _one_device(target_logits, draft_tokens, uniforms, out_tokens, out_accepted, draft_logits, draft_lens, temperature,
-                accept_probs, workspace)
-    opt = lambda t, size: None if t is None or t.numel() == 0 else ptr(t, size)
+    dev, n = target_logits.get_device(), B * (R - 1)
+    if uniforms.numel() != B * R or out_tokens.numel() != B * R or out_accepted.numel() != B:
+        return _mismatch(what, "uniforms, out_tokens or out_accepted do not match target_logits")
+    for t, size in ((draft_tokens, n), (draft_logits, n * V), (draft_lens, B), (temperature, B), (accept_probs, n)):
+        if t is not None and t.numel() != size:
+            return _mismatch(what, f"a tensor of {t.numel()} elements does not match target_logits, {size} are wanted")
+    if n == 0:  # nothing drafted: empty tensors have no address
+        draft_tokens = draft_logits = accept_probs = None
     nws = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    return _call(lib().viper_hip_verify_draft, what, target_logits.device, stream, ptr(target_logits, 2), opt(draft_logits, 2),
-                 opt(draft_tokens, 4), opt(draft_lens, 4), ptr(uniforms, 4), opt(temperature, 4), B, R, V, ptr(out_tokens, 4),
-                 ptr(out_accepted, 4), opt(accept_probs, 4), ptr(workspace), nws)
+    f = _flat
+    return _call(lib().viper_hip_verify_draft, what, dev, stream, f(target_logits, 2, dev, what), f(draft_logits, 2, dev, what),
+                 f(draft_tokens, 4, dev, what), f(draft_lens, 4, dev, what), f(uniforms, 4, dev, what), f(temperature, 4, dev, what),
+                 B, R, V, f(out_tokens, 4, dev, what), f(out_accepted, 4, dev, what), f(accept_probs, 4, dev, what),
+                 None if workspace is None else f(workspace, workspace.element_size(), dev, what), nws)
