@@ -21,9 +21,8 @@
 
 namespace vq {
 
-constexpr int VF_CHUNK = 4096;
-constexpr int VF_NT = 256, VF_PT = VF_CHUNK / VF_NT;  // verify_stats_kernel
-constexpr int VS_NT = 512, VS_PT = VF_CHUNK / VS_NT;  // verify_select_kernel
+constexpr int VF_CHUNK = 4096;  // the smaller of the two chunk sizes
+constexpr int VF_NT = 256, VS_NT = 512;  // threads of verify_stats_kernel, verify_select_kernel
 constexpr int VF_CNT = 4096;  // sequences of a call, a counter each
 
 struct VfStat {
@@ -55,34 +54,49 @@ __device__ __forceinline__ bool vf_seq(const VerifyArgs& a, int b, float& T, int
     return T >= 0.0f && T < __builtin_inff() && n >= 0 && n < a.R;
 }
 
-// N logits from index j of a row; past the row NaN, which weighs nothing
+// N logits from index j of a row, octets `step` octets apart; past the row NaN,
+// which weighs nothing
 template <bool VEC, int N>
-__device__ __forceinline__ void vf_load(const uint16_t* row, int j, int V, float* l) {
-    if constexpr (VEC) {  // rows of whole octets, 16-byte aligned
+__device__ __forceinline__ void vf_load(const uint16_t* row, int j, int step, int V, float* l) {
+    u32x4 v[N / 8];
 #pragma unroll
-        for (int h = 0; h < N / 8; ++h) {
-            u32x4 v = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            if (j + 8 * h < V) v = *(const u32x4*)(row + j + 8 * h);
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    for (int h = 0; h < N / 8; ++h) {
+        const int x = j + 8 * step * h;
+        v[h] = u32x4{0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
+        if constexpr (VEC) {  // rows of whole octets, 16-byte aligned
+            if (x < V) v[h] = *(const u32x4*)(row + x);
+        } else {
+            uint32_t w[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) l[8 * h + i] = bf16f((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+            for (int i = 0; i < 8; ++i) w[i] = x + i < V ? row[x + i] : 0xffffu;
+            v[h] = u32x4{w[0] | w[1] << 16, w[2] | w[3] << 16, w[4] | w[5] << 16, w[6] | w[7] << 16};
         }
-    } else {
+    }
 #pragma unroll
-        for (int i = 0; i < N; ++i) l[i] = j + i < V ? bf16f(row[j + i]) : __uint_as_float(0x7fc00000u);
+    for (int h = 0; h < N / 8; ++h) {
+        const uint32_t w[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) l[8 * h + i] = bf16f((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
     }
 }
 
-// e^x for x <= 0 in 64 bits: 2^n 2^f with n + f = x log2 e, |f| <= 1/2, and the
-// power series of 2^f = e^(f ln 2) to its 12th term ((ln 2 / 2)^13 / 13! =
-// 1.7e-16 is left out).  The rounding of x log2 e is off by |x| 2^-53, which
-// matters only to weights of e^x.  About 20 instructions, where the general
-// exp() with its cases takes three times as many (8 batches of full drafts: see
-// below).
-__device__ __forceinline__ double exp_neg(double x) {
-    const double y = fmax(x * 1.4426950408889634074, -1100.0), n = rint(y), f = y - n;
-    double p = 2.5678435993488196e-11;         // ln2^12 / 12!
-    p = __builtin_fma(p, f, 4.4455382718708101e-10);
+// e^((l - M) / T) in 64 bits, 1 at the maximum (also an infinite one), 0 for NaN
+// and below 2^-1000.  With y = (l - M) log2 e / T = n + f, |f| <= 1/2, it is 2^n
+// times the power series of 2^f = e^(f ln 2) to its 11th term (what is left out
+// is under (ln 2 / 2)^12 / 12! = 6.3e-15).  64-bit adds and products run at the
+// full rate, conversions, rounding and ldexp at a quarter of it: l is widened by
+// its bits (a bf16's significand fits; below the normal range it comes out under
+// 2^-126, which l - M does not show), n is the low word of y + 1.5 * 2^52 and goes
+// into the exponent.
+__device__ __forceinline__ double widen(float l) {
+    const uint32_t u = __float_as_uint(l), hi = (u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u);
+    return __longlong_as_double((long long)((unsigned long long)hi << 32));
+}
+__device__ __forceinline__ double vf_exp(float l, float M, double iT) {
+    constexpr double MAGIC = 6755399441055744.0;
+    const double y = (widen(l) - widen(M)) * iT * 1.4426950408889634074, t = y + MAGIC, f = y - (t - MAGIC);
+    const uint32_t n = (uint32_t)(unsigned long long)__double_as_longlong(t);
+    double p = 4.4455382718708101e-10;         // ln2^11 / 11!
     p = __builtin_fma(p, f, 7.0549116208011209e-09);
     p = __builtin_fma(p, f, 1.0178086009239696e-07);
     p = __builtin_fma(p, f, 1.3215486790144305e-06);
@@ -94,13 +108,8 @@ __device__ __forceinline__ double exp_neg(double x) {
     p = __builtin_fma(p, f, 2.4022650695910070e-01);
     p = __builtin_fma(p, f, 6.9314718055994531e-01);
     p = __builtin_fma(p, f, 1.0);
-    return __builtin_amdgcn_ldexp(p, (int)n);
-}
-// e^((l - M) / T): 1 at the maximum (also an infinite one), 0 for NaN
-__device__ __forceinline__ double vf_exp(float l, float M, double iT) {
-    if (l == M) return 1.0;
-    if (!(l < M)) return 0.0;
-    return exp_neg(((double)l - (double)M) * iT);
+    const double e = __longlong_as_double(__double_as_longlong(p) + (long long)((unsigned long long)n << 52));
+    return l == M ? 1.0 : l < M && y > -1000.0 ? e : 0.0;
 }
 
 // What a row's weights need: p(j) = weight(l_j, j)
@@ -115,9 +124,50 @@ struct VfRow {
     }
 };
 
+// Over the wave, every lane gets it: lane swaps within rows of 16, then the row
+// swaps (no trip through LDS, as a shuffle takes)
+template <int CTRL>
+__device__ __forceinline__ double dpp_d(double v) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+    const unsigned long long lo = (unsigned)dpp_i<CTRL>((int)(unsigned)u), hi = (unsigned)dpp_i<CTRL>((int)(unsigned)(u >> 32));
+    return __longlong_as_double((long long)(lo | hi << 32));
+}
+template <class F>
+__device__ __forceinline__ unsigned swap_rows(unsigned v, F f) {
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = f(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return f(r[0], r[1]);
+}
 __device__ __forceinline__ double wave_sum(double v) {
-    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    v += dpp_d<DPP_SWAP1>(v);
+    v += dpp_d<DPP_SWAP2>(v);
+    v += dpp_d<DPP_HALF_MIRROR>(v);
+    v += dpp_d<DPP_MIRROR>(v);
+    for (int i = 0; i < 2; ++i) {
+        const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+        const unsigned a = (unsigned)u, b = (unsigned)(u >> 32);
+        const auto lo = i == 0 ? __builtin_amdgcn_permlane16_swap(a, a, false, false) : __builtin_amdgcn_permlane32_swap(a, a, false, false);
+        const auto hi = i == 0 ? __builtin_amdgcn_permlane16_swap(b, b, false, false) : __builtin_amdgcn_permlane32_swap(b, b, false, false);
+        v = __longlong_as_double((long long)((unsigned long long)lo[0] | (unsigned long long)hi[0] << 32)) +
+            __longlong_as_double((long long)((unsigned long long)lo[1] | (unsigned long long)hi[1] << 32));
+    }
     return v;
+}
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp_f<DPP_SWAP1>(v));
+    v = fmaxf(v, dpp_f<DPP_SWAP2>(v));
+    v = fmaxf(v, dpp_f<DPP_HALF_MIRROR>(v));
+    v = fmaxf(v, dpp_f<DPP_MIRROR>(v));
+    return __uint_as_float(
+        swap_rows(__float_as_uint(v), [](unsigned a, unsigned b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+__device__ __forceinline__ int wave_min(int v) {
+    v = min(v, dpp_i<DPP_SWAP1>(v));
+    v = min(v, dpp_i<DPP_SWAP2>(v));
+    v = min(v, dpp_i<DPP_HALF_MIRROR>(v));
+    v = min(v, dpp_i<DPP_MIRROR>(v));
+    return (int)swap_rows((unsigned)v, [](unsigned a, unsigned b) { return (unsigned)min((int)a, (int)b); });
 }
 // Sum over the workgroup, in a fixed order; red holds a value per wave
 template <int NT>
@@ -146,49 +196,65 @@ __device__ __forceinline__ double wg_scan(double v, double* red) {
     return before + v;
 }
 
-template <bool VEC>
+template <bool VEC, int CH>
 __global__ void __launch_bounds__(VF_NT)
 verify_stats_kernel(VerifyArgs a) {
-    __shared__ float smax[VF_NT / 64];
-    __shared__ int sarg;
-    __shared__ double red[VF_NT / 64];
+    constexpr int PT = CH / VF_NT, W = VF_NT / 64;
+    __shared__ float smax[W];
+    __shared__ int sarg[W];
+    __shared__ double ssum[W];
     const int c = (int)blockIdx.x % a.chunks, rid = (int)blockIdx.x / a.chunks;
     const int per = a.draft != nullptr ? 2 * a.R - 1 : a.R;  // rows of a sequence
-    const int b = rid / per, i = rid % per, tid = (int)threadIdx.x;
+    const int b = rid / per, i = rid % per, tid = (int)threadIdx.x, wave = tid >> 6;
     float T;
     int n;
     if (!vf_seq(a, b, T, n)) return;
     if (i < a.R ? i > n : i - a.R >= n) return;
     const uint16_t* row = i < a.R ? a.target + ((size_t)b * a.R + i) * a.V : a.draft + ((size_t)b * (a.R - 1) + i - a.R) * a.V;
-    const int j0 = c * VF_CHUNK + tid * VF_PT;
-    float l[VF_PT];
-    vf_load<VEC, VF_PT>(row, j0, a.V, l);
+    const int j0 = c * CH + tid * 8;
+    float l[PT];
+    vf_load<VEC, PT>(row, j0, VF_NT, a.V, l);
+    // each wave by its own maximum; the waves meet at the end
     float m = -__builtin_inff();
 #pragma unroll
-    for (int k = 0; k < VF_PT; ++k) m = fmaxf(m, l[k]);
-    for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-    if ((tid & 63) == 0) smax[tid >> 6] = m;
-    if (tid == 0) sarg = 0x7fffffff;
-    __syncthreads();
-    m = fmaxf(fmaxf(smax[0], smax[1]), fmaxf(smax[2], smax[3]));
+    for (int k = 0; k < PT; ++k) m = fmaxf(m, l[k]);
+    m = wave_max(m);
     int arg = 0x7fffffff;
 #pragma unroll
-    for (int k = VF_PT - 1; k >= 0; --k)
-        if (l[k] == m) arg = j0 + k;
-    if (arg != 0x7fffffff) atomicMin(&sarg, arg);
+    for (int k = PT - 1; k >= 0; --k)
+        if (l[k] == m) arg = j0 + (k / 8) * VF_NT * 8 + k % 8;
+    arg = wave_min(arg);
     double sum = 0.0;
     if (T > 0.0f && m > -__builtin_inff()) {
         const double iT = 1.0 / (double)T;
 #pragma unroll
-        for (int k = 0; k < VF_PT; ++k) sum += vf_exp(l[k], m, iT);
+        for (int k = 0; k < PT; ++k) sum += vf_exp(l[k], m, iT);
+        sum = wave_sum(sum);
     }
-    sum = wg_sum<VF_NT>(sum, red);  // (and every thread's index)
-    if (tid == 0) a.stats[((size_t)b * (2 * a.R - 1) + i) * a.chunks + c] = VfStat{sum, m, sarg};
+    if ((tid & 63) == 0) {
+        smax[wave] = m;
+        sarg[wave] = arg;
+        ssum[wave] = sum;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        const double iT = T > 0.0f ? 1.0 / (double)T : 0.0;
+        float M = smax[0];
+        for (int w = 1; w < W; ++w) M = fmaxf(M, smax[w]);
+        double z = 0.0;
+        arg = 0x7fffffff;
+        for (int w = 0; w < W; ++w) {
+            z += ssum[w] * vf_exp(smax[w], M, iT);
+            if (smax[w] == M) arg = min(arg, sarg[w]);
+        }
+        a.stats[((size_t)b * (2 * a.R - 1) + i) * a.chunks + c] = VfStat{z, M, arg};
+    }
 }
 
-template <bool VEC>
+template <bool VEC, int CH>
 __global__ void __launch_bounds__(VS_NT)
 verify_select_kernel(VerifyArgs a) {
+    constexpr int VS_PT = CH / VS_NT;
     constexpr int W = VS_NT / 64, RPW = (2 * VIPER_QLINEAR_MAX_M + W - 1) / W;  // rows of a wave
     __shared__ VfRow rows[2 * VIPER_QLINEAR_MAX_M];
     __shared__ int taken[VIPER_QLINEAR_MAX_M];
@@ -249,14 +315,9 @@ verify_select_kernel(VerifyArgs a) {
                 arg = v.arg;
             }
         }
-        for (int off = 32; off > 0; off >>= 1) {
-            const float om = __shfl_xor(M, off, 64);
-            const int oa = __shfl_xor(arg, off, 64);
-            if (om > M || (om == M && oa < arg)) {
-                M = om;
-                arg = oa;
-            }
-        }
+        const float mine = M;
+        M = wave_max(M);
+        arg = wave_min(mine == M ? arg : 0x7fffffff);
         double z = head[i].sum * vf_exp(head[i].max, M, iT);
         for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, iT);
         z = wave_sum(z);
@@ -301,8 +362,8 @@ verify_select_kernel(VerifyArgs a) {
     // weights of consecutive tokens; plain: the target's own
     auto weights = [&](int j, bool plain, double* w) {
         float l[VS_PT], ld[VS_PT];
-        vf_load<VEC, VS_PT>(prow, j, a.V, l);
-        if (!plain && qrow != nullptr) vf_load<VEC, VS_PT>(qrow, j, a.V, ld);
+        vf_load<VEC, VS_PT>(prow, j, 1, a.V, l);
+        if (!plain && qrow != nullptr) vf_load<VEC, VS_PT>(qrow, j, 1, a.V, ld);
 #pragma unroll
         for (int k = 0; k < VS_PT; ++k) {
             double v = j + k < a.V ? pr.weight(l[k], j + k) : 0.0;
@@ -316,9 +377,9 @@ verify_select_kernel(VerifyArgs a) {
     double w[VS_PT], sum = 0.0;
     double* sums = a.sums + (size_t)b * a.chunks;
     double without = 0.0;  // the sum of the rejected token's chunk without it
-    const int dchunk = point && dtok >= 0 && dtok < a.V ? dtok / VF_CHUNK : -1;
+    const int dchunk = point && dtok >= 0 && dtok < a.V ? dtok / CH : -1;
     if (!alone || dchunk >= 0) {
-        weights((alone ? dchunk : c) * VF_CHUNK + tid * VS_PT, false, w);
+        weights((alone ? dchunk : c) * CH + tid * VS_PT, false, w);
 #pragma unroll
         for (int k = 0; k < VS_PT; ++k) sum += w[k];
         without = wg_sum<VS_NT>(sum, red);
@@ -347,7 +408,7 @@ verify_select_kernel(VerifyArgs a) {
                                                                      __HIP_MEMORY_SCOPE_AGENT));
         if (!plain && x == dchunk) return without;
         const VfStat v = stats[(size_t)r * a.chunks + x];
-        if (pr.one) return pr.arg / VF_CHUNK == x ? 1.0 : 0.0;
+        if (pr.one) return pr.arg / CH == x ? 1.0 : 0.0;
         return v.sum * vf_exp(v.max, pr.M, iT) * pr.iz;
     };
     for (int pass = 0; pass < 2; ++pass) {
@@ -399,7 +460,7 @@ verify_select_kernel(VerifyArgs a) {
     __syncthreads();
     const int ch = last_part;
     const double base = before;
-    const int j0 = ch * VF_CHUNK + tid * VS_PT;
+    const int j0 = ch * CH + tid * VS_PT;
     weights(j0, plain, w);
     sum = 0.0;
     int mylast = -1;
@@ -437,7 +498,7 @@ verify_select_kernel(VerifyArgs a) {
     if (tid == 0) a.accepted[b] = r;
 }
 
-static int64_t vf_chunks(int V) { return ((int64_t)V + VF_CHUNK - 1) / VF_CHUNK; }
+static int64_t vf_chunks(int V, int chunk = VF_CHUNK) { return ((int64_t)V + chunk - 1) / chunk; }
 static bool vf_sizes(int B, int R, int V) {
     return B > 0 && B <= VF_CNT && R > 0 && R <= VIPER_QLINEAR_MAX_M && V > 0 && V < 1 << 26 &&
            (int64_t)B * (2 * R - 1) * vf_chunks(V) <= (1 << 24) - 1;
@@ -479,18 +540,22 @@ extern "C" int viper_hip_verify_draft(const void* target_bf16, const void* draft
     a.B = B;
     a.R = R;
     a.V = V;
-    a.chunks = (int)vf_chunks(V);
+    const unsigned rows = (unsigned)B * (R > 1 && draft_bf16 != nullptr ? 2 * R - 1 : R);
+    // larger chunks where there are more of them than the GPU holds workgroups
+    const bool large = (int64_t)rows * vf_chunks(V) > 8 * device_cus();
+    a.chunks = (int)vf_chunks(V, large ? 2 * VF_CHUNK : VF_CHUNK);
     a.cnt = (unsigned*)workspace;
     a.stats = (VfStat*)((char*)workspace + VF_CNT * 4);
     a.sums = (double*)(a.stats + (size_t)B * (2 * R - 1) * a.chunks);
     const bool vec = V % 8 == 0 && !misaligned(target_bf16, 16) && !misaligned(draft_bf16, 16);
-    const unsigned rows = (unsigned)B * (a.draft != nullptr ? 2 * R - 1 : R);
     void* args[] = {&a};
-    launch(vec ? (const void*)verify_stats_kernel<true> : (const void*)verify_stats_kernel<false>, rows * (unsigned)a.chunks,
-           VF_NT, 0, (hipStream_t)stream, args);
+    const void* st = large ? (vec ? (const void*)verify_stats_kernel<true, 2 * VF_CHUNK> : (const void*)verify_stats_kernel<false, 2 * VF_CHUNK>)
+                           : (vec ? (const void*)verify_stats_kernel<true, VF_CHUNK> : (const void*)verify_stats_kernel<false, VF_CHUNK>);
+    const void* se = large ? (vec ? (const void*)verify_select_kernel<true, 2 * VF_CHUNK> : (const void*)verify_select_kernel<false, 2 * VF_CHUNK>)
+                           : (vec ? (const void*)verify_select_kernel<true, VF_CHUNK> : (const void*)verify_select_kernel<false, VF_CHUNK>);
+    launch(st, rows * (unsigned)a.chunks, VF_NT, 0, (hipStream_t)stream, args);
     const int rc = status_of(hipGetLastError());
     if (rc != VIPER_OK) return rc;
-    launch(vec ? (const void*)verify_select_kernel<true> : (const void*)verify_select_kernel<false>,
-           (unsigned)B * (unsigned)a.chunks, VS_NT, 0, (hipStream_t)stream, args);
+    launch(se, (unsigned)B * (unsigned)a.chunks, VS_NT, 0, (hipStream_t)stream, args);
     return status_of(hipGetLastError());
 }
