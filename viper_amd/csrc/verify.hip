@@ -22,7 +22,8 @@
 namespace vq {
 
 constexpr int VF_CHUNK = 4096;  // the smaller of the two chunk sizes
-constexpr int VF_NT = 256, VS_NT = 512;  // threads of verify_stats_kernel, verify_select_kernel
+constexpr int VF_NT = 256;      // threads of verify_stats_kernel
+constexpr int vs_threads(int chunk) { return chunk / 8; }  // of verify_select_kernel
 constexpr int VF_CNT = 4096;  // sequences of a call, a counter each
 
 struct VfStat {
@@ -80,47 +81,62 @@ __device__ __forceinline__ void vf_load(const uint16_t* row, int j, int step, in
     }
 }
 
-// e^((l - M) / T) in 64 bits, 1 at the maximum (also an infinite one), 0 for NaN
-// and below 2^-1000.  With y = (l - M) log2 e / T = n + f, |f| <= 1/2, it is 2^n
-// times the power series of 2^f = e^(f ln 2) to its 11th term (what is left out
-// is under (ln 2 / 2)^12 / 12! = 6.3e-15).  64-bit adds and products run at the
-// full rate, conversions, rounding and ldexp at a quarter of it: l is widened by
-// its bits (a bf16's significand fits; below the normal range it comes out under
-// 2^-126, which l - M does not show), n is the low word of y + 1.5 * 2^52 and goes
-// into the exponent.
+// e^((l - M) / T) in 64 bits: 1 at the maximum (also an infinite one), 0 for NaN
+// and below 2^-1000.  With y = 64 (l - M) log2 e / T = 64 n + k + f, |f| <= 1/2, it
+// is 2^n 2^(k/64) times the power series of 2^(f/64) to its 4th term (what is left
+// out is under (ln 2 / 128)^5 / 5! = 4e-14).  What bounds the statistics is the
+// number of instructions a logit takes (full drafts of 8 sequences, 21 million
+// logits): 64-bit adds and products run at the full rate, conversions, rounding and
+// ldexp at a quarter of it.  So l is widened by its bits (a bf16's significand
+// fits; below the normal range it comes out under 2^-126, which l - M does not show),
+// the whole part of y is the low word of y + 1.5 * 2^52, n goes into the exponent and
+// 2^(k/64) comes from a table in LDS.
+__device__ const double VF_POW2[64] = {
+    1, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
+    1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
+    1.0905077326652577, 1.1023825833078409, 1.1143867425958924, 1.1265216186082418,
+    1.1387886347566916, 1.1511892299529827, 1.1637248587775775, 1.1763969916502812,
+    1.189207115002721, 1.2021567314527031, 1.215247359980469, 1.22848053610687,
+    1.241857812073484, 1.2553807570246911, 1.2690509571917332, 1.2828700160787783,
+    1.2968395546510096, 1.3109612115247644, 1.3252366431597413, 1.3396675240533029,
+    1.3542555469368927, 1.3690024229745905, 1.383909881963832, 1.3989796725383112,
+    1.4142135623730951, 1.42961333839197, 1.4451808069770467, 1.460917794180647,
+    1.4768261459394993, 1.4929077282912648, 1.5091644275934228, 1.5255981507445384,
+    1.5422108254079407, 1.5590044002378369, 1.5759808451078865, 1.593142151342267,
+    1.6104903319492543, 1.6280274218573478, 1.6457554781539649, 1.6636765803267364,
+    1.681792830507429, 1.7001063537185235, 1.7186192981224779, 1.7373338352737062,
+    1.7562521603732995, 1.7753764925265212, 1.7947090750031072, 1.8142521755003989,
+    1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
+    1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509};
 __device__ __forceinline__ double widen(float l) {
     const uint32_t u = __float_as_uint(l), hi = (u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u);
     return __longlong_as_double((long long)((unsigned long long)hi << 32));
 }
-__device__ __forceinline__ double vf_exp(float l, float M, double iT) {
+// c = 64 log2 e / T, pow2 the table in LDS
+__device__ __forceinline__ double vf_exp(float l, float M, double c, const double* pow2) {
     constexpr double MAGIC = 6755399441055744.0;
-    const double y = (widen(l) - widen(M)) * iT * 1.4426950408889634074, t = y + MAGIC, f = y - (t - MAGIC);
+    const double y = (widen(l) - widen(M)) * c, t = y + MAGIC, f = y - (t - MAGIC);
     const uint32_t n = (uint32_t)(unsigned long long)__double_as_longlong(t);
-    double p = 4.4455382718708101e-10;         // ln2^11 / 11!
-    p = __builtin_fma(p, f, 7.0549116208011209e-09);
-    p = __builtin_fma(p, f, 1.0178086009239696e-07);
-    p = __builtin_fma(p, f, 1.3215486790144305e-06);
-    p = __builtin_fma(p, f, 1.5252733804059838e-05);
-    p = __builtin_fma(p, f, 1.5403530393381606e-04);
-    p = __builtin_fma(p, f, 1.3333558146428441e-03);
-    p = __builtin_fma(p, f, 9.6181291076284770e-03);
-    p = __builtin_fma(p, f, 5.5504108664821576e-02);
-    p = __builtin_fma(p, f, 2.4022650695910070e-01);
-    p = __builtin_fma(p, f, 6.9314718055994531e-01);
-    p = __builtin_fma(p, f, 1.0);
-    const double e = __longlong_as_double(__double_as_longlong(p) + (long long)((unsigned long long)n << 52));
-    return l == M ? 1.0 : l < M && y > -1000.0 ? e : 0.0;
+    double p = 5.7328516886404019e-10;  // (ln2 / 64)^4 / 4!
+    p = __builtin_fma(p, f, 2.1173137155464774e-07);
+    p = __builtin_fma(p, f, 5.8649049550561693e-05);
+    p = __builtin_fma(p, f, 0.010830424696249145);
+    p = __builtin_fma(p, f, 1.0) * pow2[n & 63u];
+    const double e = __longlong_as_double(__double_as_longlong(p) + (long long)((unsigned long long)(uint32_t)((int)n >> 6) << 52));
+    return l <= M && y > -64000.0 ? e : 0.0;
 }
+constexpr double VF_SCALE = 64 * 1.4426950408889634074;
+__device__ __forceinline__ double vf_c(float T) { return T > 0.0f ? VF_SCALE / (double)T : 0.0; }
 
 // What a row's weights need: p(j) = weight(l_j, j)
 struct VfRow {
-    double iz, iT;
+    double iz, c;
     float M;
     int arg;
     bool one;  // all on arg
-    __device__ __forceinline__ double weight(float l, int j) const {
+    __device__ __forceinline__ double weight(float l, int j, const double* pow2) const {
         if (one) return j == arg ? 1.0 : 0.0;
-        return vf_exp(l, M, iT) * iz;
+        return vf_exp(l, M, c, pow2) * iz;
     }
 };
 
@@ -202,7 +218,7 @@ verify_stats_kernel(VerifyArgs a) {
     constexpr int PT = CH / VF_NT, W = VF_NT / 64;
     __shared__ float smax[W];
     __shared__ int sarg[W];
-    __shared__ double ssum[W];
+    __shared__ double ssum[W], pow2[64];
     const int c = (int)blockIdx.x % a.chunks, rid = (int)blockIdx.x / a.chunks;
     const int per = a.draft != nullptr ? 2 * a.R - 1 : a.R;  // rows of a sequence
     const int b = rid / per, i = rid % per, tid = (int)threadIdx.x, wave = tid >> 6;
@@ -214,6 +230,8 @@ verify_stats_kernel(VerifyArgs a) {
     const int j0 = c * CH + tid * 8;
     float l[PT];
     vf_load<VEC, PT>(row, j0, VF_NT, a.V, l);
+    if (tid < 64) pow2[tid] = VF_POW2[tid];
+    lds_barrier();
     // each wave by its own maximum; the waves meet at the end
     float m = -__builtin_inff();
 #pragma unroll
@@ -226,9 +244,9 @@ verify_stats_kernel(VerifyArgs a) {
     arg = wave_min(arg);
     double sum = 0.0;
     if (T > 0.0f && m > -__builtin_inff()) {
-        const double iT = 1.0 / (double)T;
+        const double e = vf_c(T);
 #pragma unroll
-        for (int k = 0; k < PT; ++k) sum += vf_exp(l[k], m, iT);
+        for (int k = 0; k < PT; ++k) sum += vf_exp(l[k], m, e, pow2);
         sum = wave_sum(sum);
     }
     if ((tid & 63) == 0) {
@@ -238,13 +256,13 @@ verify_stats_kernel(VerifyArgs a) {
     }
     __syncthreads();
     if (tid == 0) {
-        const double iT = T > 0.0f ? 1.0 / (double)T : 0.0;
+        const double e = vf_c(T);
         float M = smax[0];
         for (int w = 1; w < W; ++w) M = fmaxf(M, smax[w]);
         double z = 0.0;
         arg = 0x7fffffff;
         for (int w = 0; w < W; ++w) {
-            z += ssum[w] * vf_exp(smax[w], M, iT);
+            z += ssum[w] * vf_exp(smax[w], M, e, pow2);
             if (smax[w] == M) arg = min(arg, sarg[w]);
         }
         a.stats[((size_t)b * (2 * a.R - 1) + i) * a.chunks + c] = VfStat{z, M, arg};
@@ -252,13 +270,13 @@ verify_stats_kernel(VerifyArgs a) {
 }
 
 template <bool VEC, int CH>
-__global__ void __launch_bounds__(VS_NT)
+__global__ void __launch_bounds__(vs_threads(CH))
 verify_select_kernel(VerifyArgs a) {
-    constexpr int VS_PT = CH / VS_NT;
+    constexpr int VS_NT = vs_threads(CH), VS_PT = CH / VS_NT;
     constexpr int W = VS_NT / 64, RPW = (2 * VIPER_QLINEAR_MAX_M + W - 1) / W;  // rows of a wave
     __shared__ VfRow rows[2 * VIPER_QLINEAR_MAX_M];
     __shared__ int taken[VIPER_QLINEAR_MAX_M];
-    __shared__ double red[W];
+    __shared__ double red[W], pow2[64];
     __shared__ int pick, last_part;
     __shared__ double before;
     const int c = (int)blockIdx.x % a.chunks, b = (int)blockIdx.x / a.chunks;
@@ -274,7 +292,9 @@ verify_select_kernel(VerifyArgs a) {
         }
         return;
     }
-    const double iT = T > 0.0f ? 1.0 / (double)T : 0.0;
+    const double e = vf_c(T);
+    if (tid < 64) pow2[tid] = VF_POW2[tid];
+    lds_barrier();
     const VfStat* stats = a.stats + (size_t)b * (2 * a.R - 1) * a.chunks;
     const uint16_t* trow = a.target + (size_t)b * a.R * a.V;
     const uint16_t* drow = a.draft != nullptr ? a.draft + (size_t)b * (a.R - 1) * a.V : nullptr;
@@ -318,13 +338,13 @@ verify_select_kernel(VerifyArgs a) {
         const float mine = M;
         M = wave_max(M);
         arg = wave_min(mine == M ? arg : 0x7fffffff);
-        double z = head[i].sum * vf_exp(head[i].max, M, iT);
-        for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, iT);
+        double z = head[i].sum * vf_exp(head[i].max, M, e, pow2);
+        for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, e, pow2);
         z = wave_sum(z);
         if (lane == 0) {
             VfRow r;
             r.M = M;
-            r.iT = iT;
+            r.c = e;
             r.iz = 1.0 / z;
             const bool none = !(M > -__builtin_inff());
             r.arg = none ? 0 : arg;
@@ -336,8 +356,8 @@ verify_select_kernel(VerifyArgs a) {
     if (tid < n) {
         double p = 0.0, q = 1.0;
         if (dtoken >= 0 && dtoken < a.V) {
-            p = rows[tid].weight(dp, dtoken);
-            if (drow != nullptr) q = rows[n + 1 + tid].weight(dq, dtoken);
+            p = rows[tid].weight(dp, dtoken, pow2);
+            if (drow != nullptr) q = rows[n + 1 + tid].weight(dq, dtoken, pow2);
         }
         taken[tid] = (double)du * q < p;
         if (c == 0 && a.ratios != nullptr)
@@ -366,9 +386,9 @@ verify_select_kernel(VerifyArgs a) {
         if (!plain && qrow != nullptr) vf_load<VEC, VS_PT>(qrow, j, 1, a.V, ld);
 #pragma unroll
         for (int k = 0; k < VS_PT; ++k) {
-            double v = j + k < a.V ? pr.weight(l[k], j + k) : 0.0;
+            double v = j + k < a.V ? pr.weight(l[k], j + k, pow2) : 0.0;
             if (!plain && less && j + k < a.V) {
-                const double q = point ? (j + k == dtok ? 1.0 : 0.0) : qr.weight(ld[k], j + k);
+                const double q = point ? (j + k == dtok ? 1.0 : 0.0) : qr.weight(ld[k], j + k, pow2);
                 v = fmax(v - q, 0.0);
             }
             w[k] = v;
@@ -409,7 +429,7 @@ verify_select_kernel(VerifyArgs a) {
         if (!plain && x == dchunk) return without;
         const VfStat v = stats[(size_t)r * a.chunks + x];
         if (pr.one) return pr.arg / CH == x ? 1.0 : 0.0;
-        return v.sum * vf_exp(v.max, pr.M, iT) * pr.iz;
+        return v.sum * vf_exp(v.max, pr.M, e, pow2) * pr.iz;
     };
     for (int pass = 0; pass < 2; ++pass) {
         mine = 0.0;
@@ -556,6 +576,6 @@ extern "C" int viper_hip_verify_draft(const void* target_bf16, const void* draft
     launch(st, rows * (unsigned)a.chunks, VF_NT, 0, (hipStream_t)stream, args);
     const int rc = status_of(hipGetLastError());
     if (rc != VIPER_OK) return rc;
-    launch(se, (unsigned)B * (unsigned)a.chunks, VS_NT, 0, (hipStream_t)stream, args);
+    launch(se, (unsigned)B * (unsigned)a.chunks, vs_threads(large ? 2 * VF_CHUNK : VF_CHUNK), 0, (hipStream_t)stream, args);
     return status_of(hipGetLastError());
 }
