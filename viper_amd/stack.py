@@ -4,8 +4,8 @@ A stack of `layers` weight sets applied `passes` times (the reference's
 looped 22-layer model: 44 slots, each weight set read twice), then the final
 norm, the bf16 LM head and the greedy token.  Per slot, the linear-path
 launches of the reference engine's decode step
-(include/viper/model_impl.cuh:650-728), attention itself excluded (it is not
-on this path; its output is a fixed activation):
+(include/viper/model_impl.cuh:650-728), attention itself excluded (its output
+is a fixed activation unless a context is asked for, see below):
 
     rmsnorm_quantize(x, input_ln)  -> q GEMV, fused2(k, v)
     quantize(attn)                 -> o GEMV + residual (in place on x)
@@ -26,10 +26,19 @@ quantizes h in its prologue:
 
 Device buffers are torch tensors (allocation only); every launch is a C ABI
 call on the current stream, so a whole step can be captured in a HIP graph.
+
+With `context` > 0 a step is a whole decode step: every slot has a paged
+key/value cache of that many tokens, and between the q/k/v projections and the
+o projection q and k are rotated, k and v stored and the new token attends over
+its sequence (two launches more, kv_append and attention_paged), in place of the
+fixed activation.  The sequence's length is on the device and grows by one in
+each step, a captured step's replays included; past `context` tokens results
+are NaN.
 """
 import ctypes as C
 import math
 
+from . import decode as _d
 from . import qlinear as _q
 
 Q4 = int(_q.QType.Q4_G64)
@@ -37,7 +46,8 @@ Q4 = int(_q.QType.Q4_G64)
 
 class Stack:
     def __init__(self, torch, hidden=2560, inter=10240, n_heads=20, n_kv_heads=4, head_dim=128,
-                 layers=22, passes=2, vocab=166144, seed=0x5EED0003, eps=1e-6):
+                 layers=22, passes=2, vocab=166144, seed=0x5EED0003, eps=1e-6, context=0, kv_type=_d.KVType.BF16, page_size=64,
+                 rope_theta=10000.0, window=0, sinks=0):
         self.torch = torch
         self.H, self.I = hidden, inter
         self.nQ, self.nKV = n_heads * head_dim, n_kv_heads * head_dim
@@ -114,8 +124,27 @@ class Stack:
         # MALL warming of the next slot's weights from a second stream (default priority)
         self.side = None
         self.sink = torch.zeros((1,), dtype=torch.int32, device="cuda")
+        self.context = context
+        if context:
+            pages = (context + page_size - 1) // page_size
+            self.rope_theta, self.window, self.sinks = rope_theta, window, sinks
+            self.seq_len = torch.zeros((1,), dtype=torch.int32, device="cuda")
+            table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, pages)
+            self.kv = [_d.KVCache.empty(kv_type, pages, page_size, n_kv_heads, head_dim) for _ in range(layers * passes)]
+            self.rows = _d.KVBatch(table, self.seq_len)
+            # one workspace: the slots' launches follow one another
+            nws = _d.attention_workspace_bytes(self.kv[0], self.rows, n_heads)
+            self.attn_ws = torch.zeros((max(nws, 16),), dtype=torch.uint8, device="cuda")
         L = _q.lib()
         self.L = L
+
+    def attend(self, l):
+        """Slot l's attention: q and k of self.qkv rotated, k and v stored, the row's attention left in self.attn."""
+        for st in (_d.kv_append(self.kv[l], self.rows, self.k, self.v, q=self.q, q_out=self.q, rope_theta=self.rope_theta),
+                   _d.attention_paged(self.kv[l], self.rows, self.q, self.attn, window=self.window, sinks=self.sinks,
+                                      workspace=self.attn_ws)):
+            if not st.ok():
+                raise RuntimeError(st.message)
 
     def weight_bytes_per_step(self):
         per_layer = sum(p.numel() + s.numel() * 2 for (p, s, _, _) in self.w[0])
@@ -147,7 +176,7 @@ class Stack:
 
     def attention_half(self, l, fused=True):
         """Slot l's q/k/v projections from rmsnorm(x) and the o projection of
-        the fixed attention output added into x.  Slot 0 reads the step's input
+        the attention output (fixed, or with a context computed) added into x.  Slot 0 reads the step's input
         row x0 (the embedding's output) and its o projection writes x, so a
         step needs no copy of x0 into x."""
         L, st = self.L, self.torch.cuda.current_stream().cuda_stream
@@ -159,6 +188,8 @@ class Stack:
         ln = self.ln[2 * (l % self.layers)]
         if fused:
             self._m1(2, p(xin), p(ln), [(self.wqkv[l % self.layers], self.qkv)], eps=self.eps, st=st)
+            if self.context:
+                self.attend(l)
             self._m1(0, p(self.attn), None, [(wo, x)], residual=p(xin), st=st)
             return
         self._ok(L.viper_hip_rmsnorm_quantize(p(xin), p(ln), self.eps, 1, H, 64, p(self.xn), p(self.xq),
@@ -167,6 +198,8 @@ class Stack:
                                                   p(self.q), None, st), "q")
         self._ok(L.viper_hip_qlinear_fused2_prequantized(Q4, p(wk[0]), p(wk[1]), p(wv[0]), p(wv[1]), 0, 64, nKV, H,
                                                          p(self.xq), p(self.xs), 1, p(self.k), p(self.v), st), "kv")
+        if self.context:
+            self.attend(l)
         self._ok(L.viper_hip_quantize_act(64, p(self.attn), 1, nQ, p(self.xq), p(self.xs), st), "quantize")
         self._ok(L.viper_hip_qlinear_prequantized(Q4, p(wo[0]), p(wo[1]), 0, 64, H, nQ, p(self.xq), p(self.xs), 1,
                                                   p(x), p(xin), st), "o")
@@ -224,6 +257,8 @@ class Stack:
     def _step(self, fused, prefetch=0):
         torch = self.torch
         slots = self.layers * self.passes
+        if self.context:
+            self.seq_len.add_(1)
         if prefetch:
             if self.side is None:
                 self.side = torch.cuda.Stream()
