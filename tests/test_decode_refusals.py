@@ -122,7 +122,8 @@ def verify_call(**kw):
                                  dict(B=4097), dict(R=0), dict(R=17), dict(V=0), dict(V=1 << 26), dict(ws=None), dict(nws=100),
                                  dict(ws=FAKE + 8), dict(target=FAKE + 1), dict(draft=FAKE + 1), dict(tokens=FAKE + 2),
                                  dict(lens=FAKE + 2), dict(u=FAKE + 2), dict(t=FAKE + 2), dict(out=FAKE + 2), dict(acc=FAKE + 2),
-                                 dict(probs=FAKE + 2), dict(B=4096, R=16, V=(1 << 26) - 1, nws=1 << 60)])
+                                 dict(probs=FAKE + 2), dict(B=4096, R=16, V=(1 << 26) - 1, nws=1 << 60),
+                                 dict(B=4096, R=1, V=4096 * 1024 + 1, nws=1 << 60)])
 def test_verify_refusals(bad):
     assert verify_call(**bad) == INVALID
 

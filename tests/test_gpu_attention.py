@@ -349,3 +349,83 @@ def test_a_prompt_in_chunks_then_tokens(i8):
         for j in (0, 31, 32, 74):
             want = R.rotate(R.bf16_val(x[j, heads * D:(heads + 1) * D]).astype(np.float64), j, theta)
             np.testing.assert_array_equal(R.bf16_bits(want.astype(np.float32)), R.bf16_bits(c.rows(table[0], np.array([j]), 0, True)[0]))
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("D,gqa", [(64, 1), (64, 2), (64, 3), (64, 4), (128, 1), (128, 2), (128, 3), (128, 4), (256, 1), (256, 2),
+                                   (128, 9), (256, 5)])
+def test_every_kernel_over_short_and_wide_tables(i8, D, gqa):
+    """16 rows of gqa heads: gqa groups of 16, so each number of operands; tables of few columns and of many (what decides the
+    waves of a workgroup and the parts), a length in each range of parts, one that no workgroup splits."""
+    page, rows = 64, 16
+    lens = [700, 16, 4500 if D == 64 else 1500]
+    c, table, offs, total, q, _ = setup(D, i8, page, 1, gqa, lens, rows, seed=D + gqa)
+    g = gpu_cache(c)
+    o, bound = R.attention(c, table, lens, rows, offs, q, gqa, D ** -0.5)
+    for W in (table.shape[1], 300):
+        wide = np.full((3, W), -1, np.int32)
+        wide[:, :table.shape[1]] = table
+        batch = va.KVBatch(dev(wide), dev(np.array(lens, np.int32)), rows)
+        one = va.KVBatch(dev(wide[2:]), dev(np.array(lens[2:], np.int32)), rows)
+        for b, r0, n in ((batch, 0, total), (one, 2 * rows, rows)):
+            for w in (None, workspace(g, b, gqa)):
+                out = dev(np.full((n, gqa * D), SENT))
+                assert va.attention_paged(g, b, dev(q[r0:r0 + n]), out, workspace=w).ok()
+                full = np.full((total, gqa * D), SENT)
+                full[r0:r0 + n] = back(out)
+                if n == total:
+                    check(full, o, bound, lens, rows, offs, (W, w is None))
+                else:
+                    for r in range(r0, total):
+                        off = np.abs(R.bf16_val(full[r]).reshape(gqa, D) - o[r])
+                        assert np.all(off <= bound[r]), (W, w is None, r)
+
+
+def test_a_batch_that_fills_the_gpu_by_itself():
+    """More sequences than the workspace has counters for: nothing is split, no workspace is wanted."""
+    lens = [1 + (i * 37) % 90 for i in range(1100)]
+    c, table, offs, total, q, batch = setup(64, False, 32, 2, 2, lens, 1)
+    g = gpu_cache(c)
+    assert va.attention_workspace_bytes(g, batch, 2) == 0
+    out = dev(np.full((total, 2 * 64), SENT))
+    assert va.attention_paged(g, batch, dev(q), out).ok()
+    o, bound = R.attention(c, table, lens, 1, offs, q, 2, 64 ** -0.5)
+    check(back(out), o, bound, lens, 1, offs)
+
+
+def test_sequences_that_share_pages():
+    """Two sequences with one prefix: the same pages in both rows of the table."""
+    c, table, offs, total, q, _ = setup(128, False, 64, 2, 8, [300, 300], 2)
+    table[1, :3] = table[0, :3]
+    g = gpu_cache(c)
+    batch = va.KVBatch(dev(table), dev(np.array([300, 250], np.int32)), 2)
+    out = dev(np.full((total, 8 * 128), SENT))
+    assert va.attention_paged(g, batch, dev(q), out, workspace=workspace(g, batch, 8)).ok()
+    o, bound = R.attention(c, table, [300, 250], 2, offs, q, 8, 128 ** -0.5)
+    check(back(out), o, bound, [300, 250], 2, offs)
+
+
+def test_python_refusals_and_empty_calls():
+    c, table, offs, total, q, batch = setup(128, False, 64, 2, 4, [90, 50], 1)
+    g = gpu_cache(c)
+    Q, out = dev(q), dev(np.full((2, 4 * 128), SENT))
+    S = va.StatusCode
+    assert va.attention_paged(g, batch, Q[:1], out[:1]).code == S.SHAPE_MISMATCH
+    assert va.attention_paged(g, batch, Q, out[:1]).code == S.SHAPE_MISMATCH
+    assert va.attention_paged(g, batch, dev(q[:, :200].copy()), out[:, :200]).code == S.SHAPE_MISMATCH
+    assert va.attention_paged(g, batch, Q, out, scale=0.0).code == S.INVALID_ARGUMENT
+    assert va.attention_paged(g, batch, dev(q[:, :384].copy()), dev(q[:, :384].copy())).code == S.INVALID_ARGUMENT  # 3 heads on 2
+    assert va.kv_append(g, batch, Q[:, :256], Q[:, 256:], q=Q, q_out=Q).code == S.INVALID_ARGUMENT          # no rotation
+    assert va.kv_append(g, batch, Q[:, :256], Q[:, 256:], q=Q, rope_theta=1e4).code == S.SHAPE_MISMATCH
+    for bad in (Q.cpu(), Q.float(), Q.t().contiguous().t()):
+        with pytest.raises(ValueError):
+            va.attention_paged(g, batch, bad, out)
+    with pytest.raises(AttributeError):
+        batch.seq_lens = dev(np.array([1, 2], np.int32))
+    with pytest.raises(AttributeError):
+        g.k = g.v
+    assert np.all(back(out) == SENT)
+    none = va.KVBatch(dev(table), dev(np.zeros(2, np.int32)), 1, dev(np.zeros(3, np.int32)))
+    z = torch.empty((0, 4 * 128), dtype=torch.int16, device="cuda")
+    kv = torch.empty((0, 256), dtype=torch.int16, device="cuda")
+    assert va.attention_paged(g, none, z, z).ok() and va.kv_append(g, none, kv, kv).ok() and va.kv_read(g, none, kv, kv).ok()

@@ -213,3 +213,32 @@ def test_python_refusals():
         with pytest.raises(ValueError):
             va.verify_draft(**{**ok, **bad}) if "target_logits" not in bad else va.verify_draft(
                 **{**ok, **bad, "draft_tokens": z(3, 1), "uniforms": z(3, 2, dt=torch.float32), "out_tokens": z(3, 2), "out_accepted": z(3)})
+
+
+def test_many_odd_rows():
+    """Rows of no whole octets, enough of them for the larger chunks."""
+    rng = np.random.default_rng(10)
+    for point in (False, True):
+        t, d, tokens, u = inputs(rng, 8, 16, 50257, point)
+        check(t, d, tokens, None, u, np.full(8, 0.8, np.float32))
+        check(t, d, tokens, rng.integers(0, 16, 8).astype(np.int32), u, None)
+
+
+def test_two_calls_at_once():
+    """Two streams, a workspace each."""
+    rng = np.random.default_rng(11)
+    cases = []
+    for _ in range(2):
+        t, d, tokens, u = inputs(rng, 4, 8, 40000)
+        out = torch.zeros((4, 8), dtype=torch.int32, device="cuda")
+        acc = torch.zeros((4,), dtype=torch.int32, device="cuda")
+        ws = torch.zeros((va.verify_workspace_bytes(4, 8, 40000),), dtype=torch.uint8, device="cuda")
+        cases.append((t, d, tokens, u, out, acc, ws, dev(t), dev(d), dev(tokens), dev(u), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for t, d, tokens, u, out, acc, ws, T, D, K, U, st in cases:
+            assert va.verify_draft(T, K, U, out, acc, draft_logits=D, workspace=ws, stream=st).ok()
+    torch.cuda.synchronize()
+    for t, d, tokens, u, out, acc, *_ in cases:
+        wo, wa, _ = R.verify(R.bf16_val(t).astype(np.float64), R.bf16_val(d).astype(np.float64), tokens, None, u, None)
+        assert out.tolist() == wo and acc.tolist() == wa

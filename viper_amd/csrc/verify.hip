@@ -521,7 +521,7 @@ verify_select_kernel(VerifyArgs a) {
 static int64_t vf_chunks(int V, int chunk = VF_CHUNK) { return ((int64_t)V + chunk - 1) / chunk; }
 static bool vf_sizes(int B, int R, int V) {
     return B > 0 && B <= VF_CNT && R > 0 && R <= VIPER_QLINEAR_MAX_M && V > 0 && V < 1 << 26 &&
-           (int64_t)B * (2 * R - 1) * vf_chunks(V) <= (1 << 24) - 1;
+           (int64_t)B * (2 * R - 1) * vf_chunks(V) <= 1 << 22;  // (launches stay under 2^32 threads)
 }
 static size_t vf_bytes(int B, int R, int V) {
     const size_t ch = (size_t)vf_chunks(V);

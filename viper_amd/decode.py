@@ -29,6 +29,15 @@ class KVType(enum.IntEnum):
     INT8 = 1
 
 
+class _Fixed:
+    """What a call reads is taken from the fields once, so they are not replaced afterwards (tensors change in place)."""
+
+    def __setattr__(self, name, value):
+        if "_ref" in self.__dict__ and name in self.__dataclass_fields__:
+            raise AttributeError(f"{type(self).__name__}.{name} is fixed: write into the tensor, or build another")
+        object.__setattr__(self, name, value)
+
+
 class _CCache(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("kv_type", "kv_heads", "head_dim", "page_size", "num_pages")] + \
                [(n, C.c_void_p) for n in ("k", "v", "k_scales", "v_scales")]
@@ -40,7 +49,7 @@ class _CBatch(C.Structure):
 
 
 @dataclass
-class KVCache:
+class KVCache(_Fixed):
     """Pages of keys and values of one layer: ``k`` and ``v`` bf16 or int8 tensors of num_pages * kv_heads * page_size *
     head_dim elements (their order within a page: include/viper_qlinear.h), ``k_scales`` and ``v_scales`` fp32
     [num_pages, kv_heads, page_size] for int8."""
@@ -68,10 +77,10 @@ class KVCache:
         _one_device(self.k, self.v, self.k_scales, self.v_scales)
         self._c = _CCache(int(self.kv_type), self.kv_heads, self.head_dim, self.page_size, self.num_pages, ptr(self.k, size),
                           ptr(self.v, size), ptr(self.k_scales, 4), ptr(self.v_scales, 4))
-        self._ref = C.addressof(self._c)
         self._dev = self.k.get_device()
         self._width = self.kv_heads * self.head_dim
         self._scale = 1.0 / math.sqrt(self.head_dim)
+        self._ref = C.addressof(self._c)
 
     @classmethod
     def empty(cls, kv_type, num_pages, page_size, kv_heads, head_dim, device="cuda"):
@@ -84,7 +93,7 @@ class KVCache:
 
 
 @dataclass
-class KVBatch:
+class KVBatch(_Fixed):
     """The rows of a call: ``block_table`` int32 [batch, table_width], ``seq_lens`` int32 [batch] (tokens held, the call's
     rows among them), and either ``max_rows`` rows for every sequence, or with ``row_offsets`` int32 [batch + 1] the rows
     row_offsets[b]..row_offsets[b + 1] - 1 (at most max_rows) of ``total_rows`` (default: what the row tensors hold)."""
@@ -109,8 +118,8 @@ class KVBatch:
                 raise ValueError("KVBatch: int32 arrays")
         _one_device(self.block_table, self.seq_lens, self.row_offsets)
         self._views = {}  # C views by the number of rows
-        self._ref = self._view(self.total_rows or 0)
         self._dev = self.seq_lens.get_device()
+        self._ref = self._view(self.total_rows or 0)
 
     def _rows(self, n, dev):
         """The C view for row tensors of n rows; None where they do not fit."""
@@ -206,6 +215,8 @@ def kv_append(cache: KVCache, batch: KVBatch, k, v, q=None, q_out=None, rope_the
     ref = batch._rows(rows, dev)
     if ref is None:
         return _mismatch(what, "the rows do not match the batch")
+    if rows == 0:
+        return _OK
     qp = op = None
     qs = os = heads = 0
     if q is not None:
@@ -230,6 +241,8 @@ def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, stream=None) -> Status
     ref = batch._rows(n // cache._width, dev)
     if v_out.numel() != n or n % cache._width or ref is None:
         return _mismatch(what, "the rows do not match the batch")
+    if n == 0:
+        return _OK
     return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, 2, dev, what), _flat(v_out, 2, dev, what))
 
 
@@ -253,6 +266,8 @@ def attention_paged(cache: KVCache, batch: KVBatch, q, out, scale: Optional[floa
     ref = batch._rows(rows, dev)
     if orows != rows or ref is None:
         return _mismatch(what, "the rows do not match the batch")
+    if rows == 0:
+        return _OK
     ws, nws = None, 0
     if workspace is not None:
         nws = workspace.numel() * workspace.element_size()
