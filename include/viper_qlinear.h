@@ -53,6 +53,16 @@
  *   viper_hip_sampling_greedy_split the same, each row over many workgroups that meet in a
  *                                   caller workspace (no counterpart; the reference runs one
  *                                   block per row).
+ *   viper_hip_kv_append             rope_q_k_fused with the cache's write
+ *                                   (kernels/ops/rope_kernel.cu:74-186,
+ *                                   kernels/ops/attn_decode_kernel.cu:727).
+ *   viper_hip_kv_read               no counterpart: rows of a cache back.
+ *   viper_hip_attention_paged       the decode and batch attention kernels
+ *                                   (kernels/ops/attn_decode_kernel.cu:35,155,615)
+ *                                   over a paged cache, with a window and
+ *                                   first tokens that stay visible.
+ *   viper_hip_verify_draft          no counterpart: drafted tokens against the
+ *                                   target's probabilities.
  *   viper_hip_qlinear_partials      no counterpart: the same kernels, also writing
  *                                   the exact per-group int32 dots for parity tests.
  *   viper_hip_qlinear_route         no counterpart: which kernel a call of given
