@@ -21,6 +21,12 @@
 // and the one that counts last adds them in part order, so that results do not
 // depend on which part that is.
 //
+// Measured (20 heads over 4 key heads of 128 dims, one row): 600 tokens 6.5 us, 4096 8.4,
+// 131072 45.5 (the stream alone 40.8: 6.6 TB/s); 32 sequences of 8192 85 us (6.3 TB/s), int8
+// 52; 16 rows of 2 sequences of 4100..8000 18.5 us.  Bound by the cache's stream at long
+// contexts (int8 by widening codes, 394 VALU instructions a tile against 165), by the
+// latency of one load chain and of the join at short ones.
+//
 // What a row must not see cannot reach it: masked scores are replaced (not
 // added to), places of the last tile past the length are cleared in V.  A
 // value that is not finite in V would still turn the zero weight of another row of its

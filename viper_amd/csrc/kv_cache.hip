@@ -15,6 +15,9 @@
 // v row) is D / 16 threads with octets o and o + D/16, the pair that rotation
 // mixes.  K octets are contiguous in the tile's order; V is stored token by token
 // with 2-byte stores (1-byte for int8), since 8 tokens of a dim share 16 bytes.
+// Bound by latency at a decode step's sizes (one row of 20 + 4 + 4 heads of 128: 2.7
+// us, of which 1.5 are the dispatch), by the small V stores at a batch's (512 rows of
+// 64 sequences into int8 5.9 us).
 
 #include "kv_host.h"
 
@@ -171,26 +174,34 @@ kv_append_kernel(AppendArgs a) {
     if (I8 && o == 0) a.c.vs[at * KV_TILE + t] = scale;
 }
 
-// read: a workgroup per tile of 32 tokens, head and pool (K, V).  K octets go
-// straight to their rows; V turns through LDS (8 tokens of a dim arrive together).
-// Threads follow the output rows, so that each wave stores whole lines.
+// read: a workgroup per tile of 32 tokens, pool (K, V) and head, of 64 dims two heads
+// whose loads are in flight together (a workgroup's chain of length, page and tile
+// takes longer than moving so small a tile).  K octets go straight to their rows; V turns
+// through LDS (8 tokens of a dim arrive together).  Threads follow the output rows, so
+// that each wave stores whole lines.
 struct ReadArgs {
     KvArgs c;
     uint16_t* ko;
     uint16_t* vo;
-    int tiles;  // tiles that a sequence's rows can touch
+    int tiles;   // tiles that a sequence's rows can touch
+    int groups;  // of heads
 };
+
+// (8 heads of 64 dims, int8, 18000 rows of 8 sequences: 1 head 16.2 us, 2 13.0, 4 12.6; 4 rows of
+// 16 sequences 3.1 / 3.4 / 4.3; 4 heads of 128 dims, 4096 rows of 64: 1 head 4.3, 4 7.6)
+constexpr int kr_heads(int D) { return D == 64 ? 2 : 1; }
 
 template <int D, bool I8>
 __global__ void __launch_bounds__(KA_NT)
 kv_read_kernel(ReadArgs a) {
-    constexpr int OPR = D / 8;  // octets of a row
-    __shared__ __align__(16) uint16_t lv[KV_TILE][D + 8];
+    constexpr int OPR = D / 8, HG = kr_heads(D);                 // octets of a row, heads
+    constexpr int PT = KV_TILE * OPR / KA_NT;                    // octets of a head and thread
+    __shared__ __align__(16) uint16_t lv[HG][KV_TILE][D + 8];
     int id = (int)blockIdx.x;
     const int side = id & 1;
     id >>= 1;
-    const int head = id % a.c.kvh;
-    id /= a.c.kvh;
+    const int head0 = id % a.groups * HG;
+    id /= a.groups;
     const int b = id / a.tiles;
     const KvSeq s = kv_seq(a.c, b);
     if (s.n == 0) return;
@@ -198,48 +209,72 @@ kv_read_kernel(ReadArgs a) {
     const int64_t tile0 = (p0 < 0 ? 0 : p0) / KV_TILE, tile64 = tile0 + id % a.tiles;
     if (tile64 * KV_TILE >= s.len) return;
     const int tile = (int)tile64, tid = (int)threadIdx.x;
-    const int page = kv_page(a.c, b, tile);
-    const size_t at = page < 0 ? 0 : kv_tile_at(a.c, page, head, tile), base = at * (KV_TILE * D);
-    const float* sc = side == 0 ? a.c.ks : a.c.vs;
+    const int page = kv_page_uniform(a.c, b, tile);
+    const int heads = min(HG, a.c.kvh - head0);
+    const float* scales = side == 0 ? a.c.ks : a.c.vs;
+    const void* pool = side == 0 ? a.c.k : a.c.v;
     uint16_t* out = side == 0 ? a.ko : a.vo;
-    if (side == 1 && page >= 0) {
-        // octet of dim d, tokens 8 tg .. 8 tg + 7
-        for (int i = tid; i < D * 4; i += KA_NT) {
-            const int d = i % D, tg = i / D;
+    // octet i of a thread: K (token, octet of the row), V (8 tokens, dim)
+    u32x4 x[HG][PT];
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+        if (h >= heads || page < 0) continue;
+        const size_t base = kv_tile_at(a.c, page, head0 + h, tile) * (KV_TILE * D);
+#pragma unroll
+        for (int k = 0; k < PT; ++k) {
+            const int i = tid + k * KA_NT;
+            const int e = side == 0 ? k_place<I8>(i / OPR, i % OPR) : v_place<I8>(8 * (i / D), i % D);
             if constexpr (I8) {
-                const u32x2 w = *(const u32x2*)((const int8_t*)a.c.v + base + v_place<true>(8 * tg, d));
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    lv[8 * tg + j][d] = f2bf((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * sc[at * KV_TILE + 8 * tg + j]);
+                const u32x2 w = *(const u32x2*)((const int8_t*)pool + base + e);
+                x[h][k] = u32x4{w.x, w.y, 0u, 0u};
             } else {
-                const u32x4 w = *(const u32x4*)((const uint16_t*)a.c.v + base + v_place<false>(8 * tg, d));
-                const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) lv[8 * tg + j][d] = (uint16_t)(ww[j >> 1] >> (16 * (j & 1)));
+                x[h][k] = *(const u32x4*)((const uint16_t*)pool + base + e);
             }
         }
     }
-    __syncthreads();
-    for (int i = tid; i < KV_TILE * OPR; i += KA_NT) {
-        const int t = i / OPR, c = i % OPR;
+    auto store = [&](int h, int t, int c, const u32x4& v) {
         const int64_t r = (int64_t)tile * KV_TILE + t - p0;
-        if (r < 0 || r >= s.n) continue;
-        u32x4 x = {0u, 0u, 0u, 0u};
-        if (page >= 0) {
-            if (side == 1) {
-                x = *(const u32x4*)&lv[t][8 * c];
-            } else if constexpr (I8) {
-                const u32x2 w = *(const u32x2*)((const int8_t*)a.c.k + base + k_place<true>(t, c));
-                const float f = sc[at * KV_TILE + t];
+        if (r >= 0 && r < s.n) *(u32x4*)(out + ((size_t)(s.row0 + r) * a.c.kvh + head0 + h) * D + 8 * c) = v;
+    };
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+        if (h >= heads) continue;
+        const float* sc = nullptr;
+        if (I8 && page >= 0) sc = scales + kv_tile_at(a.c, page, head0 + h, tile) * KV_TILE;
+#pragma unroll
+        for (int k = 0; k < PT; ++k) {
+            const int i = tid + k * KA_NT;
+            if (page < 0) {
+                store(h, i / OPR, i % OPR, u32x4{0u, 0u, 0u, 0u});
+                continue;
+            }
+            u32x4 v = x[h][k];
+            if constexpr (I8) {
                 float y[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) y[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * f;
-                x = to_bf16(y);
+                for (int j = 0; j < 8; ++j)
+                    y[j] = (float)(int8_t)((j < 4 ? v.x : v.y) >> (8 * (j & 3))) * (side == 0 ? sc[i / OPR] : sc[8 * (i / D) + j]);
+                v = to_bf16(y);
+            }
+            if (side == 0) {
+                store(h, i / OPR, i % OPR, v);
             } else {
-                x = *(const u32x4*)((const uint16_t*)a.c.k + base + k_place<false>(t, c));
+                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int j = 0; j < 8; ++j) lv[h][8 * (i / D) + j][i % D] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
             }
         }
-        *(u32x4*)(out + ((size_t)(s.row0 + r) * a.c.kvh + head) * D + 8 * c) = x;
+    }
+    if (side == 0 || page < 0) return;
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < HG; ++h) {
+        if (h >= heads) continue;
+#pragma unroll
+        for (int k = 0; k < PT; ++k) {
+            const int i = tid + k * KA_NT;
+            store(h, i / OPR, i % OPR, *(const u32x4*)&lv[h][i / OPR][8 * (i % OPR)]);
+        }
     }
 }
 
@@ -311,7 +346,8 @@ extern "C" int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_bat
     a.ko = (uint16_t*)k_out_bf16;
     a.vo = (uint16_t*)v_out_bf16;
     a.tiles = (batch->max_rows + KV_TILE - 2) / KV_TILE + 1;
-    const int64_t grid = (int64_t)batch->batch * a.tiles * cache->kv_heads * 2;
+    a.groups = (cache->kv_heads + kr_heads(cache->head_dim) - 1) / kr_heads(cache->head_dim);
+    const int64_t grid = (int64_t)batch->batch * a.tiles * a.groups * 2;
     if (grid > GRID_MAX) return VIPER_INVALID_ARGUMENT;
     const bool i8 = cache->kv_type == VIPER_KV_INT8;
     const void* fn = cache->head_dim == 64 ? read_fn<64>(i8) : cache->head_dim == 128 ? read_fn<128>(i8) : read_fn<256>(i8);

@@ -2,6 +2,11 @@
 // uniforms (speculative sampling): accept token d_i while u_i q_i(d_i) < p_i(d_i),
 // then draw the next token from max(p - q, 0) (or p after the last).
 //
+// Measured: 8 sequences of up to 15 drafted tokens, 166144 logits, the drafter's logits
+// too: 49 us (statistics 23-32, selection 23); one certain draft of 4 tokens, 32000 logits:
+// 17 us (4 and 12.5, the latency of the selection's steps; the tokens of an octet
+// one after the other, which is half the code, 19.9: their exponentials overlap).
+//
 // Which token comes out depends on comparisons with cumulated sums over the whole
 // vocabulary, so that a sum held in 32 bits would decide some of them by its
 // rounding (166144 terms: a few per cent of the draws of a flat row).  Weights e^((l - M) / T)
