@@ -52,7 +52,7 @@ BAD_BATCH = [dict(batch=0), dict(batch=65536, total_rows=65536), dict(max_rows=0
 def calls(c, b, **kw):
     """The status of every entry point over a cache."""
     L = va.lib()
-    a = dict(stride=512, q=FAKE, qs=2560, heads=20, theta=1e4, scale=0.1, window=0, sinks=0, out=FAKE, os=2560, ws=None, nws=0)
+    a = dict(stride=512, q=FAKE, qs=2560, heads=20, theta=1e4, scale=0.1, window=0, sinks=0, out=2 * FAKE, os=2560, ws=None, nws=0)
     a.update(kw)
     return [
         L.viper_hip_kv_append(ref(c), ref(b), FAKE, FAKE, a["stride"], a["q"], a["qs"], a["heads"], a["out"], a["os"], a["theta"],
@@ -95,6 +95,10 @@ def test_append_refusals(bad):
                                  dict(ws=FAKE + 8, nws=1 << 30)])
 def test_attention_refusals(bad):
     assert calls(cache(), batch(), **bad)[2] == INVALID
+
+
+def test_attention_in_place_is_refused():
+    assert calls(cache(), batch(), q=FAKE, out=FAKE)[2] == INVALID
 
 
 def test_attention_rows_are_a_verify_steps():

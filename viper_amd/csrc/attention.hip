@@ -81,6 +81,7 @@ extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const vipe
         return VIPER_INVALID_ARGUMENT;
     }
     if (batch->total_rows == 0) return VIPER_OK;
+    if (q_bf16 == out_bf16) return VIPER_INVALID_ARGUMENT;  // (rows may be read again after others are written)
     AttnArgs a;
     a.c = kv_args(cache, batch);
     a.q = (const uint16_t*)q_bf16;
