@@ -292,6 +292,8 @@ def verify_draft(target_logits, draft_tokens, uniforms, out_tokens, out_accepted
         return _mismatch(what, "target_logits is [B, R, V]")
     B, R, V = target_logits.shape
     dev, n = target_logits.get_device(), B * (R - 1)
+    if dev < 0:
+        raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
     if uniforms.numel() != B * R or out_tokens.numel() != B * R or out_accepted.numel() != B:
         return _mismatch(what, "uniforms, out_tokens or out_accepted do not match target_logits")
     for t, size in ((draft_tokens, n), (draft_logits, n * V), (draft_lens, B), (temperature, B), (accept_probs, n)):
