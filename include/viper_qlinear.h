@@ -549,7 +549,11 @@ int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_batch* batch
                         void* q_out_bf16, int64_t q_out_stride, double rope_theta, void* stream);
 
 /* The batch's rows (any max_rows) back from the cache, k_out and v_out
- * [total_rows][kv_heads][head_dim] bf16 (int8: bf16_RNE(code * scale)). */
+ * [total_rows][kv_heads][head_dim] bf16 (int8: bf16_RNE(code * scale)).
+ * Largest calls, with n = min(max_rows, total_rows): kv_append
+ * batch n ceil((heads + 2 kv_heads) head_dim / 4096) < 2^24 (heads 0 without q),
+ * kv_read 2 batch kv_heads (ceil((n - 1) / 32) + 1) < 2^24 (kv_heads / 2, rounded
+ * up, for 64 dims). */
 int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_batch* batch, void* k_out_bf16, void* v_out_bf16,
                       void* stream);
 

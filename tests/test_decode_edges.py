@@ -12,3 +12,20 @@ def test_verify_draft_refuses_host_tensors():
     with pytest.raises(ValueError, match="GPU"):
         va.verify_draft(z(2, 3, 100, dt=torch.bfloat16), z(2, 2), z(2, 3, dt=torch.float32), z(2, 3), z(2),
                         workspace=z(va.verify_workspace_bytes(2, 3, 100), dt=torch.uint8))
+
+
+FAKE = 0x10000  # never dereferenced: every call below fails validation first
+
+
+def test_a_bound_of_rows_that_leaves_31_bits_is_no_small_grid():
+    """max_rows = 2^31 - 1: the tiles of a sequence's rows are counted in 64 bits, and a grid too large is refused."""
+    from viper_amd.decode import _CBatch, _CCache
+    import ctypes as C
+    most = 2 ** 31 - 1
+    for D, kvh in ((128, 8), (64, 1), (256, 2)):
+        c = _CCache(0, kvh, D, 64, 8, FAKE, FAKE, None, None)
+        for batch in (4, 65535):
+            b = _CBatch(batch, most, most, 4, FAKE, FAKE, FAKE)
+            assert va.lib().viper_hip_kv_read(C.addressof(c), C.addressof(b), FAKE, FAKE, None) == 2
+            assert va.lib().viper_hip_kv_append(C.addressof(c), C.addressof(b), FAKE, FAKE, kvh * D, None, 0, 0, None, 0, 0.0,
+                                                None) == 2

@@ -289,6 +289,8 @@ static const void* read_fn(bool i8) {
 }
 
 constexpr int64_t GRID_MAX = (1 << 24) - 1;  // workgroups of 256 threads: under 2^32 threads
+// No sequence has more rows than the tensors hold: what the grid is sized by (max_rows may be any bound)
+static int rows_most(const viper_kv_batch* b) { return b->max_rows < b->total_rows ? b->max_rows : b->total_rows; }
 
 }  // namespace vq
 
@@ -324,7 +326,8 @@ extern "C" int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_b
     a.log2_theta = rope ? __builtin_log2(rope_theta) : 0.0;
     const int units = a.heads + 2 * cache->kv_heads, upb = KA_NT / (D / 16);
     a.ub = (units + upb - 1) / upb;
-    const int64_t grid = (int64_t)batch->batch * batch->max_rows * a.ub;
+    a.c.max_rows = rows_most(batch);
+    const int64_t grid = (int64_t)batch->batch * a.c.max_rows * a.ub;
     if (grid > GRID_MAX) return VIPER_INVALID_ARGUMENT;
     const bool i8 = cache->kv_type == VIPER_KV_INT8;
     const void* fn = D == 64 ? append_fn<64>(i8, rope) : D == 128 ? append_fn<128>(i8, rope) : append_fn<256>(i8, rope);
@@ -345,9 +348,11 @@ extern "C" int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_bat
     a.c = kv_args(cache, batch);
     a.ko = (uint16_t*)k_out_bf16;
     a.vo = (uint16_t*)v_out_bf16;
-    a.tiles = (batch->max_rows + KV_TILE - 2) / KV_TILE + 1;
+    a.c.max_rows = rows_most(batch);
+    const int64_t tiles = ((int64_t)a.c.max_rows + KV_TILE - 2) / KV_TILE + 1;
+    a.tiles = (int)tiles;
     a.groups = (cache->kv_heads + kr_heads(cache->head_dim) - 1) / kr_heads(cache->head_dim);
-    const int64_t grid = (int64_t)batch->batch * a.tiles * a.groups * 2;
+    const int64_t grid = (int64_t)batch->batch * tiles * a.groups * 2;
     if (grid > GRID_MAX) return VIPER_INVALID_ARGUMENT;
     const bool i8 = cache->kv_type == VIPER_KV_INT8;
     const void* fn = cache->head_dim == 64 ? read_fn<64>(i8) : cache->head_dim == 128 ? read_fn<128>(i8) : read_fn<256>(i8);
