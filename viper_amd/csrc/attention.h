@@ -225,7 +225,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, const KvSeq& sq, 
     s.lo_t = s.nsink = 0;
     if (a.window != 0) {
         const int from = max(0, s.pos0 + 1 > a.window ? s.pos0 + 1 - a.window : 0);
-        s.nsink = (min(a.sinks, from) + KV_TILE - 1) / KV_TILE;
+        s.nsink = (min(min(a.sinks, from), cap) + KV_TILE - 1) / KV_TILE;  // (a length past the table has no more tiles than it)
         s.lo_t = max(from / KV_TILE, s.nsink);
     }
     s.tiles = s.nsink + max(0, (min(s.len, cap) + KV_TILE - 1) / KV_TILE - s.lo_t);
