@@ -41,3 +41,67 @@ def test_lengths_past_the_table_walk_no_more_than_the_table(i8, ws):
             print(f"length {n} window {window} sinks {sinks}", flush=True)
             assert took_us(lambda: va.attention_paged(g, batch, Q, out, window=window, sinks=sinks, workspace=w), 2) < 2000
             assert np.all(np.isnan(R.bf16_val(back(out))))
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("ws", [True, False])
+def test_a_poisoned_token_costs_no_second_pass(i8, ws):
+    """A row that sees a key that is not a number is NaN whatever the rest holds: nothing is read again for it."""
+    D, kvh, heads = 128, 4, 20
+    n = 65536 if ws else 8192
+    c, table, offs, total, q, batch = setup(D, i8, 256, kvh, heads, [n], 1, seed=30)
+    g = gpu_cache(c)
+    Q, out = dev(q), dev(np.full((total, heads * D), SENT))
+    w = workspace(g, batch, heads) if ws else None
+
+    def call():
+        assert va.attention_paged(g, batch, Q, out, workspace=w).ok()
+
+    clean = took_us(call)
+    assert np.all(np.isfinite(R.bf16_val(back(out))))
+    j = n - 700
+    pg, at = int(table[0, j // 256]), j % 256
+    for h in range(kvh):
+        if i8:
+            g.k_scales[c.scale_at(pg, at, h)] = float("nan")
+        else:
+            g.k[torch.from_numpy(c.places(pg, at, h, True)).cuda()] = 0x7FC0
+    poisoned = took_us(call)
+    assert np.all(np.isnan(R.bf16_val(back(out))))
+    print(f"i8={i8} ws={ws}: clean {clean:.1f} us, poisoned {poisoned:.1f} us", flush=True)
+    assert poisoned < 3 * clean + 100
+    q[:, 5] = 0x7F80  # and a query that is not finite
+    Q.copy_(dev(q))
+    assert took_us(call) < 3 * clean + 100
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("ws", [True, False])
+def test_an_infinite_value_costs_one_more_pass(i8, ws):
+    """Rows that see an infinite value are computed again, each by one workgroup; rows that see a missing page are not."""
+    D, kvh, heads = 128, 4, 20
+    n = 65536 if ws else 8192
+    c, table, offs, total, q, batch = setup(D, i8, 256, kvh, heads, [n], 1, seed=34)
+    j = n - 700
+    pg, at = int(table[0, j // 256]), j % 256
+    for h in range(kvh):
+        if i8:
+            c.vs[c.scale_at(pg, at, h)] = np.inf
+            c.v[c.places(pg, at, h, False)] = 3
+        else:
+            c.v[c.places(pg, at, h, False)] = 0x7F80
+    g = gpu_cache(c)
+    Q, out = dev(q), dev(np.full((total, heads * D), SENT))
+    w = workspace(g, batch, heads) if ws else None
+
+    def call(b=batch):
+        assert va.attention_paged(g, b, Q, out, workspace=w).ok()
+
+    us = took_us(call)
+    assert np.all(np.isinf(R.bf16_val(back(out))))
+    table[0, 1] = -1
+    missing = va.KVBatch(dev(table), dev(np.array([n], np.int32)), 1)
+    us_missing = took_us(lambda: call(missing))
+    assert np.all(np.isnan(R.bf16_val(back(out))))
+    print(f"i8={i8} ws={ws}: infinite value {us:.0f} us, missing page {us_missing:.0f} us", flush=True)
+    assert us < (8000 if ws else 2500) and us_missing < 500

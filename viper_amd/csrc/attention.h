@@ -28,9 +28,11 @@
 // latency of one load chain and of the join at short ones.
 //
 // What a row must not see cannot reach it: masked scores are replaced (not
-// added to), places of the last tile past the length are cleared in V.  A
+// added to), places of the last tile past the length are cleared in V.  So a row's
+// sum of weights is NaN only where a score that it sees is NaN or +inf, and 0 only
+// where all of them are -inf: its result is NaN then, and nothing is read again.  A
 // value that is not finite in V would still turn the zero weight of another row of its
-// tile into NaN, so rows whose result is not finite are computed again, one by
+// tile into NaN, so other rows whose result is not finite are computed again, one by
 // one, over what they see (row_again).
 #pragma once
 
@@ -73,7 +75,7 @@ constexpr int at_qt_max(int D) { return D <= 128 ? 4 : 2; }
 // Floats that one part leaves for one group of rows: sums, then {m, l} per row
 __host__ __device__ constexpr size_t at_part_floats(int D, int qt) { return (size_t)qt * 16 * (D + 2); }
 // LDS: Q's operands; then the waves' sums and {m, l}, or 40 bytes a thread to
-// join parts, or 8 a thread and 4 a wave for row_again
+// join parts, or 8 a thread and 4 a tile for row_again
 inline size_t at_lds_bytes(int D, int qt, int W, int lrows) {
     const size_t S = (size_t)at_slots(D, qt, W), a = S * lrows * (D + 4) * 4 + S * lrows * 8, b = (size_t)W * 64 * 40;
     return (size_t)qt * 16 * D * 2 + (a > b ? a : b);
@@ -114,88 +116,93 @@ struct Sight {
     }
 };
 
-// One row computed on its own over the tokens that it sees: scores and weights
-// by the thread of a token, sums by the thread of a dim.  Reached only by rows
-// whose sums are not finite (values that are not, or pages that are missing).
+// 8 values of 16 or 8 bytes
+__device__ __forceinline__ void again_bf16(const u32x4& v, float* f) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = bf16f((w[i >> 1] >> (16 * (i & 1))) & 0xffffu);
+}
+__device__ __forceinline__ void again_codes(const u32x2& v, float* f) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)((i < 4 ? v.x : v.y) >> (8 * (i & 3)));
+}
+
+// One row computed on its own over the tokens that it sees, from the maximum m and the sum
+// of weights l that the first pass found: weights by the thread of a token, sums by the
+// thread of a dim and 8 tokens.  Reached only by rows whose sums are not finite though
+// their weights are numbers: values in V that are not, seen or in a seen token's tile, and
+// missing pages (which are looked for first).  One workgroup reads the row's K and V at the
+// latency of its loads, rows side by side where the parts are joined by a launch of their own
+// (65536 tokens of 128 dims 3.6 ms), else one after the other (5 rows of 8192 tokens 0.8 ms).
 template <int D, bool I8, int NT>
 __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, const uint16_t* q, uint16_t* o,
-                                                    int p, float* lds) {
+                                                    int p, float2 ml, float* lds) {
+    constexpr int TILES = NT / KV_TILE, G = NT / D;  // tiles of a chunk of tokens; groups of threads over its octets
     const int tid = (int)threadIdx.x;
     const Sight sight{a.window, a.sinks};
     const int64_t cap = ((int64_t)a.c.width << a.c.tpl) * KV_TILE;
-    float* w = lds;            // [NT] weights of a chunk of tokens, -1: not seen
-    float* acc = lds + NT;  // [NT]
-    float* red = acc + NT;  // [waves]
-    float m = -__builtin_inff(), l = 0.0f, sum = 0.0f;
+    float* w = lds;                // [NT] weights of a chunk of tokens, -1: not seen
+    float* acc = w + NT;           // [NT]
+    int* pages = (int*)(acc + NT);  // [TILES]
+    // chunks between the first tokens and the window are skipped
+    auto between = [&](int64_t j0, int n) { return a.window != 0 && j0 >= a.sinks && j0 + n - 1 <= (int64_t)p - a.window; };
     bool bad = p >= cap;
-#pragma unroll 1
-    for (int pass = 0; pass < 2 && !bad; ++pass) {
-        for (int64_t j0 = 0; j0 <= p; j0 += NT) {
-            // chunks between the first tokens and the window
-            if (a.window != 0 && j0 >= a.sinks && j0 + NT - 1 <= (int64_t)p - a.window) continue;
-            const int64_t j64 = j0 + tid;
-            const bool in = j64 <= p && sight.sees((int)j64, p);
-            const int j = (int)(in ? j64 : p);
-            const int tile = j / KV_TILE, t = j % KV_TILE;
-            const int page = in ? kv_page(a.c, b, tile) : 0;
+    if (!bad) {
+        for (int64_t tile = tid; tile * KV_TILE <= p; tile += NT)
+            if (!between(tile * KV_TILE, KV_TILE) && kv_page(a.c, b, (int)tile) < 0) bad = true;
+    }
+    bad = __syncthreads_or(bad);
+    float sum = 0.0f;
+    for (int64_t j0 = 0; j0 <= p && !bad; j0 += NT) {
+        if (between(j0, NT)) continue;
+        const bool in = j0 + tid <= p && sight.sees((int)(j0 + tid), p);
+        float e = -1.0f;
+        if (in) {
+            const int j = (int)j0 + tid, tile = j / KV_TILE, t = j % KV_TILE;
+            const size_t at = kv_tile_at(a.c, kv_page(a.c, b, tile), head, tile), base = at * (KV_TILE * D);
             float s = 0.0f;
-            if (in && page < 0) bad = true;
-            if (in && page >= 0) {
-                const size_t at = kv_tile_at(a.c, page, head, tile), base = at * (KV_TILE * D);
-#pragma unroll 1
-                for (int c = 0; c < D / 8; ++c) {
-                    for (int e = 0; e < 8; ++e) {
-                        const float kv = I8 ? (float)((const int8_t*)a.c.k)[base + k_place<true>(t, c) + e]
-                                            : bf16f(((const uint16_t*)a.c.k)[base + k_place<false>(t, c) + e]);
-                        s = __builtin_fmaf(bf16f(q[8 * c + e]), kv, s);
-                    }
-                }
-                if (I8) s *= a.c.ks[at * KV_TILE + t];
-                s *= a.scale;
+#pragma unroll 2
+            for (int c = 0; c < D / 8; ++c) {
+                float k[8], x[8];
+                if constexpr (I8) again_codes(*(const u32x2*)((const int8_t*)a.c.k + base + k_place<true>(t, c)), k);
+                else again_bf16(*(const u32x4*)((const uint16_t*)a.c.k + base + k_place<false>(t, c)), k);
+                again_bf16(*(const u32x4*)(q + 8 * c), x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x[i], k[i], s);
             }
-            if (pass == 0) {
-                if (in) m = fmaxf(m, s);
-                continue;
-            }
-            const float e = in ? __builtin_amdgcn_exp2f(s - m) : -1.0f;
-            if (in) l += e;
-            __syncthreads();
-            w[tid] = e;
-            __syncthreads();
-            const int d = tid % D;
-#pragma unroll 1
-            for (int i = tid / D; i < NT; i += NT / D) {
-                if (w[i] == -1.0f) continue;  // (a weight is >= 0 or NaN)
-                const int jt = (int)j0 + i, tl = jt / KV_TILE, tt = jt % KV_TILE;
-                const size_t at = kv_tile_at(a.c, kv_page(a.c, b, tl), head, tl), base = at * (KV_TILE * D);
-                const float vv = I8 ? (float)((const int8_t*)a.c.v)[base + v_place<true>(tt, d)] * a.c.vs[at * KV_TILE + tt]
-                                    : bf16f(((const uint16_t*)a.c.v)[base + v_place<false>(tt, d)]);
-                sum = __builtin_fmaf(w[i], vv, sum);
-            }
-        }
-        // the maximum (first pass) and whether a page was missing, over the workgroup
-        bad = __syncthreads_or(bad);
-        if (pass == 0) {
-            for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-            if ((tid & 63) == 0) red[tid >> 6] = m;
-            __syncthreads();
-            m = red[0];
-            for (int i = 1; i < NT / 64; ++i) m = fmaxf(m, red[i]);
-        } else {
-            for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
-            if ((tid & 63) == 0) red[tid >> 6] = l;
-            acc[tid] = sum;
+            if (I8) s *= a.c.ks[at * KV_TILE + t];
+            e = __builtin_amdgcn_exp2f(s * a.scale - ml.x);
         }
         __syncthreads();
+        w[tid] = e;
+        if (tid < TILES) pages[tid] = kv_page(a.c, b, (int)min(j0 / KV_TILE + tid, (int64_t)p / KV_TILE));
+        __syncthreads();
+        const int d = tid % D;
+#pragma unroll 2
+        for (int i = tid / D; i < NT / 8; i += G) {
+            const int pg = pages[i / 4];  // (4 octets of tokens a tile)
+            if (pg < 0) continue;         // (none of its tokens is seen)
+            const size_t at = kv_tile_at(a.c, pg, head, (int)(j0 / KV_TILE) + i / 4), base = at * (KV_TILE * D);
+            float v[8];
+            if constexpr (I8) {
+                again_codes(*(const u32x2*)((const int8_t*)a.c.v + base + v_place<true>(8 * (i & 3), d)), v);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] *= a.c.vs[at * KV_TILE + 8 * (i & 3) + x];
+            } else {
+                again_bf16(*(const u32x4*)((const uint16_t*)a.c.v + base + v_place<false>(8 * (i & 3), d)), v);
+            }
+#pragma unroll
+            for (int x = 0; x < 8; ++x) sum = w[8 * i + x] == -1.0f ? sum : __builtin_fmaf(w[8 * i + x], v[x], sum);
+        }
     }
+    acc[tid] = sum;
+    __syncthreads();
     if (tid < D) {
         float v = __uint_as_float(0x7fc00000u);
         if (!bad) {
-            float lt = 0.0f;
             v = 0.0f;
             for (int i = tid; i < NT; i += D) v += acc[i];
-            for (int i = 0; i < NT / 64; ++i) lt += red[i];
-            v /= lt;
+            v /= ml.y;
         }
         o[tid] = f2bf(v);
     }
@@ -233,7 +240,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, const KvSeq& sq, 
     return s;
 }
 
-// Row rr of group qg as a result; false where it is not finite (0 * x is NaN then)
+// Row rr of group qg as a result; false where it has to be computed again: its weights are
+// numbers, the sums of its values are not finite (0 * x is NaN then)
 template <int D, int ROWS>
 __device__ __forceinline__ bool attn_store(const AttnArgs& a, const AttnSeq& s, int qg, int head, int rr, int d, at_f32x4 o,
                                            float l) {
@@ -241,16 +249,18 @@ __device__ __forceinline__ bool attn_store(const AttnArgs& a, const AttnSeq& s, 
     o = o * (1.0f / l);
     bool fine = true;
     if (s.pos0 + i < 0) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    else if (!(l > 0.0f)) o = o + __uint_as_float(0x7fc00000u);
     else fine = o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f == 0.0f;
     *(u32x2*)(a.out + (size_t)(s.sq.row0 + i) * a.out_stride + (size_t)(head * a.gqa + hh) * D + d) =
         u32x2{f2bf2(o[0], o[1]), f2bf2(o[2], o[3])};
     return fine;
 }
 template <int D, bool I8, int NT, int ROWS>
-__device__ __forceinline__ void attn_again(const AttnArgs& a, const AttnSeq& s, int b, int qg, int head, int rr, float* lds) {
+__device__ __forceinline__ void attn_again(const AttnArgs& a, const AttnSeq& s, int b, int qg, int head, int rr, float2 ml,
+                                           float* lds) {
     const int r = qg * ROWS + rr, i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
     const size_t row = (size_t)s.sq.row0 + i, h = (size_t)(head * a.gqa + hh) * D;
-    row_again<D, I8, NT>(a, b, head, a.q + row * a.q_stride + h, a.out + row * a.out_stride + h, s.pos0 + i, lds);
+    row_again<D, I8, NT>(a, b, head, a.q + row * a.q_stride + h, a.out + row * a.out_stride + h, s.pos0 + i, ml, lds);
 }
 
 // Sums of 8 values (row rr, dims d ..) over parts first, first + step, ...
@@ -295,9 +305,10 @@ __device__ __forceinline__ AttnSum attn_join(__amdgpu_buffer_rsrc_t recs, int rr
     return s;
 }
 // The groups of threads meet: thread t < 2 * units stores 4 values of unit t % units
+// and leaves the row's maximum and sum in ml
 template <int D, int ROWS>
 __device__ __forceinline__ bool attn_meet(const AttnArgs& a, const AttnSeq& s, int qg, int head, int rr0, float* lds, int NT,
-                                          int units, int G) {
+                                          int units, int G, float2& ml) {
     const at_f32x4* jo = (const at_f32x4*)lds;
     const float* jm = lds + 8 * NT;
     const int tid = (int)threadIdx.x, half = tid >= units, u = tid - half * units;
@@ -309,6 +320,7 @@ __device__ __forceinline__ bool attn_meet(const AttnArgs& a, const AttnSeq& s, i
         o += jo[half * NT + k * units + u] * f;
         l += lw == lw ? lw * f : lw;
     }
+    ml = make_float2(M, l);
     return attn_store<D, ROWS>(a, s, qg, head, rr0 + u / (D / 8), u % (D / 8) * 8 + 4 * half, o, l);
 }
 __device__ __forceinline__ void attn_lay(float* lds, int NT, const AttnSum& s) {
@@ -334,6 +346,7 @@ attn_kernel(AttnArgs a) {
     float* lml = lds + SLOTS * LR * ST;  // [SLOTS][LR][2]
     __shared__ int last_part;
     __shared__ unsigned again[(ROWS + 31) / 32];
+    __shared__ float2 again_ml[ROWS];
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
@@ -416,7 +429,7 @@ attn_kernel(AttnArgs a) {
 
     // A tile's K is asked for once the products that read the one before are
     // issued, its V likewise, its page two tiles ahead.  A tile whose page is missing
-    // reads page 0 and makes every row of the wave NaN (row_again sorts them out).
+    // reads page 0 and makes the sums of every row of the wave NaN (row_again sorts them out).
     auto page_of = [&](int v) {
         const int p = v < tiles ? kv_page_uniform(a.c, b, s.tile_of(v)) : 0;
         if (p < 0) missing = true;
@@ -561,7 +574,10 @@ attn_kernel(AttnArgs a) {
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
         l[qt] = sum_over_groups(l[qt]);
-        if (missing) l[qt] = __uint_as_float(0x7fc00000u);
+        if (missing) {
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) O[qt][db][0] = __uint_as_float(0x7fc00000u);
+        }
     }
     auto put = [&](int slot) {
 #pragma unroll
@@ -600,8 +616,12 @@ attn_kernel(AttnArgs a) {
 
     const int rec = (qg * a.c.batch + b) * a.c.kvh + head;
     constexpr int PF = (int)at_part_floats(D, QT);
-    auto store = [&](int rr, int d, at_f32x4 o, float lt) {
-        if (!attn_store<D, ROWS>(a, s, qg, head, rr, d, o, lt)) atomicOr(&again[rr >> 5], 1u << (rr & 31));
+    auto once_more = [&](int rr, float2 ml) {  // (threads of one row have the same ml)
+        again_ml[rr] = ml;
+        atomicOr(&again[rr >> 5], 1u << (rr & 31));
+    };
+    auto store = [&](int rr, int d, at_f32x4 o, float M, float lt) {
+        if (!attn_store<D, ROWS>(a, s, qg, head, rr, d, o, lt)) once_more(rr, make_float2(M, lt));
     };
     const auto recs = buf(a.part + (size_t)rec * a.splits * PF, (uint32_t)(parts * PF * 4));
     for (int i = tid; i < rows * (D / 4); i += NT) {
@@ -618,7 +638,7 @@ attn_kernel(AttnArgs a) {
             lt += lw == lw ? lw * f : lw;
         }
         if (parts == 1) {
-            store(rr, d, o, lt);
+            store(rr, d, o, M, lt);
         } else {
             bstore16<AUX_SC1>(recs, (split * PF + rr * D + d) * 4, __builtin_bit_cast(u32x4, o));
             if (d == 0)
@@ -642,23 +662,22 @@ attn_kernel(AttnArgs a) {
             const int rr = i / (D / 8), d = i % (D / 8) * 8;
             const AttnSum t = attn_join<D, ROWS>(recs, rr, d, grp, G, parts);
             if (G == 1) {
-                store(rr, d, t.o0, t.l);
-                store(rr, d + 4, t.o1, t.l);
+                store(rr, d, t.o0, t.M, t.l);
+                store(rr, d + 4, t.o1, t.M, t.l);
             } else {
                 attn_lay(lds, NT, t);
             }
         }
         if (G > 1) {
             __syncthreads();
-            if (tid < 2 * units && !attn_meet<D, ROWS>(a, s, qg, head, 0, lds, NT, units, G)) {
-                const int rr = (tid >= units ? tid - units : tid) / (D / 8);
-                atomicOr(&again[rr >> 5], 1u << (rr & 31));
-            }
+            float2 ml;
+            if (tid < 2 * units && !attn_meet<D, ROWS>(a, s, qg, head, 0, lds, NT, units, G, ml))
+                once_more((tid >= units ? tid - units : tid) / (D / 8), ml);
         }
     }
     __syncthreads();
     for (int rr = 0; rr < rows; ++rr)
-        if ((again[rr >> 5] >> (rr & 31)) & 1u) attn_again<D, I8, NT, ROWS>(a, s, b, qg, head, rr, lds);
+        if ((again[rr >> 5] >> (rr & 31)) & 1u) attn_again<D, I8, NT, ROWS>(a, s, b, qg, head, rr, again_ml[rr], lds);
 }
 
 // The join as a launch of its own: a workgroup per row and group of rows, its
@@ -670,6 +689,7 @@ attn_join_kernel(AttnArgs a) {
     constexpr int ROWS = QT * 16, U = D / 8, G = AT_JNT / U;
     __shared__ __align__(16) float lds[AT_JNT * 10];
     __shared__ int again;
+    __shared__ float2 again_ml;
     const int b = (int)blockIdx.z, rr = (int)blockIdx.x, tid = (int)threadIdx.x;
     int head = (int)blockIdx.y, qg = 0;
     if (a.qgroups > 1) {
@@ -684,9 +704,13 @@ attn_join_kernel(AttnArgs a) {
     attn_lay(lds, AT_JNT, attn_join<D, ROWS>(recs, rr, tid % U * 8, tid / U, G, s.parts));
     if (tid == 0) again = 0;
     __syncthreads();
-    if (tid < 2 * U && !attn_meet<D, ROWS>(a, s, qg, head, rr, lds, AT_JNT, U, G)) again = 1;
+    float2 ml;
+    if (tid < 2 * U && !attn_meet<D, ROWS>(a, s, qg, head, rr, lds, AT_JNT, U, G, ml)) {
+        again_ml = ml;
+        again = 1;
+    }
     __syncthreads();
-    if (again) attn_again<D, I8, AT_JNT, ROWS>(a, s, b, qg, head, rr, lds);
+    if (again) attn_again<D, I8, AT_JNT, ROWS>(a, s, b, qg, head, rr, again_ml, lds);
 }
 
 struct AttnFn {
