@@ -105,3 +105,22 @@ def test_an_infinite_value_costs_one_more_pass(i8, ws):
     assert np.all(np.isnan(R.bf16_val(back(out))))
     print(f"i8={i8} ws={ws}: infinite value {us:.0f} us, missing page {us_missing:.0f} us", flush=True)
     assert us < (8000 if ws else 2500) and us_missing < 500
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("ws", [True, False])
+def test_values_whose_sum_leaves_32_bits(i8, ws):
+    """A weighted mean of finite values is finite, also where the sum of the values is not."""
+    D, page, kvh, heads, lens, rows = 64, 32, 2, 4, [700, 33, 5], 3
+    c, table, offs, total, q, batch = setup(D, i8, page, kvh, heads, lens, rows, seed=31, std=0.3)
+    if i8:
+        c.vs[:] = np.float32(2.6e36)  # codes up to 127: 3.3e38
+        c.v[:] = np.abs(c.v)
+    else:
+        c.v[:] = R.bf16_bits(np.float32(3e38) * (1 + 0.1 * np.random.default_rng(32).uniform(-1, 1, len(c.v))).astype(np.float32))
+    g = gpu_cache(c)
+    out = dev(np.full((total, heads * D), SENT))
+    assert va.attention_paged(g, batch, dev(q), out, workspace=workspace(g, batch, heads) if ws else None).ok()
+    o, bound = R.attention(c, table, lens, rows, offs, q, heads, D ** -0.5)
+    assert all(np.isfinite(x).all() for x in o.values())
+    check(back(out), o, bound, lens, rows, offs)

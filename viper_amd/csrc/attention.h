@@ -130,10 +130,11 @@ __device__ __forceinline__ void again_codes(const u32x2& v, float* f) {
 // One row computed on its own over the tokens that it sees, from the maximum m and the sum
 // of weights l that the first pass found: weights by the thread of a token, sums by the
 // thread of a dim and 8 tokens.  Reached only by rows whose sums are not finite though
-// their weights are numbers: values in V that are not, seen or in a seen token's tile, and
-// missing pages (which are looked for first).  One workgroup reads the row's K and V at the
-// latency of its loads, rows side by side where the parts are joined by a launch of their own
-// (65536 tokens of 128 dims 3.6 ms), else one after the other (5 rows of 8192 tokens 0.8 ms).
+// their weights are numbers: values in V that are not, seen or in a seen token's tile, finite
+// ones whose sum leaves 32 bits (10^38; their mean does not), and missing pages (which are
+// looked for first).  One workgroup reads the row's K and V at the latency of its loads, rows
+// side by side where the parts are joined by a launch of their own (65536 tokens of 128 dims
+// 3.6 ms), else one after the other (5 rows of 8192 tokens 0.8 ms).
 template <int D, bool I8, int NT>
 __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, const uint16_t* q, uint16_t* o,
                                                     int p, float2 ml, float* lds) {
@@ -152,6 +153,8 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
             if (!between(tile * KV_TILE, KV_TILE) && kv_page(a.c, b, (int)tile) < 0) bad = true;
     }
     bad = __syncthreads_or(bad);
+    // (weights of the mean: a sum of them times finite values stays finite)
+    const float il = 1.0f / ml.y;
     float sum = 0.0f;
     for (int64_t j0 = 0; j0 <= p && !bad; j0 += NT) {
         if (between(j0, NT)) continue;
@@ -171,7 +174,7 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
                 for (int i = 0; i < 8; ++i) s = __builtin_fmaf(x[i], k[i], s);
             }
             if (I8) s *= a.c.ks[at * KV_TILE + t];
-            e = __builtin_amdgcn_exp2f(s * a.scale - ml.x);
+            e = __builtin_amdgcn_exp2f(s * a.scale - ml.x) * il;
         }
         __syncthreads();
         w[tid] = e;
@@ -202,7 +205,6 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
         if (!bad) {
             v = 0.0f;
             for (int i = tid; i < NT; i += D) v += acc[i];
-            v /= ml.y;
         }
         o[tid] = f2bf(v);
     }
