@@ -588,8 +588,10 @@ int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch*
  * out_tokens [B][R]: the accepted tokens, the next one, then -1; out_accepted
  * [B]: how many were accepted.  accept_probs (fp32 [B][R-1], may be NULL):
  * min(1, p_i(d_i) / q_i(d_i)), 0 past draft_lens.  uniforms fp32 [B][R] in
- * [0, 1).  Weights and sums in 64 bits.  NaN logits weigh nothing, a row with
- * nothing above -inf gives token 0, infinite logits share the mass.  R = 1
+ * [0, 1).  Weights (each to 4e-14 of itself) and sums are 64-bit.  NaN logits weigh
+ * nothing, and -inf at no temperature; a row with nothing above -inf gives token
+ * 0; infinite logits share the mass, none of which is left to finite ones.
+ * Temperatures above 0 and under 2^-120 count as 2^-120.  R = 1
  * samples (draft_tokens may be NULL).  A draft token outside the vocabulary is
  * rejected; a temperature that is negative or not finite, or a draft_lens[b]
  * outside 0 .. R - 1, makes out_accepted[b] and the sequence's tokens -1.

@@ -86,15 +86,15 @@ __device__ __forceinline__ void vf_load(const uint16_t* row, int j, int step, in
     }
 }
 
-// e^((l - M) / T) in 64 bits: 1 at the maximum (also an infinite one), 0 for NaN
-// and below 2^-1000.  With y = 64 (l - M) log2 e / T = 64 n + k + f, |f| <= 1/2, it
+// e^((l - M) / T): 1 at the maximum (also an infinite one), 0 for NaN, for what is
+// infinitely far below the maximum at any T, and below 2^-1000.  With y = 64 (l - M) log2 e / T = 64 n + k + f, |f| <= 1/2, it
 // is 2^n 2^(k/64) times the power series of 2^(f/64) to its 4th term (what is left
 // out is under (ln 2 / 128)^5 / 5! = 4e-14).  What bounds the statistics is the
 // number of instructions a logit takes (full drafts of 8 sequences, 21 million
 // logits): 64-bit adds and products run at the full rate, conversions, rounding and
-// ldexp at a quarter of it.  So l is widened by its bits (a bf16's significand
-// fits; below the normal range it comes out under 2^-126, which l - M does not show),
-// the whole part of y is the low word of y + 1.5 * 2^52, n goes into the exponent and
+// ldexp at a quarter of it.  So l is widened by its bits: placed in a double they
+// read as 2^-896 l, exactly, below the normal range too (an infinite l as 2^128, which
+// vf_floor takes care of), and 2^896 goes into the factor; the whole part of y is the low word of y + 1.5 * 2^52, n goes into the exponent and
 // 2^(k/64) comes from a table in LDS.
 __device__ const double VF_POW2[64] = {
     1, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
@@ -114,11 +114,31 @@ __device__ const double VF_POW2[64] = {
     1.8340080864093424, 1.8539791250833855, 1.8741676341103, 1.8945759815869656,
     1.9152065613971474, 1.9360617934922943, 1.9571441241754002, 1.9784560263879509};
 __device__ __forceinline__ double widen(float l) {
-    const uint32_t u = __float_as_uint(l), hi = (u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u);
+    const uint32_t u = __float_as_uint(l), hi = (u & 0x80000000u) | ((u & 0x7fffffffu) >> 3);
     return __longlong_as_double((long long)((unsigned long long)hi << 32));
 }
-// c = 64 log2 e / T, pow2 the table in LDS
-__device__ __forceinline__ double vf_exp(float l, float M, double c, const double* pow2) {
+// 2^896 64 log2 e / T.  It fits in 64 bits down to T = 2^-121; below 2^-120 (what
+// only logits under 10^-34 tell apart) that is taken.
+__device__ __forceinline__ double vf_c(float T) {
+    constexpr double SCALE = 0x1p896 * 64 * 1.4426950408889634074;
+    return T > 0.0f ? SCALE / fmax((double)T, 0x1p-120) : 0.0;
+}
+// The y above which a logit weighs: 2^-1000, or at temperatures where that lies
+// further down, what separates -inf from the finite ones, and these from +inf
+__device__ __forceinline__ double vf_floor(float M, double c) {
+    const double inf = widen(__builtin_inff());
+    const double gap = M == __builtin_inff() ? 0x1p-776 : inf + widen(M);  // (2^120 is the step below 2^128)
+    return fmax(-64000.0, -gap * c);
+}
+// A value that all lanes have, in scalar registers
+__device__ __forceinline__ double wave_uniform(double v) {
+    const unsigned long long u = (unsigned long long)__double_as_longlong(v);
+    const unsigned lo = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)u);
+    const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
+    return __longlong_as_double((long long)(lo | (unsigned long long)hi << 32));
+}
+// c = vf_c(T), lo = vf_floor(M, c), pow2 the table in LDS
+__device__ __forceinline__ double vf_exp(float l, float M, double c, double lo, const double* pow2) {
     constexpr double MAGIC = 6755399441055744.0;
     const double y = (widen(l) - widen(M)) * c, t = y + MAGIC, f = y - (t - MAGIC);
     const uint32_t n = (uint32_t)(unsigned long long)__double_as_longlong(t);
@@ -128,20 +148,18 @@ __device__ __forceinline__ double vf_exp(float l, float M, double c, const doubl
     p = __builtin_fma(p, f, 0.010830424696249145);
     p = __builtin_fma(p, f, 1.0) * pow2[n & 63u];
     const double e = __longlong_as_double(__double_as_longlong(p) + (long long)((unsigned long long)(uint32_t)((int)n >> 6) << 52));
-    return l <= M && y > -64000.0 ? e : 0.0;
+    return l <= M && y > lo ? e : 0.0;
 }
-constexpr double VF_SCALE = 64 * 1.4426950408889634074;
-__device__ __forceinline__ double vf_c(float T) { return T > 0.0f ? VF_SCALE / (double)T : 0.0; }
 
 // What a row's weights need: p(j) = weight(l_j, j)
 struct VfRow {
-    double iz, c;
+    double iz, c, lo;
     float M;
     int arg;
     bool one;  // all on arg
     __device__ __forceinline__ double weight(float l, int j, const double* pow2) const {
         if (one) return j == arg ? 1.0 : 0.0;
-        return vf_exp(l, M, c, pow2) * iz;
+        return vf_exp(l, M, c, lo, pow2) * iz;
     }
 };
 
@@ -249,9 +267,9 @@ verify_stats_kernel(VerifyArgs a) {
     arg = wave_min(arg);
     double sum = 0.0;
     if (T > 0.0f && m > -__builtin_inff()) {
-        const double e = vf_c(T);
+        const double e = vf_c(T), lo = wave_uniform(vf_floor(m, e));
 #pragma unroll
-        for (int k = 0; k < PT; ++k) sum += vf_exp(l[k], m, e, pow2);
+        for (int k = 0; k < PT; ++k) sum += vf_exp(l[k], m, e, lo, pow2);
         sum = wave_sum(sum);
     }
     if ((tid & 63) == 0) {
@@ -264,10 +282,11 @@ verify_stats_kernel(VerifyArgs a) {
         const double e = vf_c(T);
         float M = smax[0];
         for (int w = 1; w < W; ++w) M = fmaxf(M, smax[w]);
+        const double lo = vf_floor(M, e);
         double z = 0.0;
         arg = 0x7fffffff;
         for (int w = 0; w < W; ++w) {
-            z += ssum[w] * vf_exp(smax[w], M, e, pow2);
+            z += ssum[w] * vf_exp(smax[w], M, e, lo, pow2);
             if (smax[w] == M) arg = min(arg, sarg[w]);
         }
         a.stats[((size_t)b * (2 * a.R - 1) + i) * a.chunks + c] = VfStat{z, M, arg};
@@ -343,13 +362,15 @@ verify_select_kernel(VerifyArgs a) {
         const float mine = M;
         M = wave_max(M);
         arg = wave_min(mine == M ? arg : 0x7fffffff);
-        double z = head[i].sum * vf_exp(head[i].max, M, e, pow2);
-        for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, e, pow2);
+        const double lo = vf_floor(M, e);
+        double z = head[i].sum * vf_exp(head[i].max, M, e, lo, pow2);
+        for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, e, lo, pow2);
         z = wave_sum(z);
         if (lane == 0) {
             VfRow r;
             r.M = M;
             r.c = e;
+            r.lo = lo;
             r.iz = 1.0 / z;
             const bool none = !(M > -__builtin_inff());
             r.arg = none ? 0 : arg;
@@ -373,14 +394,18 @@ verify_select_kernel(VerifyArgs a) {
     __syncthreads();
     int r = 0;  // the deciding row
     while (r < n && taken[r]) ++r;
-    const VfRow pr = rows[r];
+    VfRow pr = rows[r];
+    pr.lo = wave_uniform(pr.lo);
     const bool less = r < n;  // a rejected token: what the drafter gave is taken away
     const bool point = less && drow == nullptr;
     const bool alone = !less || point;
     if (alone && c != 0) return;
     const int dtok = less ? a.tokens[(size_t)b * (a.R - 1) + r] : -1;
     VfRow qr = pr;
-    if (less && drow != nullptr) qr = rows[n + 1 + r];
+    if (less && drow != nullptr) {
+        qr = rows[n + 1 + r];
+        qr.lo = wave_uniform(qr.lo);
+    }
     const uint16_t* prow = trow + (size_t)r * a.V;
     const uint16_t* qrow = less && drow != nullptr ? drow + (size_t)r * a.V : nullptr;
 
@@ -434,7 +459,7 @@ verify_select_kernel(VerifyArgs a) {
         if (!plain && x == dchunk) return without;
         const VfStat v = stats[(size_t)r * a.chunks + x];
         if (pr.one) return pr.arg / CH == x ? 1.0 : 0.0;
-        return v.sum * vf_exp(v.max, pr.M, e, pow2) * pr.iz;
+        return v.sum * vf_exp(v.max, pr.M, e, pr.lo, pow2) * pr.iz;
     };
     for (int pass = 0; pass < 2; ++pass) {
         mine = 0.0;
