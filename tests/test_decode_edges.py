@@ -29,3 +29,20 @@ def test_a_bound_of_rows_that_leaves_31_bits_is_no_small_grid():
             assert va.lib().viper_hip_kv_read(C.addressof(c), C.addressof(b), FAKE, FAKE, None) == 2
             assert va.lib().viper_hip_kv_append(C.addressof(c), C.addressof(b), FAKE, FAKE, kvh * D, None, 0, 0, None, 0, 0.0,
                                                 None) == 2
+
+
+def test_pools_and_arrays_of_another_type():
+    """Elements of the same size that are read as something else are refused before the device is looked at."""
+    pool = lambda dt: torch.zeros((2, 4, 2, 32 * 128), dtype=dt)
+    scales = torch.zeros((2, 4, 64))
+    for kv, bad in ((va.KVType.BF16, torch.float16), (va.KVType.BF16, torch.int8), (va.KVType.BF16, torch.float32),
+                    (va.KVType.INT8, torch.bool), (va.KVType.INT8, torch.bfloat16)):
+        sc = (scales, scales) if kv == va.KVType.INT8 else (None, None)
+        with pytest.raises(ValueError, match="elements"):
+            va.KVCache(kv, pool(bad), pool(bad), 64, 4, 128, *sc)
+    with pytest.raises(ValueError, match="fp32 elements"):
+        va.KVCache(va.KVType.INT8, pool(torch.int8), pool(torch.int8), 64, 4, 128, scales.int(), scales.int())
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    for args in ((i32(1, 2).float(), i32(1)), (i32(1, 2), i32(1).float()), (i32(1, 2), i32(1), 1, i32(2).float())):
+        with pytest.raises(ValueError, match="int32"):
+            va.KVBatch(*args)

@@ -1,0 +1,44 @@
+"""What the Python calls of the cache, attention and verification refuse on the GPU, and that a refused call writes nothing."""
+import numpy as np
+import pytest
+
+import viper_amd as va
+from test_gpu_attention import setup
+from test_gpu_kv_cache import SENT, back, dev, gpu_cache
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+def verify_args(B=2, R=3, V=104):
+    z = lambda *s, dt=torch.int32: torch.zeros(s, dtype=dt, device="cuda")
+    return dict(target_logits=z(B, R, V, dt=torch.bfloat16), draft_tokens=z(B, R - 1), uniforms=z(B, R, dt=torch.float32),
+                out_tokens=z(B, R) - 7, out_accepted=z(B) - 7, draft_logits=z(B, R - 1, V, dt=torch.bfloat16), draft_lens=z(B),
+                temperature=z(B, dt=torch.float32), accept_probs=z(B, R - 1, dt=torch.float32),
+                workspace=z(va.verify_workspace_bytes(B, R, V), dt=torch.uint8))
+
+
+@pytest.mark.parametrize("name", ["target_logits", "draft_logits", "draft_tokens", "uniforms", "out_tokens", "out_accepted",
+                                  "draft_lens", "temperature", "accept_probs"])
+def test_verify_refuses_elements_of_another_type(name):
+    ok = verify_args()
+    other = {torch.bfloat16: torch.float16, torch.float32: torch.int32, torch.int32: torch.float32}[ok[name].dtype]
+    with pytest.raises(ValueError, match="elements"):
+        va.verify_draft(**{**ok, name: ok[name].to(other)})
+    assert torch.all(ok["out_tokens"] == -7) and torch.all(ok["out_accepted"] == -7)
+    assert va.verify_draft(**ok).ok()
+
+
+def test_rows_of_another_type():
+    c, table, offs, total, q, batch = setup(128, False, 64, 2, 4, [90, 50], 1)
+    g = gpu_cache(c)
+    out = dev(np.full((2, 512), SENT))
+    half = lambda n: torch.zeros((2, n), dtype=torch.float16, device="cuda")
+    good = lambda n: torch.zeros((2, n), dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: va.attention_paged(g, batch, half(512), out), lambda: va.attention_paged(g, batch, good(512), half(512)),
+                 lambda: va.kv_append(g, batch, half(256), good(256)), lambda: va.kv_append(g, batch, good(256), half(256)),
+                 lambda: va.kv_append(g, batch, good(256), good(256), q=half(512), q_out=half(512), rope_theta=1e4),
+                 lambda: va.kv_read(g, batch, half(256), good(256)), lambda: va.kv_read(g, batch, good(256), half(256))):
+        with pytest.raises(ValueError, match="bf16 elements"):
+            call()
+    assert np.all(back(out) == SENT) and np.array_equal(back(g.k), c.k) and np.array_equal(back(g.v), c.v)

@@ -64,7 +64,12 @@ class KVCache(_Fixed):
     num_pages: int = field(init=False, default=0)
 
     def __post_init__(self):
-        size = 1 if int(self.kv_type) == KVType.INT8 else 2
+        i8 = int(self.kv_type) == KVType.INT8
+        for t in (self.k, self.v):
+            _typed(t, "int8" if i8 else "bf16")
+        for t in (self.k_scales, self.v_scales):
+            _typed(t, "fp32")
+        size = 1 if i8 else 2
         page = self.kv_heads * self.page_size * self.head_dim
         if page <= 0 or self.k.numel() != self.v.numel() or self.k.numel() % page:
             raise ValueError("KVCache: k and v hold whole pages of kv_heads * page_size * head_dim elements")
@@ -114,8 +119,7 @@ class KVBatch(_Fixed):
                 raise ValueError("KVBatch: without row_offsets every sequence has max_rows rows")
             self.total_rows = self.batch * self.max_rows
         for t in (self.block_table, self.seq_lens, self.row_offsets):
-            if t is not None and (t.is_floating_point() or t.element_size() != 4):
-                raise ValueError("KVBatch: int32 arrays")
+            _typed(t, "int32")
         _one_device(self.block_table, self.seq_lens, self.row_offsets)
         self._views = {}  # C views by the number of rows
         self._dev = self.seq_lens.get_device()
@@ -136,6 +140,18 @@ class KVBatch(_Fixed):
         return C.addressof(self._views.setdefault(n, v))
 
 
+# What an argument of each kind may be: bf16 values also as their bit patterns
+_KINDS = {"bf16": (torch.bfloat16, torch.int16, torch.uint16), "int8": (torch.int8, torch.uint8), "fp32": (torch.float32,),
+          "int32": (torch.int32, torch.uint32)}
+
+
+def _typed(t, kind):
+    """t, whose elements are of the kind asked for (or None): another type of the same size would be read as it."""
+    if t is not None and t.dtype not in _KINDS[kind]:
+        raise ValueError(f"viper_amd: expected {kind} elements, got {t.dtype}")
+    return t
+
+
 def _one_device(*tensors):
     d = [t.device for t in tensors if t is not None]
     if any(x != d[0] for x in d):
@@ -145,10 +161,9 @@ def _one_device(*tensors):
 def _row_view(t, width, dev):
     """(address, row stride in elements, rows) of a bf16 tensor of rows of `width` values on device number dev: [rows, width]
     or [rows, heads, head_dim], each row dense, rows any multiple of 8 elements apart (columns of a wider matrix)."""
+    _typed(t, "bf16")
     if t.get_device() != dev:
         raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
-    if t.element_size() != 2:
-        raise ValueError(f"viper_amd: expected 2-byte elements, got {t.dtype}")
     shape, s = t.shape, t.stride()
     if len(s) == 2:
         fine = shape[1] == width and s[1] == 1
@@ -166,16 +181,16 @@ def _row_width(t):
     return t.shape[-1] if t.dim() == 2 else t.shape[-1] * t.shape[1]
 
 
-def _flat(t, size, dev, what):
-    """Address of a dense tensor of elements of `size` bytes on device number dev."""
+def _flat(t, kind, dev):
+    """Address of a dense tensor of elements of `kind` (None: any) on device number dev."""
     if t is None:
         return None
+    if kind is not None:
+        _typed(t, kind)
     if t.get_device() != dev:
         raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
     if not t.is_contiguous():
         raise ValueError("viper_amd: tensor arguments must be contiguous")
-    if t.element_size() != size:
-        raise ValueError(f"viper_amd: {what}: expected {size}-byte elements, got {t.dtype}")
     return t.data_ptr()
 
 
@@ -243,7 +258,7 @@ def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, stream=None) -> Status
         return _mismatch(what, "the rows do not match the batch")
     if n == 0:
         return _OK
-    return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, 2, dev, what), _flat(v_out, 2, dev, what))
+    return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, "bf16", dev), _flat(v_out, "bf16", dev))
 
 
 def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int:
@@ -272,7 +287,7 @@ def attention_paged(cache: KVCache, batch: KVBatch, q, out, scale: Optional[floa
     if workspace is not None:
         nws = workspace.numel() * workspace.element_size()
         if nws:
-            ws = _flat(workspace, workspace.element_size(), dev, what)
+            ws = _flat(workspace, None, dev)
     return _call(lib().viper_hip_attention_paged, what, dev, stream, cache._ref, ref, qp, qs, heads,
                  cache._scale if scale is None else scale, window, sinks, op, os, ws, nws)
 
@@ -303,7 +318,7 @@ def verify_draft(target_logits, draft_tokens, uniforms, out_tokens, out_accepted
         draft_tokens = draft_logits = accept_probs = None
     nws = 0 if workspace is None else workspace.numel() * workspace.element_size()
     f = _flat
-    return _call(lib().viper_hip_verify_draft, what, dev, stream, f(target_logits, 2, dev, what), f(draft_logits, 2, dev, what),
-                 f(draft_tokens, 4, dev, what), f(draft_lens, 4, dev, what), f(uniforms, 4, dev, what), f(temperature, 4, dev, what),
-                 B, R, V, f(out_tokens, 4, dev, what), f(out_accepted, 4, dev, what), f(accept_probs, 4, dev, what),
-                 None if workspace is None else f(workspace, workspace.element_size(), dev, what), nws)
+    return _call(lib().viper_hip_verify_draft, what, dev, stream, f(target_logits, "bf16", dev), f(draft_logits, "bf16", dev),
+                 f(draft_tokens, "int32", dev), f(draft_lens, "int32", dev), f(uniforms, "fp32", dev), f(temperature, "fp32", dev),
+                 B, R, V, f(out_tokens, "int32", dev), f(out_accepted, "int32", dev), f(accept_probs, "fp32", dev),
+                 f(workspace, None, dev), nws)
