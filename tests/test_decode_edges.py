@@ -46,3 +46,26 @@ def test_pools_and_arrays_of_another_type():
     for args in ((i32(1, 2).float(), i32(1)), (i32(1, 2), i32(1).float()), (i32(1, 2), i32(1), 1, i32(2).float())):
         with pytest.raises(ValueError, match="int32"):
             va.KVBatch(*args)
+
+
+def test_verify_draft_refuses_another_order_of_axes():
+    """Tensors that hold as many elements, laid out [R, B] for [B, R]; flat ones and axes of one are taken."""
+    z = lambda *s, dt=torch.int32: torch.zeros(s, dtype=dt)
+    f32, bf = torch.float32, torch.bfloat16
+    B, R, V = 4, 3, 104
+    ok = dict(target_logits=z(B, R, V, dt=bf), draft_tokens=z(B, R - 1), uniforms=z(B, R, dt=f32), out_tokens=z(B, R),
+              out_accepted=z(B), draft_logits=z(B, R - 1, V, dt=bf), draft_lens=z(B), temperature=z(B, dt=f32),
+              accept_probs=z(B, R - 1, dt=f32))
+    for bad in (dict(draft_tokens=z(R - 1, B)), dict(uniforms=z(R, B, dt=f32)), dict(out_tokens=z(R, B)),
+                dict(draft_logits=z(R - 1, B, V, dt=bf)), dict(draft_logits=z(B, V, R - 1, dt=bf)),
+                dict(accept_probs=z(R - 1, B, dt=f32)), dict(out_accepted=z(2, 2)), dict(draft_lens=z(5)), dict(uniforms=z(2, 6, dt=f32))):
+        assert va.verify_draft(**{**ok, **bad}).code == va.StatusCode.SHAPE_MISMATCH, bad.keys()
+    for fine in ({}, dict(draft_tokens=z(B * (R - 1))), dict(uniforms=z(B, 1, R, dt=f32)), dict(out_accepted=z(B, 1))):
+        with pytest.raises(ValueError, match="GPU"):  # (host tensors: what comes after the shapes)
+            va.verify_draft(**{**ok, **fine})
+
+
+def test_scales_of_another_order_of_axes():
+    pool, scales = torch.zeros((2, 4, 2, 32 * 128), dtype=torch.int8), torch.zeros((2, 64, 4))
+    with pytest.raises(ValueError, match="one scale"):
+        va.KVCache(va.KVType.INT8, pool, pool, 64, 4, 128, scales, scales)

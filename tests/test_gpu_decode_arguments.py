@@ -42,3 +42,20 @@ def test_rows_of_another_type():
         with pytest.raises(ValueError, match="bf16 elements"):
             call()
     assert np.all(back(out) == SENT) and np.array_equal(back(g.k), c.k) and np.array_equal(back(g.v), c.v)
+
+
+def test_rows_of_another_shape():
+    """Rows by head instead of by token, and tensors that are no rows."""
+    c, table, offs, total, q, batch = setup(128, False, 64, 4, 4, [90, 50], 1)
+    g = gpu_cache(c)
+    z = lambda *s: torch.zeros(s, dtype=torch.bfloat16, device="cuda")
+    out = z(2, 512)
+    for bad in (z(4, 2, 128), z(2, 128, 4), z(4, 256)):
+        assert va.kv_read(g, batch, bad, z(2, 4, 128)).code == va.StatusCode.SHAPE_MISMATCH
+        assert va.kv_read(g, batch, z(2, 4, 128), bad).code == va.StatusCode.SHAPE_MISMATCH
+    for fine in (z(2, 4, 128), z(2, 512), z(1024), z(1, 1024)):
+        assert va.kv_read(g, batch, fine, z(2, 4, 128)).ok()
+    for call in (lambda: va.attention_paged(g, batch, z(1024), out), lambda: va.attention_paged(g, batch, out, z(1024)),
+                 lambda: va.kv_append(g, batch, z(1024), out), lambda: va.kv_append(g, batch, out, out, q=z(1024), q_out=out, rope_theta=1e4)):
+        with pytest.raises(ValueError, match="rows"):
+            call()

@@ -76,9 +76,9 @@ class KVCache(_Fixed):
         self.num_pages = self.k.numel() // page
         if (self.k_scales is None) != (self.v_scales is None):
             raise ValueError("KVCache: k_scales and v_scales go together")
-        if self.k_scales is not None and not (self.k_scales.numel() == self.v_scales.numel() ==
-                                              self.num_pages * self.kv_heads * self.page_size):
-            raise ValueError("KVCache: one scale for each token and head")
+        if self.k_scales is not None and not all(_laid(t, [self.num_pages, self.kv_heads, self.page_size])
+                                                 for t in (self.k_scales, self.v_scales)):
+            raise ValueError("KVCache: one scale for each token and head, [num_pages, kv_heads, page_size]")
         _one_device(self.k, self.v, self.k_scales, self.v_scales)
         self._c = _CCache(int(self.kv_type), self.kv_heads, self.head_dim, self.page_size, self.num_pages, ptr(self.k, size),
                           ptr(self.v, size), ptr(self.k_scales, 4), ptr(self.v_scales, 4))
@@ -152,6 +152,14 @@ def _typed(t, kind):
     return t
 
 
+def _laid(t, shape):
+    """Whether t has this shape, but for axes of one, or is flat with as many elements."""
+    if [*t.shape] == shape:
+        return True
+    a, b = ([n for n in x if n != 1] for x in (t.shape, shape))
+    return t.numel() == math.prod(shape) and (a == b or len(a) < 2)
+
+
 def _one_device(*tensors):
     d = [t.device for t in tensors if t is not None]
     if any(x != d[0] for x in d):
@@ -178,6 +186,8 @@ def _row_view(t, width, dev):
 
 
 def _row_width(t):
+    if t.dim() < 2:
+        raise ValueError(f"viper_amd: expected rows, got a tensor of shape {tuple(t.shape)}")
     return t.shape[-1] if t.dim() == 2 else t.shape[-1] * t.shape[1]
 
 
@@ -256,6 +266,10 @@ def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, stream=None) -> Status
     ref = batch._rows(n // cache._width, dev)
     if v_out.numel() != n or n % cache._width or ref is None:
         return _mismatch(what, "the rows do not match the batch")
+    rows = n // cache._width
+    for t in (k_out, v_out):
+        if not _laid(t, [rows, cache.kv_heads, cache.head_dim]) and not _laid(t, [rows, cache._width]):
+            return _mismatch(what, f"rows of shape {tuple(t.shape)} are not [rows, kv_heads, head_dim]")
     if n == 0:
         return _OK
     return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, "bf16", dev), _flat(v_out, "bf16", dev))
@@ -307,13 +321,12 @@ def verify_draft(target_logits, draft_tokens, uniforms, out_tokens, out_accepted
         return _mismatch(what, "target_logits is [B, R, V]")
     B, R, V = target_logits.shape
     dev, n = target_logits.get_device(), B * (R - 1)
+    for t, *shape in ((uniforms, B, R), (out_tokens, B, R), (out_accepted, B), (draft_tokens, B, R - 1), (draft_logits, B, R - 1, V),
+                      (draft_lens, B), (temperature, B), (accept_probs, B, R - 1)):
+        if t is not None and not _laid(t, shape):
+            return _mismatch(what, f"a tensor of shape {tuple(t.shape)} does not match target_logits, {tuple(shape)} is wanted")
     if dev < 0:
         raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
-    if uniforms.numel() != B * R or out_tokens.numel() != B * R or out_accepted.numel() != B:
-        return _mismatch(what, "uniforms, out_tokens or out_accepted do not match target_logits")
-    for t, size in ((draft_tokens, n), (draft_logits, n * V), (draft_lens, B), (temperature, B), (accept_probs, n)):
-        if t is not None and t.numel() != size:
-            return _mismatch(what, f"a tensor of {t.numel()} elements does not match target_logits, {size} are wanted")
     if n == 0:  # nothing drafted: empty tensors have no address
         draft_tokens = draft_logits = accept_probs = None
     nws = 0 if workspace is None else workspace.numel() * workspace.element_size()
