@@ -69,3 +69,15 @@ def test_scales_of_another_order_of_axes():
     pool, scales = torch.zeros((2, 4, 2, 32 * 128), dtype=torch.int8), torch.zeros((2, 64, 4))
     with pytest.raises(ValueError, match="one scale"):
         va.KVCache(va.KVType.INT8, pool, pool, 64, 4, 128, scales, scales)
+
+
+def test_numbers_that_leave_32_bits():
+    """2^32 + n is not n, and an unknown type is not bf16."""
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    for kw in (dict(max_rows=(1 << 32) + 1), dict(max_rows=1 << 31), dict(max_rows=4, row_offsets=i32(2), total_rows=(1 << 32) + 4)):
+        with pytest.raises(ValueError, match="32-bit"):
+            va.KVBatch(i32(1, 2), i32(1), **kw)
+    pool = torch.zeros((2, 4, 2, 32 * 128), dtype=torch.bfloat16)
+    for kv in (1 << 32, 2, -1):
+        with pytest.raises(ValueError, match="KVType"):
+            va.KVCache(kv, pool, pool, 64, 4, 128)

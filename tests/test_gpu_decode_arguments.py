@@ -59,3 +59,16 @@ def test_rows_of_another_shape():
                  lambda: va.kv_append(g, batch, z(1024), out), lambda: va.kv_append(g, batch, out, out, q=z(1024), q_out=out, rope_theta=1e4)):
         with pytest.raises(ValueError, match="rows"):
             call()
+
+
+def test_a_window_that_leaves_32_bits():
+    """A window of 2^32 tokens hides nothing: it is refused rather than taken for one of 0 or of a few tokens."""
+    c, table, offs, total, q, batch = setup(128, False, 64, 2, 4, [90, 50], 1)
+    g = gpu_cache(c)
+    out = dev(np.full((2, 512), SENT))
+    for kw in (dict(window=1 << 32), dict(window=(1 << 32) + 5), dict(window=1 << 31), dict(window=5, sinks=1 << 32), dict(window=-1),
+               dict(window=3, sinks=-1)):
+        assert va.attention_paged(g, batch, dev(q), out, **kw).code == va.StatusCode.INVALID_ARGUMENT
+    assert np.all(back(out) == SENT)
+    assert va.attention_workspace_bytes(g, batch, (1 << 32) + 4) == 0
+    assert va.attention_paged(g, batch, dev(q), out, window=2 ** 31 - 1, sinks=2 ** 31 - 1).ok()

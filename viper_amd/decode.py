@@ -64,7 +64,7 @@ class KVCache(_Fixed):
     num_pages: int = field(init=False, default=0)
 
     def __post_init__(self):
-        i8 = int(self.kv_type) == KVType.INT8
+        i8 = KVType(self.kv_type) == KVType.INT8
         for t in (self.k, self.v):
             _typed(t, "int8" if i8 else "bf16")
         for t in (self.k_scales, self.v_scales):
@@ -118,6 +118,8 @@ class KVBatch(_Fixed):
             if self.total_rows not in (None, self.batch * self.max_rows):
                 raise ValueError("KVBatch: without row_offsets every sequence has max_rows rows")
             self.total_rows = self.batch * self.max_rows
+        if not (_int32(self.max_rows) and _int32(self.total_rows or 0)):
+            raise ValueError("KVBatch: max_rows and total_rows are 32-bit")
         for t in (self.block_table, self.seq_lens, self.row_offsets):
             _typed(t, "int32")
         _one_device(self.block_table, self.seq_lens, self.row_offsets)
@@ -158,6 +160,11 @@ def _laid(t, shape):
         return True
     a, b = ([n for n in x if n != 1] for x in (t.shape, shape))
     return t.numel() == math.prod(shape) and (a == b or len(a) < 2)
+
+
+def _int32(n):
+    """Whether n reaches the library as it is (ctypes drops the bits that do not fit)."""
+    return -1 << 31 <= n < 1 << 31
 
 
 def _one_device(*tensors):
@@ -278,6 +285,8 @@ def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, stream=None) -> Status
 def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int:
     """Bytes of workspace (zero before its first use) that lets attention_paged split the cache's length over workgroups;
     0 where the batch alone fills the GPU."""
+    if not _int32(heads):
+        return 0
     return int(lib().viper_hip_attention_workspace_bytes(cache._ref, batch._ref, heads))
 
 
@@ -292,6 +301,8 @@ def attention_paged(cache: KVCache, batch: KVBatch, q, out, scale: Optional[floa
         return _mismatch(what, "q rows are not whole heads")
     qp, qs, rows = _row_view(q, width, dev)
     op, os, orows = _row_view(out, width, dev)
+    if not (_int32(window) and _int32(sinks)):
+        return Status(StatusCode.INVALID_ARGUMENT, f"{what}: window and sinks are 32-bit")
     ref = batch._rows(rows, dev)
     if orows != rows or ref is None:
         return _mismatch(what, "the rows do not match the batch")
