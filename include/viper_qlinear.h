@@ -540,7 +540,8 @@ typedef struct viper_kv_batch {
  * kv_stride elements from row to row) in the cache.  rope_theta > 0: k is
  * rotated by its position first, x_i, x_(i + D/2) by the angle position *
  * theta^(-2i/D) (angles and products in 64 bits, rounded to fp32, then bf16), and so
- * is q (heads * head_dim values a row; may be NULL) into q_out, which may be q;
+ * is q (heads * head_dim values a row; may be NULL) into q_out, which may be q and
+ * otherwise overlaps neither q nor k nor v (refused);
  * rope_theta = 0: k is stored as it is, q must be NULL.  Strides are multiples
  * of 8 elements, all pointers 16-byte aligned.  Two rows of one call must not be
  * one token. */
@@ -549,7 +550,7 @@ int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_batch* batch
                         void* q_out_bf16, int64_t q_out_stride, double rope_theta, void* stream);
 
 /* The batch's rows (any max_rows) back from the cache, k_out and v_out
- * [total_rows][kv_heads][head_dim] bf16 (int8: bf16_RNE(code * scale)).
+ * [total_rows][kv_heads][head_dim] bf16, not overlapping (int8: bf16_RNE(code * scale)).
  * Largest calls, with n = min(max_rows, total_rows): kv_append
  * batch n ceil((heads + 2 kv_heads) head_dim / 4096) < 2^24 (heads 0 without q),
  * kv_read 2 batch kv_heads (ceil((n - 1) / 32) + 1) < 2^24 (kv_heads / 2, rounded
@@ -562,7 +563,7 @@ int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_batch* batch, 
  * or j < sinks.  max_rows <= VIPER_QLINEAR_MAX_M; heads a multiple of kv_heads
  * (query head h reads key head h / (heads / kv_heads)), at most 64 to one key
  * head; q and out rows of heads * head_dim bf16 values, strides multiples of 8 elements, 16-byte
- * aligned, out not overlapping q; scale finite and > 0.  Values that a row does not see (masked rows,
+ * aligned, no row of out overlapping one of q (refused); scale finite and > 0.  Values that a row does not see (masked rows,
  * stale or unwritten places of a page) never reach its output, whatever they
  * hold.  The cache's length is split over workgroups that meet through
  * workspace (16-byte aligned, viper_hip_attention_workspace_bytes() bytes, zero

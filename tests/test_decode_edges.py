@@ -81,3 +81,33 @@ def test_numbers_that_leave_32_bits():
     for kv in (1 << 32, 2, -1):
         with pytest.raises(ValueError, match="KVType"):
             va.KVCache(kv, pool, pool, 64, 4, 128)
+
+
+def test_rows_that_overlap_are_refused():
+    from viper_amd.decode import _CBatch, _CCache
+    import ctypes as C
+    L, c = va.lib(), _CCache(0, 4, 128, 64, 8, FAKE, FAKE, None, None)
+
+    def attn(q, qs, o, os, n=8):
+        b = _CBatch(n, 1, n, 4, FAKE, FAKE, None)
+        return L.viper_hip_attention_paged(C.addressof(c), C.addressof(b), q, qs, 8, 0.1, 0, 0, o, os, None, 0, None)
+
+    def append(k, v, ks, q, qs, o, os, n=8):
+        b = _CBatch(n, 1, n, 4, FAKE, FAKE, None)
+        return L.viper_hip_kv_append(C.addressof(c), C.addressof(b), k, v, ks, q, qs, 8, o, os, 1e4, None)
+
+    W, F = 1024, 1 << 30  # 8 heads of 128
+    for q, qs, o, os in ((F, W, F, W), (F, W, F + 2 * W, W), (F + 2 * W, W, F, W), (F, W, F + 16, W), (F, 2 * W, F + 2 * W - 16, 2 * W),
+                         (F, 2 * W, F - 2 * W + 16, 2 * W), (F, W, F + 2 * 7 * W, W), (F, 2 * W, F + 2 * 7 * W, W),
+                         (F, W, F + 2 * W, 2 * W), (F, 2 * W, F + 2 * 3 * W + 16, 3 * W), (F, 1 << 40, F + 2 * (1 << 40), 1 << 40)):
+        assert attn(q, qs, o, os) == 2, (q - F, qs, o - F, os)
+    assert attn(F, W, F + 2 * W - 16, W, 1) == 2
+    K = F << 2
+    for k, v, ks, q, qs, o, os in ((K, K, 512, F, W, F + 16, W), (K, K, 512, F, W, F, W + 8), (K, K, 512, F, W, F + 2 * W, W),
+                                   (K, K, 512, F, W, K, W), (K, 3 * K, 512, F, W, 3 * K + 7 * 1024, W),
+                                   (F + 2 * W - 1024, K, 2048, F, 2048, F, 2048)):
+        assert append(k, v, ks, q, qs, o, os) == 2, (k, v, ks, q - F, qs, o - F, os)
+    for d in (0, 16, 2 * 512 * 7):
+        b = _CBatch(8, 1, 8, 4, FAKE, FAKE, None)
+        assert L.viper_hip_kv_read(C.addressof(c), C.addressof(b), F, F + d, None) == 2
+        assert L.viper_hip_kv_read(C.addressof(c), C.addressof(b), F + d, F, None) == 2

@@ -72,3 +72,32 @@ def test_a_window_that_leaves_32_bits():
     assert np.all(back(out) == SENT)
     assert va.attention_workspace_bytes(g, batch, (1 << 32) + 4) == 0
     assert va.attention_paged(g, batch, dev(q), out, window=2 ** 31 - 1, sinks=2 ** 31 - 1).ok()
+
+
+def test_overlapping_rows_are_refused_and_no_others():
+    """Rows of q and of the output anywhere in one buffer, against a look at every element."""
+    rng = np.random.default_rng(50)
+    c, table, offs, total, q, _ = setup(64, False, 32, 1, 1, [40] * 6, 1)
+    g = gpu_cache(c)
+    buf = torch.zeros((6000,), dtype=torch.bfloat16, device="cuda")
+    seen = {True: 0, False: 0}
+    for _ in range(300):
+        n = int(rng.integers(1, 7))
+        batch = va.KVBatch(dev(table[:n].copy()), dev(np.full(n, 40, np.int32)), 1)
+        strides = [64 + 8 * int(rng.integers(0, 12)) for _ in range(2)]
+        if rng.random() < 0.5:
+            strides[1] = strides[0]
+        at = [8 * int(rng.integers(0, 200)) for _ in range(2)]
+        rows = [{a + i * s + e for i in range(n) for e in range(64)} for a, s in zip(at, strides)]
+        Q, out = (buf.as_strided((n, 64), (s, 1), a) for a, s in zip(at, strides))
+        meet = bool(rows[0] & rows[1])
+        st = va.attention_paged(g, batch, Q, out)
+        assert st.code == (va.StatusCode.INVALID_ARGUMENT if meet else va.StatusCode.OK), (n, at, strides)
+        seen[meet] += 1
+        same = at[0] == at[1] and (strides[0] == strides[1] or n == 1)
+        kv = torch.zeros((n, 64), dtype=torch.bfloat16, device="cuda")
+        st = va.kv_append(g, batch, kv, kv, q=Q, q_out=out, rope_theta=1e4)
+        assert st.code == (va.StatusCode.INVALID_ARGUMENT if meet and not same else va.StatusCode.OK), (n, at, strides)
+        assert va.kv_append(g, batch, kv, kv, q=Q, q_out=Q, rope_theta=1e4).ok()
+        assert va.kv_append(g, batch, Q, Q, q=kv, q_out=out, rope_theta=1e4).ok() != meet, (n, at, strides)
+    assert min(seen.values()) > 40

@@ -81,7 +81,8 @@ extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const vipe
         return VIPER_INVALID_ARGUMENT;
     }
     if (batch->total_rows == 0) return VIPER_OK;
-    if (q_bf16 == out_bf16) return VIPER_INVALID_ARGUMENT;  // (rows may be read again after others are written)
+    // (rows may be read again after others are written)
+    if (rows_meet(q_bf16, q_stride, width, out_bf16, out_stride, width, batch->total_rows)) return VIPER_INVALID_ARGUMENT;
     AttnArgs a;
     a.c = kv_args(cache, batch);
     a.q = (const uint16_t*)q_bf16;

@@ -313,6 +313,15 @@ extern "C" int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_b
         return VIPER_INVALID_ARGUMENT;
     }
     if (batch->total_rows == 0) return VIPER_OK;
+    if (q_bf16 != nullptr) {  // q_out may be q, and nothing else that other workgroups read
+        const int64_t n = batch->total_rows, qw = (int64_t)heads * D;
+        if ((q_out_bf16 != q_bf16 || (q_out_stride != q_stride && n > 1)) &&
+            rows_meet(q_bf16, q_stride, qw, q_out_bf16, q_out_stride, qw, n))
+            return VIPER_INVALID_ARGUMENT;
+        if (rows_meet(k_bf16, kv_stride, width, q_out_bf16, q_out_stride, qw, n) ||
+            rows_meet(v_bf16, kv_stride, width, q_out_bf16, q_out_stride, qw, n))
+            return VIPER_INVALID_ARGUMENT;
+    }
     AppendArgs a;
     a.c = kv_args(cache, batch);
     a.k = (const uint16_t*)k_bf16;
@@ -344,6 +353,8 @@ extern "C" int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_bat
     if (k_out_bf16 == nullptr || v_out_bf16 == nullptr || misaligned(k_out_bf16, 16) || misaligned(v_out_bf16, 16))
         return VIPER_INVALID_ARGUMENT;
     if (batch->total_rows == 0) return VIPER_OK;
+    const int64_t row = (int64_t)cache->kv_heads * cache->head_dim;
+    if (rows_meet(k_out_bf16, row, row, v_out_bf16, row, row, batch->total_rows)) return VIPER_INVALID_ARGUMENT;
     ReadArgs a;
     a.c = kv_args(cache, batch);
     a.ko = (uint16_t*)k_out_bf16;

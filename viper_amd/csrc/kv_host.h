@@ -53,4 +53,24 @@ inline bool bad_rows(const void* p, int64_t stride, int64_t width) {
     return p == nullptr || misaligned(p, 16) || stride < width || stride % 8 != 0 || stride > (int64_t)1 << 40;
 }
 
+// Whether two tensors of n rows (dense rows of pw and ow bf16 values, their strides
+// in elements) have a value in common, or reach further than any memory.  Columns of
+// one wider matrix have one stride and need no walk.
+inline bool rows_meet(const void* p, int64_t ps, int64_t pw, const void* o, int64_t os, int64_t ow, int64_t n) {
+    if (ps > ((int64_t)1 << 48) / n || os > ((int64_t)1 << 48) / n) return true;
+    // the second begins d elements past the first
+    const int64_t d = ((int64_t)(uintptr_t)o - (int64_t)(uintptr_t)p) / 2;
+    if (d >= (n - 1) * ps + pw || -d >= (n - 1) * os + ow) return false;
+    auto below = [](int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); };  // floor(a / b)
+    if (ps == os) {  // row i + k of the second begins d + k s past row i: from -ow + 1 to pw - 1 they meet
+        const int64_t k0 = below(-ow - d, os) + 1, k1 = below(pw - 1 - d, os);
+        return (k0 > 1 - n ? k0 : 1 - n) <= (k1 < n - 1 ? k1 : n - 1);
+    }
+    for (int64_t i = 0; i < n; ++i) {
+        const int64_t e = i * ps - d, j0 = below(e - ow, os) + 1, j1 = below(e + pw - 1, os);
+        if ((j0 > 0 ? j0 : 0) <= (j1 < n - 1 ? j1 : n - 1)) return true;
+    }
+    return false;
+}
+
 }  // namespace vq
