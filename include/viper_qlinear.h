@@ -596,6 +596,7 @@ int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch*
  * samples (draft_tokens may be NULL).  A draft token outside the vocabulary is
  * rejected; a temperature that is negative or not finite, or a draft_lens[b]
  * outside 0 .. R - 1, makes out_accepted[b] and the sequence's tokens -1.
+ * Outputs and workspace overlap neither the inputs nor one another (refused).
  * B <= 4096, V < 2^26, B (2R - 1) ceil(V / 4096) <= 2^22.  workspace: viper_hip_verify_workspace_bytes(B, R, V)
  * bytes, 16-byte aligned, zero before the first call; every call leaves it fit
  * for the next call of any shape that it is large enough for; calls in flight

@@ -111,3 +111,21 @@ def test_rows_that_overlap_are_refused():
         b = _CBatch(8, 1, 8, 4, FAKE, FAKE, None)
         assert L.viper_hip_kv_read(C.addressof(c), C.addressof(b), F, F + d, None) == 2
         assert L.viper_hip_kv_read(C.addressof(c), C.addressof(b), F + d, F, None) == 2
+
+
+def test_verify_outputs_that_overlap_are_refused():
+    import ctypes as C
+    L, M = va.lib(), 1 << 20
+    B, R, V = 4, 5, 1000
+    ws = va.verify_workspace_bytes(B, R, V)
+    ok = dict(target=10 * M, draft=20 * M, tokens=30 * M, lens=31 * M, u=32 * M, t=33 * M, out=34 * M, acc=35 * M, probs=36 * M, ws=40 * M)
+    size = dict(target=B * R * V * 2, draft=B * (R - 1) * V * 2, tokens=B * (R - 1) * 4, lens=B * 4, u=B * R * 4, t=B * 4, out=B * R * 4,
+                acc=B * 4, probs=B * (R - 1) * 4, ws=ws)
+    for x in ("out", "acc", "probs", "ws"):
+        for y in ok:
+            if x == y:
+                continue
+            for at in (ok[y], ok[y] + size[y] // 32 * 16, ok[y] + size[y] - 16):
+                a = {**ok, x: at}
+                assert L.viper_hip_verify_draft(a["target"], a["draft"], a["tokens"], a["lens"], a["u"], a["t"], B, R, V, a["out"], a["acc"],
+                                                a["probs"], a["ws"], ws, None) == 2, (x, y, at)

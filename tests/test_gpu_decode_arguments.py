@@ -101,3 +101,23 @@ def test_overlapping_rows_are_refused_and_no_others():
         assert va.kv_append(g, batch, kv, kv, q=Q, q_out=Q, rope_theta=1e4).ok()
         assert va.kv_append(g, batch, Q, Q, q=kv, q_out=out, rope_theta=1e4).ok() != meet, (n, at, strides)
     assert min(seen.values()) > 40
+
+
+def test_verify_takes_neighbours_in_one_buffer():
+    """Everything but the logits side by side in one buffer, with nothing between: nothing overlaps."""
+    a = verify_args(B=3, R=4, V=100)
+    assert va.verify_draft(**a).ok()
+    names = ["draft_tokens", "out_tokens", "draft_lens", "out_accepted", "uniforms", "accept_probs", "temperature"]
+    buf = torch.zeros((sum(a[n].numel() for n in names),), dtype=torch.int32, device="cuda")
+    at, views = 0, {}
+    for n in names:
+        views[n] = buf[at:at + a[n].numel()].view(a[n].dtype).view(a[n].shape)
+        at += a[n].numel()
+    assert va.verify_draft(**{**a, **views}).ok()
+    for n in ("out_tokens", "out_accepted", "accept_probs"):
+        assert views[n].tolist() == a[n].tolist()
+    assert a["out_accepted"].tolist() == [0] * 3 and a["out_tokens"].tolist() == [[0, -1, -1, -1]] * 3
+    for x, y in (("out_tokens", "uniforms"), ("accept_probs", "uniforms"), ("out_accepted", "draft_lens")):
+        over = views[y].view(torch.int32).flatten()
+        if over.numel() == a[x].numel():
+            assert va.verify_draft(**{**a, **views, x: over.view(a[x].dtype)}).code == va.StatusCode.INVALID_ARGUMENT

@@ -577,6 +577,19 @@ extern "C" int viper_hip_verify_draft(const void* target_bf16, const void* draft
         misaligned(accept_probs, 4))
         return VIPER_INVALID_ARGUMENT;
     if (workspace == nullptr || misaligned(workspace, 16) || workspace_bytes < vf_bytes(B, R, V)) return VIPER_INVALID_ARGUMENT;
+    // what is written (the first four) overlaps nothing else: other workgroups may still read it
+    const size_t rows4 = (size_t)B * R * 4, drafted = (size_t)B * (R - 1);
+    const struct {
+        const void* p;
+        size_t bytes;
+    } at[] = {{out_tokens, rows4}, {out_accepted, (size_t)B * 4}, {accept_probs, drafted * 4}, {workspace, vf_bytes(B, R, V)},
+              {target_bf16, (size_t)B * R * V * 2}, {draft_bf16, drafted * V * 2}, {draft_tokens, drafted * 4},
+              {draft_lens, (size_t)B * 4}, {uniforms, rows4}, {temperature, (size_t)B * 4}};
+    for (size_t i = 0; i < 4; ++i)
+        for (size_t j = i + 1; j < sizeof(at) / sizeof(at[0]); ++j)
+            if (at[i].p != nullptr && at[j].p != nullptr && at[i].bytes != 0 && at[j].bytes != 0 &&
+                (uintptr_t)at[i].p < (uintptr_t)at[j].p + at[j].bytes && (uintptr_t)at[j].p < (uintptr_t)at[i].p + at[i].bytes)
+                return VIPER_INVALID_ARGUMENT;
     VerifyArgs a;
     a.target = (const uint16_t*)target_bf16;
     a.draft = R > 1 ? (const uint16_t*)draft_bf16 : nullptr;
