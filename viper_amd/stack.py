@@ -28,11 +28,11 @@ Device buffers are torch tensors (allocation only); every launch is a C ABI
 call on the current stream, so a whole step can be captured in a HIP graph.
 
 With `context` > 0 a step is a whole decode step: every slot has a paged
-key/value cache of that many tokens, and between the q/k/v projections and the
+key/value cache of that many tokens, rounded up to whole pages (`capacity`), and between the q/k/v projections and the
 o projection q and k are rotated, k and v stored and the new token attends over
 its sequence (two launches more, kv_append and attention_paged), in place of the
 fixed activation.  The sequence's length is on the device and grows by one in
-each step, a captured step's replays included; past `context` tokens results
+each step, a captured step's replays included; past `capacity` tokens results
 are NaN.
 """
 import ctypes as C
@@ -127,6 +127,7 @@ class Stack:
         self.context = context
         if context:
             pages = (context + page_size - 1) // page_size
+            self.capacity = pages * page_size
             self.rope_theta, self.window, self.sinks = rope_theta, window, sinks
             self.seq_len = torch.zeros((1,), dtype=torch.int32, device="cuda")
             table = torch.arange(pages, dtype=torch.int32, device="cuda").view(1, pages)
