@@ -124,3 +124,105 @@ def test_values_whose_sum_leaves_32_bits(i8, ws):
     o, bound = R.attention(c, table, lens, rows, offs, q, heads, D ** -0.5)
     assert all(np.isfinite(x).all() for x in o.values())
     check(back(out), o, bound, lens, rows, offs)
+
+
+def apart(D, i8, kvh, heads, lens, rows, seed, **kw):
+    """A setup whose table is wide enough that parts are joined by a launch of their own (80000 bytes of sums and more)."""
+    c, table, offs, total, q, _ = setup(D, i8, 64, kvh, heads, lens, rows, seed=seed, **kw)
+    wide = np.full((len(lens), 600), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    batch = va.KVBatch(dev(wide), dev(np.array(lens, np.int32)), rows)
+    return c, wide, offs, total, q, batch
+
+
+def assert_apart(batch, cache, D, kvh, heads, rows):
+    g = heads // kvh * rows
+    qt = -(-g // 16)
+    assert qt <= 2  # (one group of rows)
+    splits = (va.attention_workspace_bytes(cache, batch, heads) - 8192) // (batch.batch * kvh * qt * 16 * (D + 2) * 4)
+    assert splits * g * D * 4 >= 80000
+
+
+SHAPES = [(128, 4, 20, 3), (64, 2, 16, 4), (256, 1, 5, 3)]
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("D,kvh,heads,rows", SHAPES)
+@pytest.mark.parametrize("value", [0x7F80, 0xFF80, 0x7FC0])
+def test_join_of_values_that_are_not_finite(i8, D, kvh, heads, rows, value):
+    """The newest row's own token holds it: the rows before do not see it; with a window that leaves an early one behind."""
+    n = 3000
+    for window, sinks, hit in ((0, 0, n - 1), (700, 5, n - 1), (700, 0, n - 701)):  # the last: behind the newest row's window
+        c, table, offs, total, q, batch = apart(D, i8, kvh, heads, [n], rows, 60)
+        pg, at = table[0, hit // 64], hit % 64
+        for h in range(kvh):
+            if i8:
+                c.vs[c.scale_at(pg, at, h)] = R.bf16_val(np.uint16(value))
+                c.v[c.places(pg, at, h, False)] = np.int8(3)
+            else:
+                c.v[c.places(pg, at, h, False)[::7]] = value
+        g = gpu_cache(c)
+        assert_apart(batch, g, D, kvh, heads, rows)
+        out = dev(np.full((total, heads * D), SENT))
+        assert va.attention_paged(g, batch, dev(q), out, window=window, sinks=sinks, workspace=workspace(g, batch, heads)).ok()
+        o, bound = R.attention(c, table, [n], rows, offs, q, heads, D ** -0.5, window, sinks)
+        finite = [bool(np.all(np.isfinite(o[r]))) for r in range(rows)]
+        assert finite == ([True] * (rows - 1) + [False] if hit == n - 1 else [False] * (rows - 1) + [True])
+        check(back(out), o, bound, [n], rows, offs, (window, hit))
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("D,kvh,heads,rows", SHAPES)
+def test_join_of_missing_pages_and_keys_that_are_not_numbers(i8, D, kvh, heads, rows):
+    """A page that only the newest row sees, one that every row sees, a NaN key of the newest token, a length past the table."""
+    n = 45 * 64 + 1  # the newest token begins a page, the rows before it see the whole pages up to there
+    c, table, offs, total, q, _ = apart(D, i8, kvh, heads, [n], rows, 61)
+    o, bound = R.attention(c, table, [n], rows, offs, q, heads, D ** -0.5)
+
+    def run(tb, length=n, cache=c):
+        g = gpu_cache(cache)
+        b = va.KVBatch(dev(tb), dev(np.array([length], np.int32)), rows)
+        assert_apart(b, g, D, kvh, heads, rows)
+        out = dev(np.full((total, heads * D), SENT))
+        assert va.attention_paged(g, b, dev(q), out, workspace=workspace(g, b, heads)).ok()
+        return back(out)
+
+    def older_rows_only(got):
+        y = R.bf16_val(got)
+        assert np.all(np.isnan(y[rows - 1]))
+        for r in range(rows - 1):
+            assert np.all(np.abs(y[r].reshape(heads, D) - o[r]) <= bound[r]), r
+
+    bad = table.copy()
+    bad[0, 45] = c.pages  # the newest token's page
+    older_rows_only(run(bad))
+    bad[0, 45], bad[0, 20] = table[0, 45], -1
+    assert np.all(np.isnan(R.bf16_val(run(bad))))
+    for h in range(kvh):
+        if i8:
+            c.ks[c.scale_at(table[0, 45], 0, h)] = np.nan
+        else:
+            c.k[c.places(table[0, 45], 0, h, True)[9]] = 0x7FC0
+    older_rows_only(run(table))
+    cap = table.shape[1] * 64
+    full = np.zeros_like(table)  # (every page is there: page 0 again and again)
+    y = R.bf16_val(run(full, cap + 1))
+    assert np.all(np.isnan(y[rows - 1])) and np.all(np.isfinite(y[:rows - 1]))
+
+
+@pytest.mark.parametrize("i8", [False, True])
+@pytest.mark.parametrize("D,kvh,heads,rows", SHAPES)
+def test_join_of_values_whose_sum_leaves_32_bits(i8, D, kvh, heads, rows):
+    n = 1500
+    c, table, offs, total, q, batch = apart(D, i8, kvh, heads, [n], rows, 62, std=0.3)
+    if i8:
+        c.vs[:] = np.float32(2.6e36)
+        c.v[:] = np.abs(c.v)
+    else:
+        c.v[:] = R.bf16_bits(np.float32(3e38) * (1 + 0.1 * np.random.default_rng(63).uniform(-1, 1, len(c.v))).astype(np.float32))
+    g = gpu_cache(c)
+    assert_apart(batch, g, D, kvh, heads, rows)
+    out = dev(np.full((total, heads * D), SENT))
+    assert va.attention_paged(g, batch, dev(q), out, workspace=workspace(g, batch, heads)).ok()
+    o, bound = R.attention(c, table, [n], rows, offs, q, heads, D ** -0.5)
+    check(back(out), o, bound, [n], rows, offs)
