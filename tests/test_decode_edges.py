@@ -129,3 +129,32 @@ def test_verify_outputs_that_overlap_are_refused():
                 a = {**ok, x: at}
                 assert L.viper_hip_verify_draft(a["target"], a["draft"], a["tokens"], a["lens"], a["u"], a["t"], B, R, V, a["out"], a["acc"],
                                                 a["probs"], a["ws"], ws, None) == 2, (x, y, at)
+
+
+def test_workspace_is_sized_for_the_cache_s_device(monkeypatch):
+    """The plan counts the CUs of the device that the call runs on, not of the current one."""
+    import ctypes as C
+    from types import SimpleNamespace
+    from viper_amd import decode
+    from viper_amd.decode import _CBatch, _CCache
+    c, b = _CCache(0, 4, 128, 64, 8, FAKE, FAKE, None, None), _CBatch(1, 1, 1, 512, FAKE, FAKE, None)
+    seen, now = [], [0]
+
+    class Device:
+        def __init__(self, n):
+            self.n = n
+
+        def __enter__(self):
+            now.append(self.n)
+
+        def __exit__(self, *e):
+            now.pop()
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: now[-1])
+    monkeypatch.setattr(decode, "lib", lambda: SimpleNamespace(
+        viper_hip_attention_workspace_bytes=lambda *a: seen.append(now[-1]) or va.lib().viper_hip_attention_workspace_bytes(*a)))
+    for dev in (1, 0):
+        n = va.attention_workspace_bytes(SimpleNamespace(_ref=C.addressof(c), _dev=dev), SimpleNamespace(_ref=C.addressof(b)), 20)
+        assert n > 8192
+    assert seen == [1, 0] and now == [0]

@@ -287,6 +287,9 @@ def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int
     0 where the batch alone fills the GPU."""
     if not _int32(heads):
         return 0
+    if cache._dev != torch.cuda.current_device():  # (the plan counts a device's CUs)
+        with torch.cuda.device(cache._dev):
+            return int(lib().viper_hip_attention_workspace_bytes(cache._ref, batch._ref, heads))
     return int(lib().viper_hip_attention_workspace_bytes(cache._ref, batch._ref, heads))
 
 
