@@ -248,11 +248,10 @@ template <int D, int ROWS>
 __device__ __forceinline__ bool attn_store(const AttnArgs& a, const AttnSeq& s, int qg, int head, int rr, int d, at_f32x4 o,
                                            float l) {
     const int r = qg * ROWS + rr, i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
-    o = o * (1.0f / l);
-    bool fine = true;
+    o = o * (1.0f / l);  // (NaN where l is 0 or NaN)
+    bool fine = !(l > 0.0f);
     if (s.pos0 + i < 0) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    else if (!(l > 0.0f)) o = o + __uint_as_float(0x7fc00000u);
-    else fine = o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f == 0.0f;
+    fine |= o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f == 0.0f;
     *(u32x2*)(a.out + (size_t)(s.sq.row0 + i) * a.out_stride + (size_t)(head * a.gqa + hh) * D + d) =
         u32x2{f2bf2(o[0], o[1]), f2bf2(o[2], o[3])};
     return fine;

@@ -66,9 +66,9 @@ class KVCache(_Fixed):
     def __post_init__(self):
         i8 = KVType(self.kv_type) == KVType.INT8
         for t in (self.k, self.v):
-            _typed(t, "int8" if i8 else "bf16")
+            _typed(t, _INT8 if i8 else _BF16)
         for t in (self.k_scales, self.v_scales):
-            _typed(t, "fp32")
+            _typed(t, _FP32)
         size = 1 if i8 else 2
         page = self.kv_heads * self.page_size * self.head_dim
         if page <= 0 or self.k.numel() != self.v.numel() or self.k.numel() % page:
@@ -76,7 +76,7 @@ class KVCache(_Fixed):
         self.num_pages = self.k.numel() // page
         if (self.k_scales is None) != (self.v_scales is None):
             raise ValueError("KVCache: k_scales and v_scales go together")
-        if self.k_scales is not None and not all(_laid(t, [self.num_pages, self.kv_heads, self.page_size])
+        if self.k_scales is not None and not all(_laid(t, (self.num_pages, self.kv_heads, self.page_size))
                                                  for t in (self.k_scales, self.v_scales)):
             raise ValueError("KVCache: one scale for each token and head, [num_pages, kv_heads, page_size]")
         _one_device(self.k, self.v, self.k_scales, self.v_scales)
@@ -121,7 +121,7 @@ class KVBatch(_Fixed):
         if not (_int32(self.max_rows) and _int32(self.total_rows or 0)):
             raise ValueError("KVBatch: max_rows and total_rows are 32-bit")
         for t in (self.block_table, self.seq_lens, self.row_offsets):
-            _typed(t, "int32")
+            _typed(t, _INT32)
         _one_device(self.block_table, self.seq_lens, self.row_offsets)
         self._views = {}  # C views by the number of rows
         self._dev = self.seq_lens.get_device()
@@ -142,22 +142,26 @@ class KVBatch(_Fixed):
         return C.addressof(self._views.setdefault(n, v))
 
 
-# What an argument of each kind may be: bf16 values also as their bit patterns
-_KINDS = {"bf16": (torch.bfloat16, torch.int16, torch.uint16), "int8": (torch.int8, torch.uint8), "fp32": (torch.float32,),
-          "int32": (torch.int32, torch.uint32)}
+# What the elements of each kind of argument may be (bf16 values also as their bit patterns): another type of the same size
+# would be read as it
+_BF16 = (torch.bfloat16, torch.int16, torch.uint16)
+_INT8 = (torch.int8, torch.uint8)
+_FP32 = (torch.float32,)
+_INT32 = (torch.int32, torch.uint32)
 
 
-def _typed(t, kind):
-    """t, whose elements are of the kind asked for (or None): another type of the same size would be read as it."""
-    if t is not None and t.dtype not in _KINDS[kind]:
-        raise ValueError(f"viper_amd: expected {kind} elements, got {t.dtype}")
-    return t
+def _typed(t, types):
+    if t is not None and t.dtype not in types:
+        raise _untyped(t, types)
+
+
+def _untyped(t, types):
+    name = {_BF16: "bf16", _INT8: "int8", _FP32: "fp32", _INT32: "int32"}[types]
+    return ValueError(f"viper_amd: expected {name} elements, got {t.dtype}")
 
 
 def _laid(t, shape):
     """Whether t has this shape, but for axes of one, or is flat with as many elements."""
-    if [*t.shape] == shape:
-        return True
     a, b = ([n for n in x if n != 1] for x in (t.shape, shape))
     return t.numel() == math.prod(shape) and (a == b or len(a) < 2)
 
@@ -176,7 +180,8 @@ def _one_device(*tensors):
 def _row_view(t, width, dev):
     """(address, row stride in elements, rows) of a bf16 tensor of rows of `width` values on device number dev: [rows, width]
     or [rows, heads, head_dim], each row dense, rows any multiple of 8 elements apart (columns of a wider matrix)."""
-    _typed(t, "bf16")
+    if t.dtype not in _BF16:
+        raise _untyped(t, _BF16)
     if t.get_device() != dev:
         raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
     shape, s = t.shape, t.stride()
@@ -198,12 +203,12 @@ def _row_width(t):
     return t.shape[-1] if t.dim() == 2 else t.shape[-1] * t.shape[1]
 
 
-def _flat(t, kind, dev):
-    """Address of a dense tensor of elements of `kind` (None: any) on device number dev."""
+def _flat(t, types, dev):
+    """Address of a dense tensor of elements of one of `types` (None: any) on device number dev."""
     if t is None:
         return None
-    if kind is not None:
-        _typed(t, kind)
+    if types is not None and t.dtype not in types:
+        raise _untyped(t, types)
     if t.get_device() != dev:
         raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
     if not t.is_contiguous():
@@ -275,11 +280,12 @@ def kv_read(cache: KVCache, batch: KVBatch, k_out, v_out, stream=None) -> Status
         return _mismatch(what, "the rows do not match the batch")
     rows = n // cache._width
     for t in (k_out, v_out):
-        if not _laid(t, [rows, cache.kv_heads, cache.head_dim]) and not _laid(t, [rows, cache._width]):
+        if t.shape != (rows, cache.kv_heads, cache.head_dim) and t.shape != (rows, cache._width) and \
+                not _laid(t, (rows, cache.kv_heads, cache.head_dim)) and not _laid(t, (rows, cache._width)):
             return _mismatch(what, f"rows of shape {tuple(t.shape)} are not [rows, kv_heads, head_dim]")
     if n == 0:
         return _OK
-    return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, "bf16", dev), _flat(v_out, "bf16", dev))
+    return _call(lib().viper_hip_kv_read, what, dev, stream, cache._ref, ref, _flat(k_out, _BF16, dev), _flat(v_out, _BF16, dev))
 
 
 def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int:
@@ -335,17 +341,18 @@ def verify_draft(target_logits, draft_tokens, uniforms, out_tokens, out_accepted
         return _mismatch(what, "target_logits is [B, R, V]")
     B, R, V = target_logits.shape
     dev, n = target_logits.get_device(), B * (R - 1)
-    for t, *shape in ((uniforms, B, R), (out_tokens, B, R), (out_accepted, B), (draft_tokens, B, R - 1), (draft_logits, B, R - 1, V),
-                      (draft_lens, B), (temperature, B), (accept_probs, B, R - 1)):
-        if t is not None and not _laid(t, shape):
-            return _mismatch(what, f"a tensor of shape {tuple(t.shape)} does not match target_logits, {tuple(shape)} is wanted")
+    each, every, drafted = (B,), (B, R), (B, R - 1)
+    for t, shape in ((uniforms, every), (out_tokens, every), (out_accepted, each), (draft_tokens, drafted),
+                     (draft_logits, (B, R - 1, V)), (draft_lens, each), (temperature, each), (accept_probs, drafted)):
+        if t is not None and t.shape != shape and not _laid(t, shape):
+            return _mismatch(what, f"a tensor of shape {tuple(t.shape)} does not match target_logits, {shape} is wanted")
     if dev < 0:
         raise ValueError("viper_amd: tensor arguments must be GPU tensors, all on one device")
     if n == 0:  # nothing drafted: empty tensors have no address
         draft_tokens = draft_logits = accept_probs = None
     nws = 0 if workspace is None else workspace.numel() * workspace.element_size()
     f = _flat
-    return _call(lib().viper_hip_verify_draft, what, dev, stream, f(target_logits, "bf16", dev), f(draft_logits, "bf16", dev),
-                 f(draft_tokens, "int32", dev), f(draft_lens, "int32", dev), f(uniforms, "fp32", dev), f(temperature, "fp32", dev),
-                 B, R, V, f(out_tokens, "int32", dev), f(out_accepted, "int32", dev), f(accept_probs, "fp32", dev),
+    return _call(lib().viper_hip_verify_draft, what, dev, stream, f(target_logits, _BF16, dev), f(draft_logits, _BF16, dev),
+                 f(draft_tokens, _INT32, dev), f(draft_lens, _INT32, dev), f(uniforms, _FP32, dev), f(temperature, _FP32, dev),
+                 B, R, V, f(out_tokens, _INT32, dev), f(out_accepted, _INT32, dev), f(accept_probs, _FP32, dev),
                  f(workspace, None, dev), nws)
