@@ -87,15 +87,18 @@ __device__ __forceinline__ void vf_load(const uint16_t* row, int j, int step, in
 }
 
 // e^((l - M) / T): 1 at the maximum (also an infinite one), 0 for NaN, for what is
-// infinitely far below the maximum at any T, and below 2^-1000.  With y = 64 (l - M) log2 e / T = 64 n + k + f, |f| <= 1/2, it
-// is 2^n 2^(k/64) times the power series of 2^(f/64) to its 4th term (what is left
-// out is under (ln 2 / 128)^5 / 5! = 4e-14).  What bounds the statistics is the
+// infinitely far below the maximum at any T, and below 2^-1000.  With y = 64 (l - M)
+// log2 e / T = 64 n + k + f, |f| <= 1/2, it is 2^n 2^(k/64) times the power series of
+// 2^(f/64) to its 4th term (what is left out is under (ln 2 / 128)^5 / 5! = 4e-14 of
+// the weight, so that a token can differ from one drawn by exact weights where the
+// uniform lies that close to a border).  What bounds the statistics is the
 // number of instructions a logit takes (full drafts of 8 sequences, 21 million
 // logits): 64-bit adds and products run at the full rate, conversions, rounding and
 // ldexp at a quarter of it.  So l is widened by its bits: placed in a double they
 // read as 2^-896 l, exactly, below the normal range too (an infinite l as 2^128, which
-// vf_floor takes care of), and 2^896 goes into the factor; the whole part of y is the low word of y + 1.5 * 2^52, n goes into the exponent and
-// 2^(k/64) comes from a table in LDS.
+// vf_floor takes care of), and 2^896 goes into the factor; the whole part of y is the
+// low word of y + 1.5 * 2^52, n goes into the exponent and 2^(k/64) comes from a table
+// in LDS.
 __device__ const double VF_POW2[64] = {
     1, 1.0108892860517005, 1.0218971486541166, 1.0330248790212284,
     1.0442737824274138, 1.0556451783605572, 1.0671404006768237, 1.0787607977571199,
@@ -125,7 +128,10 @@ __device__ __forceinline__ double vf_c(float T) {
 }
 // The y above which a logit weighs: 2^-1000, or at temperatures where that lies
 // further down, what separates -inf from the finite ones, and these from +inf
-__device__ __forceinline__ double vf_floor(float M, double c) {
+// (the logits next to an infinite one are 2^120 from it: 64 log2 e 2^120 / T passes
+// 64000 up to T = 1.9e33, so that an ordinary temperature waits for no M here)
+__device__ __forceinline__ double vf_floor(float M, float T, double c) {
+    if (T < 1e33f) return -64000.0;
     const double inf = widen(__builtin_inff());
     const double gap = M == __builtin_inff() ? 0x1p-776 : inf + widen(M);  // (2^120 is the step below 2^128)
     return fmax(-64000.0, -gap * c);
@@ -137,7 +143,7 @@ __device__ __forceinline__ double wave_uniform(double v) {
     const unsigned hi = (unsigned)__builtin_amdgcn_readfirstlane((int)(unsigned)(u >> 32));
     return __longlong_as_double((long long)(lo | (unsigned long long)hi << 32));
 }
-// c = vf_c(T), lo = vf_floor(M, c), pow2 the table in LDS
+// c = vf_c(T), lo = vf_floor(M, T, c), pow2 the table in LDS
 __device__ __forceinline__ double vf_exp(float l, float M, double c, double lo, const double* pow2) {
     constexpr double MAGIC = 6755399441055744.0;
     const double y = (widen(l) - widen(M)) * c, t = y + MAGIC, f = y - (t - MAGIC);
@@ -267,7 +273,7 @@ verify_stats_kernel(VerifyArgs a) {
     arg = wave_min(arg);
     double sum = 0.0;
     if (T > 0.0f && m > -__builtin_inff()) {
-        const double e = vf_c(T), lo = wave_uniform(vf_floor(m, e));
+        const double e = vf_c(T), lo = wave_uniform(vf_floor(m, T, e));
 #pragma unroll
         for (int k = 0; k < PT; ++k) sum += vf_exp(l[k], m, e, lo, pow2);
         sum = wave_sum(sum);
@@ -282,7 +288,7 @@ verify_stats_kernel(VerifyArgs a) {
         const double e = vf_c(T);
         float M = smax[0];
         for (int w = 1; w < W; ++w) M = fmaxf(M, smax[w]);
-        const double lo = vf_floor(M, e);
+        const double lo = vf_floor(M, T, e);
         double z = 0.0;
         arg = 0x7fffffff;
         for (int w = 0; w < W; ++w) {
@@ -362,7 +368,7 @@ verify_select_kernel(VerifyArgs a) {
         const float mine = M;
         M = wave_max(M);
         arg = wave_min(mine == M ? arg : 0x7fffffff);
-        const double lo = vf_floor(M, e);
+        const double lo = vf_floor(M, T, e);
         double z = head[i].sum * vf_exp(head[i].max, M, e, lo, pow2);
         for (int x = lane + 64; x < a.chunks; x += 64) z += s[x].sum * vf_exp(s[x].max, M, e, lo, pow2);
         z = wave_sum(z);
