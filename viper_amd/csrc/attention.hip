@@ -15,6 +15,9 @@ AttnFn attn_kernels_int8(int D, int qt, int W);
 //  * 80 KB of parts or more of a group of rows are joined by a launch of their own,
 //    below by the workgroup that counts last: 16384 tokens in 64 parts 13.3 us
 //    against 16.1, 512 in 4 parts 8.5 against 7.1 (2 x 16 rows of 8000: 20 against 37).
+// Both limits lie between measured sizes, and both count what the table could hold (the
+// host does not know the lengths): 611 tokens take 6.4 us in a table of 640, 7.5 in one
+// of 4096 (a join launch for 5 parts), 7.0 of 4160 and 8.1 of 32768 (3 parts of 8 waves).
 // Parts of equal steps dealt out over all sequences of a batch, whatever their
 // lengths, were slower (32 x 8192 tokens 92.9 us against 85.7, 256 x 600 76 against
 // 36): a part that ends one sequence and begins another waits at both.

@@ -3,7 +3,7 @@
 // then draw the next token from max(p - q, 0) (or p after the last).
 //
 // Measured: 8 sequences of up to 15 drafted tokens, 166144 logits, the drafter's logits
-// too: 49 us (statistics 23-32, selection 23); one certain draft of 4 tokens, 32000 logits:
+// too: 49 us (statistics 21-27, selection 23); one certain draft of 4 tokens, 32000 logits:
 // 17 us (4 and 12.5, the latency of the selection's steps; the tokens of an octet
 // one after the other, which is half the code, 19.9: their exponentials overlap).
 //
