@@ -562,8 +562,9 @@ int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_batch* batch, 
  * that the row sees: j <= p (its position) and, with window > 0, j > p - window
  * or j < sinks.  max_rows <= VIPER_QLINEAR_MAX_M; heads a multiple of kv_heads
  * (query head h reads key head h / (heads / kv_heads)), at most 64 to one key
- * head; q and out rows of heads * head_dim bf16 values, strides multiples of 8 elements, 16-byte
- * aligned, no row of out overlapping one of q (refused); scale finite and > 0.  Values that a row does not see (masked rows,
+ * head; q and out rows of heads * head_dim bf16 values, strides multiples of 8
+ * elements, 16-byte aligned, no row of out overlapping one of q (refused); scale
+ * finite and > 0.  Values that a row does not see (masked rows,
  * stale or unwritten places of a page) never reach its output, whatever they
  * hold.  The cache's length is split over workgroups that meet through
  * workspace (16-byte aligned, viper_hip_attention_workspace_bytes() bytes, zero

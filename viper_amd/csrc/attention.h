@@ -24,9 +24,10 @@
 // Measured (20 heads over 4 key heads of 128 dims, one row): 600 tokens 6.5 us, 4096 8.4,
 // 131072 45.5 (the stream alone 40.2: 6.7 TB/s); 32 sequences of 8192 85 us (6.3 TB/s), int8
 // 52; 16 rows of 2 sequences of 4100..8000 18.8 us.  Bound by the cache's stream at long
-// contexts (int8 at 5.3 TB/s: 395 VALU instructions a tile to widen codes against 165; sequences of
-// uneven lengths by the longest one's parts), by the latency of one load chain and of the
-// join at short ones and in 16 rows (where MFMA and softmax issue 6 of the 14.4 us).
+// contexts (int8 at 5.3 TB/s: 395 VALU instructions a tile to widen codes against 165;
+// sequences of uneven lengths by the longest one's parts), by the latency of one load
+// chain and of the join at short ones and in 16 rows (where MFMA and softmax issue 6 of
+// the 14.4 us).
 //
 // What a row must not see cannot reach it: masked scores are replaced (not
 // added to), places of the last tile past the length are cleared in V.  So a row's
@@ -235,7 +236,8 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, const KvSeq& sq, 
     s.lo_t = s.nsink = 0;
     if (a.window != 0) {
         const int from = max(0, s.pos0 + 1 > a.window ? s.pos0 + 1 - a.window : 0);
-        s.nsink = (min(min(a.sinks, from), cap) + KV_TILE - 1) / KV_TILE;  // (a length past the table has no more tiles than it)
+        // (a length past the table has no more tiles than it)
+        s.nsink = (min(min(a.sinks, from), cap) + KV_TILE - 1) / KV_TILE;
         s.lo_t = max(from / KV_TILE, s.nsink);
     }
     s.tiles = s.nsink + max(0, (min(s.len, cap) + KV_TILE - 1) / KV_TILE - s.lo_t);
