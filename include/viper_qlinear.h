@@ -477,19 +477,33 @@ int viper_hip_empty_dispatch(int workgroups, int threads, void* y_bf16, void* st
  *
  * A cache is two pools of pages (K and V) of page_size tokens (32, 64, 128 or
  * 256), [num_pages][kv_heads][page_size / 32] tiles of 32 tokens x head_dim
- * (64, 128 or 256) values, bf16 or int8, each tile in the order in which the
+ * (64, 128 or 256) values, bf16, int8 or 4-bit, each tile in the order in which the
  * matrix instructions take it, so that a wave reads whole tiles with
  * contiguous 1 KiB loads straight into operands.  Token t of its tile and
  * dimension d of its row are element
  *   K bf16  512 * (2 * (d / 32) + s) + 8 * (16 * g + m) + d % 8
  *   K int8  1024 * (2 * (d / 64) + s) + 16 * (16 * g + m) + 8 * (d / 32 % 2) + d % 8
  *           with s = t / 4 % 2, m = 4 * (t / 8) + t % 4, g = d / 8 % 4;
+ *   K FP4   2048 * (2 * (d / 128) + s) + 32 * (16 * (d / 32 % 4) + m) + d % 32
+ *           (head_dim 64: 32 * (16 * (d / 16) + m) + 16 * s + d % 16);
  *   V bf16  512 * (d / 16) + 8 * (16 * (t / 8) + d % 16) + t % 8
- *   V int8  1024 * (d / 32) + 16 * (16 * (t / 8) + d % 16) + 8 * (d / 16 % 2) + t % 8.
+ *   V int8  1024 * (d / 32) + 16 * (16 * (t / 8) + d % 16) + 8 * (d / 16 % 2) + t % 8
+ *   V FP4   2048 * (d / 64) + 32 * (16 * (t / 8) + d % 16) + 8 * (d / 16 % 4) + t % 8.
  * int8 rows (the head_dim values of one token and head) have one fp32 scale
  * each, k_scales and v_scales [num_pages][kv_heads][page_size]:
  * s = max(amax / 127, 1e-8), code = RNE(x / s), the activation quantizer's
  * rule over the row.  bf16 caches have no scales (NULL).
+ * FP4 codes are e2m1 (a sign bit, then 0, 0.5, 1, 1.5, 2, 3, 4, 6), element e in
+ * the low (even e) or high half of byte e / 2.  Keys have a power of two for
+ * each 32 dimensions of a token and head, which the products over dimensions take
+ * with the codes: 2^e, e the least in -125 .. 125 with amax <= 7 * 2^e, code =
+ * RNE(x / 2^e), at most 6; k_scales (uint8) holds e + 127, or 255 for a block with
+ * a value that is not finite (it reads back as NaN), in tiles of head_dim bytes,
+ * [num_pages][kv_heads][page_size / 32] of them; with block c = d / 32 byte
+ *   (16 * (c % 4) + m) * (head_dim / 64) + 2 * (c / 4) + s (head_dim 64: 2 * (16 * c + m) + s).
+ * Products over tokens cannot take scales of values, so values have one fp32
+ * scale per row, v_scales as int8 has them: s = max(amax / 6, 1e-8), code =
+ * RNE(x / s) of the fp32 quotient.
  *
  * Reference counterparts: the engine's caches and decode attention
  * (kernels/ops/attn_decode_kernel.cu:35,155,615,727, kernels/ops/q8_kv_cache.cuh)
@@ -497,17 +511,18 @@ int viper_hip_empty_dispatch(int workgroups, int threads, void* y_bf16, void* st
  * window, sinks and verification have none. */
 #define VIPER_KV_BF16 0
 #define VIPER_KV_INT8 1
+#define VIPER_KV_FP4 4
 #define VIPER_KV_TILE 32
 
 typedef struct viper_kv_cache {
-    int32_t kv_type; /* VIPER_KV_BF16 or VIPER_KV_INT8 */
+    int32_t kv_type; /* VIPER_KV_BF16, VIPER_KV_INT8 or VIPER_KV_FP4 */
     int32_t kv_heads;
     int32_t head_dim;  /* 64, 128 or 256 */
     int32_t page_size; /* tokens: 32, 64, 128 or 256 */
     int32_t num_pages;
     void* k; /* the pools, 16-byte aligned */
     void* v;
-    float* k_scales; /* int8 only, 16-byte aligned */
+    void* k_scales;  /* int8 (fp32) and FP4 (uint8) only, 16-byte aligned */
     float* v_scales;
 } viper_kv_cache;
 

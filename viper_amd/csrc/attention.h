@@ -1,5 +1,5 @@
 // Attention of a sequence's newest rows over its pages (one pass, running maximum
-// and sum), instantiated per cache type in attention_{bf16,int8}.hip.
+// and sum), instantiated per cache type in attention_{bf16,int8,fp4}.hip.
 //
 // For a row with query q and the tokens j that it sees:
 //   s_j = scale q . k_j,  o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m),  m = max s_j.
@@ -137,10 +137,11 @@ __device__ __forceinline__ void again_codes(const u32x2& v, float* f) {
 // looked for first).  One workgroup reads the row's K and V at the latency of its loads, rows
 // side by side where the parts are joined by a launch of their own (65536 tokens of 128 dims
 // 3.6 ms), else one after the other (5 rows of 8192 tokens 0.8 ms).
-template <int D, bool I8, int NT>
+template <int D, int KT, int NT>
 __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, const uint16_t* q, uint16_t* o,
                                                     int p, float2 ml, float* lds) {
     constexpr int TILES = NT / KV_TILE, G = NT / D;  // tiles of a chunk of tokens; groups of threads over its octets
+    constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4;
     const int tid = (int)threadIdx.x;
     const Sight sight{a.window, a.sinks};
     const int64_t cap = ((int64_t)a.c.width << a.c.tpl) * KV_TILE;
@@ -170,6 +171,9 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
             for (int c = 0; c < D / 8; ++c) {
                 float k[8], x[8];
                 if constexpr (I8) again_codes(*(const u32x2*)((const int8_t*)a.c.k + base + k_place<true>(t, c)), k);
+                else if constexpr (F4)
+                    fp4_f32(*(const uint32_t*)((const uint8_t*)a.c.k + base / 2 + k4_place<D>(t, c)),
+                            fp4_power(((const uint8_t*)a.c.ks)[at * D + k4_exp_place<D>(t, c / 4)]), k);
                 else again_bf16(*(const u32x4*)((const uint16_t*)a.c.k + base + k_place<false>(t, c)), k);
                 again_bf16(*(const u32x4*)(q + 8 * c), x);
 #pragma unroll
@@ -191,6 +195,10 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
             float v[8];
             if constexpr (I8) {
                 again_codes(*(const u32x2*)((const int8_t*)a.c.v + base + v_place<true>(8 * (i & 3), d)), v);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) v[x] *= a.c.vs[at * KV_TILE + 8 * (i & 3) + x];
+            } else if constexpr (F4) {
+                fp4_f32(*(const uint32_t*)((const uint8_t*)a.c.v + base / 2 + v4_place(8 * (i & 3), d)), 1.0f, v);
 #pragma unroll
                 for (int x = 0; x < 8; ++x) v[x] *= a.c.vs[at * KV_TILE + 8 * (i & 3) + x];
             } else {
@@ -259,12 +267,12 @@ __device__ __forceinline__ bool attn_store(const AttnArgs& a, const AttnSeq& s, 
         u32x2{f2bf2(o[0], o[1]), f2bf2(o[2], o[3])};
     return fine;
 }
-template <int D, bool I8, int NT, int ROWS>
+template <int D, int KT, int NT, int ROWS>
 __device__ __forceinline__ void attn_again(const AttnArgs& a, const AttnSeq& s, int b, int qg, int head, int rr, float2 ml,
                                            float* lds) {
     const int r = qg * ROWS + rr, i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
     const size_t row = (size_t)s.sq.row0 + i, h = (size_t)(head * a.gqa + hh) * D;
-    row_again<D, I8, NT>(a, b, head, a.q + row * a.q_stride + h, a.out + row * a.out_stride + h, s.pos0 + i, ml, lds);
+    row_again<D, KT, NT>(a, b, head, a.q + row * a.q_stride + h, a.out + row * a.out_stride + h, s.pos0 + i, ml, lds);
 }
 
 // Sums of 8 values (row rr, dims d ..) over parts first, first + step, ...
@@ -336,12 +344,13 @@ __device__ __forceinline__ void attn_lay(float* lds, int NT, const AttnSum& s) {
     jm[2 * threadIdx.x + 1] = s.l;
 }
 
-template <int D, bool I8, int QT, int W>
-__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(at_two(D, I8, QT) ? 4 : 1)))
+template <int D, int KT, int QT, int W>
+__global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(at_two(D, KT != VIPER_KV_BF16, QT) ? 4 : 1)))
 attn_kernel(AttnArgs a) {
     constexpr int NT = W * 64;
+    constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4, VS = I8 || F4;  // VS: values have scales
     constexpr int NKB = D / 32, NDB = D / 16, ROWS = QT * 16, ST = D + 4;
-    constexpr int NK = I8 ? NKB : 2 * NKB, NV = I8 ? NDB / 2 : NDB;  // 16-byte loads of a lane per tile
+    constexpr int NK = F4 ? D / 64 : I8 ? NKB : 2 * NKB, NV = F4 ? D / 64 : I8 ? NDB / 2 : NDB;  // 16-byte loads of a lane per tile
     constexpr int SLOTS = at_slots(D, QT, W);
     extern __shared__ __align__(16) u32x4 lq[];  // Q's operands [QT][NKB][64]
     const int LR = a.lrows;
@@ -380,8 +389,8 @@ attn_kernel(AttnArgs a) {
         const int i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
         qv[k] = u32x4{0u, 0u, 0u, 0u};
         if (rr < rows)
-            qv[k] = *(const u32x4*)(a.q + (size_t)(sq.row0 + i) * a.q_stride + (size_t)(head * a.gqa + hh) * D + kb * 32 +
-                                    8 * ((x >> 4) & 3));
+            qv[k] = *(const u32x4*)(a.q + (size_t)(sq.row0 + i) * a.q_stride + (size_t)(head * a.gqa + hh) * D +
+                                    (F4 ? q4_dim<D>(kb, (x >> 4) & 3) : kb * 32 + 8 * ((x >> 4) & 3)));
     }
     int pos[QT];  // position of the lane's row, -1: no row
 #pragma unroll
@@ -403,7 +412,8 @@ attn_kernel(AttnArgs a) {
 
     u32x4 kr[NK], vr[NV];
     u32x4 ksc[2], vsc[2];
-    constexpr int TB = KV_TILE * D * (I8 ? 1 : 2);  // bytes of a tile
+    uint32_t kex = 0;  // FP4: the lane's powers of two, byte 2 (kb / 4) + h
+    constexpr int TB = F4 ? KV_TILE * D / 2 : KV_TILE * D * (I8 ? 1 : 2);  // bytes of a tile
     // A tile that one workgroup reads is not kept (131072 tokens, one row: 58 us
     // instead of 68); several groups of rows read it again from L2.
     constexpr int AUX = QT < at_qt_max(D) && QT <= 2 ? AUX_NT : 0;
@@ -424,11 +434,15 @@ attn_kernel(AttnArgs a) {
         const size_t at = kv_tile_at(a.c, page, head, tile);
         load_tile(a.c.k, at, kr, [] { return NK; });
         if constexpr (I8) load_scales(a.c.ks, at, ksc);
+        if constexpr (F4) {
+            const auto t = buf((const uint8_t*)a.c.ks + at * D, D);
+            kex = D == 256 ? bload4(t, lane * 4) : bload2(t, D == 64 ? (16 * (g >> 1) + l16) * 2 : lane * 2);
+        }
     };
     auto load_v = [&](int page, int tile) {
         const size_t at = kv_tile_at(a.c, page, head, tile);
         load_tile(a.c.v, at, vr, [] { return NV; });
-        if constexpr (I8) load_scales(a.c.vs, at, vsc);
+        if constexpr (VS) load_scales(a.c.vs, at, vsc);
     };
 
     // A tile's K is asked for once the products that read the one before are
@@ -460,7 +474,7 @@ attn_kernel(AttnArgs a) {
         pn = pnn;
         pnn = page_of(v + 2 * stride);
         issue_fence();  // (Q is read again for each tile: its registers go to K and V)
-        if constexpr (I8) {  // (codes are not widened before their tile's turn)
+        if constexpr (VS) {  // (codes are not widened before their tile's turn)
 #pragma unroll
             for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(kr[i]));
         }
@@ -478,6 +492,9 @@ attn_kernel(AttnArgs a) {
                 if constexpr (I8) {
                     const u32x4 w = kr[(kb >> 1) * 2 + h];
                     k = kb & 1 ? codes_bf16(w.z, w.w) : codes_bf16(w.x, w.y);
+                } else if constexpr (F4) {
+                    const uint32_t w = D == 64 ? kr[0][2 * h + kb] : kr[2 * (kb >> 2) + h][kb & 3];
+                    k = __builtin_bit_cast(at_bf16x8, fp4_bf16(w, fp4_power((kex >> (8 * (2 * (kb >> 2) + h))) & 0xffu)));
                 } else {
                     k = __builtin_bit_cast(at_bf16x8, kr[kb * 2 + h]);
                 }
@@ -487,10 +504,10 @@ attn_kernel(AttnArgs a) {
             }
         }
         float kscale[8], vscale[8];
-        if constexpr (I8) {
+        if constexpr (VS) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                kscale[e] = __uint_as_float(ksc[e >> 2][e & 3]) * a.scale;
+                if constexpr (I8) kscale[e] = __uint_as_float(ksc[e >> 2][e & 3]) * a.scale;
                 vscale[e] = __uint_as_float(vsc[e >> 2][e & 3]);
             }
         }
@@ -529,7 +546,7 @@ attn_kernel(AttnArgs a) {
             for (int e = 0; e < 8; ++e) {
                 p[e] = __builtin_amdgcn_exp2f(x[e] - ms);
                 sum += p[e];
-                if constexpr (I8) p[e] = (seen >> e) & 1 ? p[e] * vscale[e] : 0.0f;
+                if constexpr (VS) p[e] = (seen >> e) & 1 ? p[e] * vscale[e] : 0.0f;
             }
             l[qt] = l[qt] * f + sum;
 #pragma unroll
@@ -544,7 +561,7 @@ attn_kernel(AttnArgs a) {
             ph[qt] = __builtin_bit_cast(at_bf16x8, h);
             pl[qt] = __builtin_bit_cast(at_bf16x8, r);
         }
-        if (!I8 && j0 + KV_TILE > len) {  // places past the length hold anything
+        if (!VS && j0 + KV_TILE > len) {  // places past the length hold anything
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
 #pragma unroll
@@ -552,7 +569,7 @@ attn_kernel(AttnArgs a) {
                     vr[i][e] &= (jl + 2 * e < len ? 0xffffu : 0u) | (jl + 2 * e + 1 < len ? 0xffff0000u : 0u);
             }
         }
-        if constexpr (I8) {
+        if constexpr (VS) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(vr[i]));
         }
@@ -562,6 +579,8 @@ attn_kernel(AttnArgs a) {
             if constexpr (I8) {
                 const u32x4 w = vr[db >> 1];
                 vv = db & 1 ? codes_bf16(w.z, w.w) : codes_bf16(w.x, w.y);
+            } else if constexpr (F4) {
+                vv = __builtin_bit_cast(at_bf16x8, fp4_bf16(vr[db >> 2][db & 3], 1.0f));
             } else {
                 vv = __builtin_bit_cast(at_bf16x8, vr[db]);
             }
@@ -681,13 +700,13 @@ attn_kernel(AttnArgs a) {
     }
     __syncthreads();
     for (int rr = 0; rr < rows; ++rr)
-        if ((again[rr >> 5] >> (rr & 31)) & 1u) attn_again<D, I8, NT, ROWS>(a, s, b, qg, head, rr, again_ml[rr], lds);
+        if ((again[rr >> 5] >> (rr & 31)) & 1u) attn_again<D, KT, NT, ROWS>(a, s, b, qg, head, rr, again_ml[rr], lds);
 }
 
 // The join as a launch of its own: a workgroup per row and group of rows, its
 // threads D / 8 values wide and G parts deep.
 constexpr int AT_JNT = 256;
-template <int D, bool I8, int QT, int W>
+template <int D, int KT, int QT, int W>
 __global__ void __launch_bounds__(AT_JNT)
 attn_join_kernel(AttnArgs a) {
     constexpr int ROWS = QT * 16, U = D / 8, G = AT_JNT / U;
@@ -714,36 +733,36 @@ attn_join_kernel(AttnArgs a) {
         again = 1;
     }
     __syncthreads();
-    if (again) attn_again<D, I8, AT_JNT, ROWS>(a, s, b, qg, head, rr, again_ml, lds);
+    if (again) attn_again<D, KT, AT_JNT, ROWS>(a, s, b, qg, head, rr, again_ml, lds);
 }
 
 struct AttnFn {
     const void* attn;
     const void* join;
 };
-template <int D, bool I8, int QT, int W>
+template <int D, int KT, int QT, int W>
 inline AttnFn attn_pair() {
-    return AttnFn{(const void*)attn_kernel<D, I8, QT, W>, (const void*)attn_join_kernel<D, I8, QT, W>};
+    return AttnFn{(const void*)attn_kernel<D, KT, QT, W>, (const void*)attn_join_kernel<D, KT, QT, W>};
 }
-template <int D, bool I8, int QT>
+template <int D, int KT, int QT>
 inline AttnFn attn_of(int W) {
     if constexpr (at_waves(D, QT) == 8)
-        if (W == 8) return attn_pair<D, I8, QT, 8>();
-    return attn_pair<D, I8, QT, 4>();
+        if (W == 8) return attn_pair<D, KT, QT, 8>();
+    return attn_pair<D, KT, QT, 4>();
 }
-template <bool I8>
+template <int KT>
 inline AttnFn attn_fn(int D, int qt, int W) {
     switch (D * 8 + qt) {
-        case 64 * 8 + 1: return attn_of<64, I8, 1>(W);
-        case 64 * 8 + 2: return attn_of<64, I8, 2>(W);
-        case 64 * 8 + 3: return attn_of<64, I8, 3>(W);
-        case 64 * 8 + 4: return attn_of<64, I8, 4>(W);
-        case 128 * 8 + 1: return attn_of<128, I8, 1>(W);
-        case 128 * 8 + 2: return attn_of<128, I8, 2>(W);
-        case 128 * 8 + 3: return attn_of<128, I8, 3>(W);
-        case 128 * 8 + 4: return attn_of<128, I8, 4>(W);
-        case 256 * 8 + 1: return attn_of<256, I8, 1>(W);
-        case 256 * 8 + 2: return attn_of<256, I8, 2>(W);
+        case 64 * 8 + 1: return attn_of<64, KT, 1>(W);
+        case 64 * 8 + 2: return attn_of<64, KT, 2>(W);
+        case 64 * 8 + 3: return attn_of<64, KT, 3>(W);
+        case 64 * 8 + 4: return attn_of<64, KT, 4>(W);
+        case 128 * 8 + 1: return attn_of<128, KT, 1>(W);
+        case 128 * 8 + 2: return attn_of<128, KT, 2>(W);
+        case 128 * 8 + 3: return attn_of<128, KT, 3>(W);
+        case 128 * 8 + 4: return attn_of<128, KT, 4>(W);
+        case 256 * 8 + 1: return attn_of<256, KT, 1>(W);
+        case 256 * 8 + 2: return attn_of<256, KT, 2>(W);
         default: return AttnFn{nullptr, nullptr};
     }
 }

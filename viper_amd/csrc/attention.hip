@@ -6,6 +6,7 @@ namespace vq {
 
 AttnFn attn_kernels_bf16(int D, int qt, int W);
 AttnFn attn_kernels_int8(int D, int qt, int W);
+AttnFn attn_kernels_fp4(int D, int qt, int W);
 
 // One row of 20 heads over 4 key heads, 128 dims:
 //  * 8 waves a CU (one workgroup, each wave a tile in use and one in flight): 131072
@@ -41,7 +42,7 @@ static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int 
     if (tiles <= AT_SHORT) p.waves = 4;
     int64_t s = 1;
     if (base <= AT_CNT) {
-        const bool two = b->batch > 1 && at_two(c->head_dim, c->kv_type == VIPER_KV_INT8, p.qt);
+        const bool two = b->batch > 1 && at_two(c->head_dim, c->kv_type != VIPER_KV_BF16, p.qt);
         const int64_t wgs = (int64_t)device_cus() * AT_WAVES * (two ? 2 : 1) / p.waves;
         s = (wgs + base - 1) / base;
         const int64_t fit = (tiles + p.waves - 1) / p.waves;
@@ -103,7 +104,9 @@ extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const vipe
     a.sinks = sinks;
     a.scale = scale * 1.44269504088896340736f;
     const int D = cache->head_dim;
-    const AttnFn fn = cache->kv_type == VIPER_KV_INT8 ? attn_kernels_int8(D, p.qt, p.waves) : attn_kernels_bf16(D, p.qt, p.waves);
+    const AttnFn fn = cache->kv_type == VIPER_KV_INT8  ? attn_kernels_int8(D, p.qt, p.waves)
+                      : cache->kv_type == VIPER_KV_FP4 ? attn_kernels_fp4(D, p.qt, p.waves)
+                                                       : attn_kernels_bf16(D, p.qt, p.waves);
     if (fn.attn == nullptr) return VIPER_INTERNAL;
     a.by_gqa = (65536u + (unsigned)a.gqa - 1) / (unsigned)a.gqa;
     a.apart = p.splits > 1 && (int64_t)p.splits * p.lrows * D * 4 >= AT_APART;

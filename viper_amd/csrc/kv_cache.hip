@@ -32,7 +32,8 @@ struct AppendArgs {
     const uint16_t* q;
     uint16_t* qo;
     int64_t kv_stride, q_stride, qo_stride;
-    int heads, ub;  // workgroups per row
+    int heads, ub;  // workgroups per row (FP4: per octet of tokens)
+    int octets;     // FP4: that a sequence's rows can touch
     double log2_theta;
 };
 
@@ -56,6 +57,22 @@ __device__ __forceinline__ float unit_max(float v) {
     if constexpr (L >= 8) v = fmaxf(v, dpp_f<DPP_HALF_MIRROR>(v));
     if constexpr (L >= 16) v = fmaxf(v, dpp_f<DPP_MIRROR>(v));
     return v;
+}
+
+// FP4: the exponent of a block of keys whose largest magnitude is m, 2^e the least
+// power with m <= 7 * 2^e (a value over 6 becomes 6, which is as near as 8 would be)
+__device__ __forceinline__ int fp4_exponent(float m) {
+    const uint32_t u = __float_as_uint(m);
+    const int e = (int)(u >> 23) - 129 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+    return min(125, max(-125, e));
+}
+// Codes of 8 values times f, rounded to nearest even and at most 6 in magnitude
+__device__ __forceinline__ uint32_t fp4_codes(const float* x, float f) {
+    uint32_t w = 0;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0] * f, x[1] * f, 1.0f, 0);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2] * f, x[3] * f, 1.0f, 1);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4] * f, x[5] * f, 1.0f, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6] * f, x[7] * f, 1.0f, 3);
 }
 
 template <int D, bool I8, bool ROPE>
@@ -174,6 +191,140 @@ kv_append_kernel(AppendArgs a) {
     if (I8 && o == 0) a.c.vs[at * KV_TILE + t] = scale;
 }
 
+// FP4: two tokens of a value share a byte and eight a word, so a workgroup takes the
+// rows of one octet of tokens (one row of a decode step, eight of a prompt): an octet
+// that the call fills is stored word by word, of others the words' other halves are
+// kept by an atomic that flips the bits that change (no other row of the call
+// changes this row's), whoever else writes the octet.  Angles of all rows are in LDS
+// before the first; a row's values are in flight while the one before is rounded.
+template <int D, bool ROPE>
+__global__ void __launch_bounds__(KA_NT)
+kv_append4_kernel(AppendArgs a) {
+    constexpr int TPU = D / 16, UPB = KA_NT / TPU;
+    __shared__ double cs[8][D / 2], sn[8][D / 2];
+    int id = (int)blockIdx.x;
+    const int ub = id % a.ub;
+    id /= a.ub;
+    const int b = id / a.octets, oc = id % a.octets;
+    const KvSeq s = kv_seq(a.c, b);
+    const int64_t p0 = (int64_t)s.len - s.n;  // position of row 0
+    const int64_t from = p0 < 0 ? 0 : p0;
+    const int64_t lo64 = (from / 8 + oc) * 8;
+    if (s.n == 0 || lo64 >= s.len) return;
+    const int lo = (int)lo64;
+    const int t0 = (int)(from > lo64 ? from - lo64 : 0), t1 = min(8, s.len - lo);  // rows of the octet
+    const int tid = (int)threadIdx.x;
+    const int unit = ub * UPB + tid / TPU, o = tid % TPU;
+    const int nq = ROPE && a.q != nullptr ? a.heads : 0;
+    const bool is_q = unit < nq, is_k = !is_q && unit < nq + a.c.kvh, live = unit < nq + 2 * a.c.kvh;
+    const int head = is_q ? unit : (unit - nq) % a.c.kvh;
+    const size_t row0 = (size_t)(s.row0 + ((int64_t)lo - p0));  // row of the octet's token 0
+    const int64_t stride = is_q ? a.q_stride : a.kv_stride;
+    const uint16_t* src = (is_q ? a.q : is_k ? a.k : a.v) + (size_t)head * D + 8 * o;
+    u32x4 n0 = {0u, 0u, 0u, 0u}, n1 = n0;
+    auto fetch = [&](int t) {
+        if (!live || t >= t1) return;
+        const uint16_t* p = src + (row0 + t) * stride;
+        n0 = *(const u32x4*)p;
+        n1 = *(const u32x4*)(p + D / 2);
+    };
+    fetch(t0);
+    const int tile = lo / KV_TILE, tt = lo % KV_TILE;
+    const int page = is_q ? -1 : kv_page(a.c, b, tile);
+    const size_t at = page >= 0 ? kv_tile_at(a.c, page, head, tile) : 0;
+    uint8_t* const kt = (uint8_t*)a.c.k + at * (KV_TILE * D / 2);
+    uint8_t* const vt = (uint8_t*)a.c.v + at * (KV_TILE * D / 2);
+    const bool is_v = live && !is_q && !is_k && page >= 0, full = t0 == 0 && t1 == 8;
+    uint32_t words[16], old[16];
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        words[j] = old[j] = 0u;
+        if (is_v && !full) old[j] = *(const uint32_t*)(vt + v4_place(tt, (j < 8 ? 8 * o : D / 2 + 8 * o - 8) + j));
+    }
+    if constexpr (ROPE) {
+        for (int i = t0 * (D / 2) + tid; i < t1 * (D / 2); i += KA_NT) {
+            const int t = i / (D / 2), d = i % (D / 2);
+            const double f = exp2(-(double)d * (2.0 / D) * a.log2_theta);
+            double sv, cv;
+            sincos((double)(lo + t) * f, &sv, &cv);
+            cs[t][d] = cv;
+            sn[t][d] = sv;
+        }
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        u32x4 x0 = n0, x1 = n1;
+        fetch(t + 1);
+        float f0[8], f1[8];
+        to_f32(x0, f0);
+        to_f32(x1, f1);
+        if (ROPE && (is_q || is_k)) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const double c = cs[t][8 * o + j], n = sn[t][8 * o + j], u = (double)f0[j], w = (double)f1[j];
+                f0[j] = (float)(u * c - w * n);
+                f1[j] = (float)(w * c + u * n);
+            }
+            x0 = to_bf16(f0);
+            x1 = to_bf16(f1);
+            if (is_q) {
+                uint16_t* dst = a.qo + (row0 + t) * a.qo_stride + (size_t)head * D + 8 * o;
+                *(u32x4*)dst = x0;
+                *(u32x4*)(dst + D / 2) = x1;
+            }
+            to_f32(x0, f0);
+            to_f32(x1, f1);
+        }
+        // blocks of 32 dims are four lanes' octets, on either side of the row's middle
+        float m0 = 0.0f, m1 = 0.0f, bad0 = 0.0f, bad1 = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            m0 = fmaxf(m0, fabsf(f0[j]));
+            m1 = fmaxf(m1, fabsf(f1[j]));
+            bad0 += f0[j] * 0.0f;  // NaN where a value is not finite
+            bad1 += f1[j] * 0.0f;
+        }
+        m0 = group_max<4>(m0);
+        m1 = group_max<4>(m1);
+        bad0 = group_max<4>(bad0 == bad0 ? 0.0f : 1.0f);
+        bad1 = group_max<4>(bad1 == bad1 ? 0.0f : 1.0f);
+        if (is_k && page >= 0) {
+            const int e0 = fp4_exponent(m0), e1 = fp4_exponent(m1);
+            *(uint32_t*)(kt + k4_place<D>(tt + t, o)) = fp4_codes(f0, __uint_as_float((uint32_t)(127 - e0) << 23));
+            *(uint32_t*)(kt + k4_place<D>(tt + t, o + TPU)) = fp4_codes(f1, __uint_as_float((uint32_t)(127 - e1) << 23));
+            if (o % 4 == 0) {
+                uint8_t* const ex = (uint8_t*)a.c.ks + at * D;
+                ex[k4_exp_place<D>(tt + t, o / 4)] = (uint8_t)(bad0 != 0.0f ? 255 : e0 + 127);
+                ex[k4_exp_place<D>(tt + t, (o + TPU) / 4)] = (uint8_t)(bad1 != 0.0f ? 255 : e1 + 127);
+            }
+        }
+        const float amax = unit_max<TPU>(fmaxf(m0, m1)), bad = unit_max<TPU>(fmaxf(bad0, bad1));
+        if (is_v) {
+            const float scale = fmaxf(amax / 6.0f, 1e-8f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                f0[j] /= scale;
+                f1[j] /= scale;
+            }
+            const uint32_t c0 = fp4_codes(f0, 1.0f), c1 = fp4_codes(f1, 1.0f);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                words[j] |= ((c0 >> (4 * j)) & 15u) << (4 * t);
+                words[8 + j] |= ((c1 >> (4 * j)) & 15u) << (4 * t);
+            }
+            if (o == 0) a.c.vs[at * KV_TILE + tt + t] = bad != 0.0f ? __uint_as_float(0x7fc00000u) : scale;
+        }
+    }
+    if (!is_v) return;
+    const uint32_t mine = (t1 == 8 ? 0xffffffffu : (1u << (4 * t1)) - 1u) & (0xffffffffu << (4 * t0));
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        uint32_t* const p = (uint32_t*)(vt + v4_place(tt, (j < 8 ? 8 * o : D / 2 + 8 * o - 8) + j));
+        if (full) *p = words[j];
+        else __hip_atomic_fetch_xor(p, (old[j] ^ words[j]) & mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+
 // read: a workgroup per tile of 32 tokens, pool (K, V) and head, of 64 dims two heads
 // whose loads are in flight together (a workgroup's chain of length, page and tile
 // takes longer than moving so small a tile).  K octets go straight to their rows; V turns
@@ -191,9 +342,10 @@ struct ReadArgs {
 // 16 sequences 3.1 / 3.4 / 4.3; 4 heads of 128 dims, 4096 rows of 64: 1 head 4.3, 4 7.6)
 constexpr int kr_heads(int D) { return D == 64 ? 2 : 1; }
 
-template <int D, bool I8>
+template <int D, int KT>
 __global__ void __launch_bounds__(KA_NT)
 kv_read_kernel(ReadArgs a) {
+    constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4;
     constexpr int OPR = D / 8, HG = kr_heads(D);                 // octets of a row, heads
     constexpr int PT = KV_TILE * OPR / KA_NT;                    // octets of a head and thread
     __shared__ __align__(16) uint16_t lv[HG][KV_TILE][D + 8];
@@ -223,6 +375,11 @@ kv_read_kernel(ReadArgs a) {
 #pragma unroll
         for (int k = 0; k < PT; ++k) {
             const int i = tid + k * KA_NT;
+            if constexpr (F4) {
+                const int e = side == 0 ? k4_place<D>(i / OPR, i % OPR) : v4_place(8 * (i / D), i % D);
+                x[h][k] = u32x4{*(const uint32_t*)((const uint8_t*)pool + base / 2 + e), 0u, 0u, 0u};
+                continue;
+            }
             const int e = side == 0 ? k_place<I8>(i / OPR, i % OPR) : v_place<I8>(8 * (i / D), i % D);
             if constexpr (I8) {
                 const u32x2 w = *(const u32x2*)((const int8_t*)pool + base + e);
@@ -240,7 +397,12 @@ kv_read_kernel(ReadArgs a) {
     for (int h = 0; h < HG; ++h) {
         if (h >= heads) continue;
         const float* sc = nullptr;
-        if (I8 && page >= 0) sc = scales + kv_tile_at(a.c, page, head0 + h, tile) * KV_TILE;
+        const uint8_t* ex = nullptr;
+        if ((I8 || F4) && page >= 0) {
+            const size_t at = kv_tile_at(a.c, page, head0 + h, tile);
+            sc = scales + at * KV_TILE;
+            ex = (const uint8_t*)a.c.ks + at * D;
+        }
 #pragma unroll
         for (int k = 0; k < PT; ++k) {
             const int i = tid + k * KA_NT;
@@ -255,6 +417,16 @@ kv_read_kernel(ReadArgs a) {
                 for (int j = 0; j < 8; ++j)
                     y[j] = (float)(int8_t)((j < 4 ? v.x : v.y) >> (8 * (j & 3))) * (side == 0 ? sc[i / OPR] : sc[8 * (i / D) + j]);
                 v = to_bf16(y);
+            } else if constexpr (F4) {
+                if (side == 0) {
+                    v = fp4_bf16(v.x, fp4_power(ex[k4_exp_place<D>(i / OPR, i % OPR / 4)]));
+                } else {
+                    float y[8];
+                    fp4_f32(v.x, 1.0f, y);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] *= sc[8 * (i / D) + j];
+                    v = to_bf16(y);
+                }
             }
             if (side == 0) {
                 store(h, i / OPR, i % OPR, v);
@@ -284,8 +456,14 @@ static const void* append_fn(bool i8, bool rope) {
     return rope ? (const void*)kv_append_kernel<D, false, true> : (const void*)kv_append_kernel<D, false, false>;
 }
 template <int D>
-static const void* read_fn(bool i8) {
-    return i8 ? (const void*)kv_read_kernel<D, true> : (const void*)kv_read_kernel<D, false>;
+static const void* append4_fn(bool rope) {
+    return rope ? (const void*)kv_append4_kernel<D, true> : (const void*)kv_append4_kernel<D, false>;
+}
+template <int D>
+static const void* read_fn(int kv) {
+    return kv == VIPER_KV_INT8  ? (const void*)kv_read_kernel<D, VIPER_KV_INT8>
+           : kv == VIPER_KV_FP4 ? (const void*)kv_read_kernel<D, VIPER_KV_FP4>
+                                : (const void*)kv_read_kernel<D, VIPER_KV_BF16>;
 }
 
 constexpr int64_t GRID_MAX = (1 << 24) - 1;  // workgroups of 256 threads: under 2^32 threads
@@ -336,10 +514,12 @@ extern "C" int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_b
     const int units = a.heads + 2 * cache->kv_heads, upb = KA_NT / (D / 16);
     a.ub = (units + upb - 1) / upb;
     a.c.max_rows = rows_most(batch);
-    const int64_t grid = (int64_t)batch->batch * a.c.max_rows * a.ub;
+    const bool i8 = cache->kv_type == VIPER_KV_INT8, f4 = cache->kv_type == VIPER_KV_FP4;
+    a.octets = (int)(((int64_t)a.c.max_rows + 6) / 8 + 1);
+    const int64_t grid = (int64_t)batch->batch * (f4 ? a.octets : a.c.max_rows) * a.ub;
     if (grid > GRID_MAX) return VIPER_INVALID_ARGUMENT;
-    const bool i8 = cache->kv_type == VIPER_KV_INT8;
-    const void* fn = D == 64 ? append_fn<64>(i8, rope) : D == 128 ? append_fn<128>(i8, rope) : append_fn<256>(i8, rope);
+    const void* fn = f4 ? (D == 64 ? append4_fn<64>(rope) : D == 128 ? append4_fn<128>(rope) : append4_fn<256>(rope))
+                     : D == 64 ? append_fn<64>(i8, rope) : D == 128 ? append_fn<128>(i8, rope) : append_fn<256>(i8, rope);
     void* args[] = {&a};
     launch(fn, (unsigned)grid, KA_NT, 0, (hipStream_t)stream, args);
     return status_of(hipGetLastError());
@@ -365,8 +545,8 @@ extern "C" int viper_hip_kv_read(const viper_kv_cache* cache, const viper_kv_bat
     a.groups = (cache->kv_heads + kr_heads(cache->head_dim) - 1) / kr_heads(cache->head_dim);
     const int64_t grid = (int64_t)batch->batch * tiles * a.groups * 2;
     if (grid > GRID_MAX) return VIPER_INVALID_ARGUMENT;
-    const bool i8 = cache->kv_type == VIPER_KV_INT8;
-    const void* fn = cache->head_dim == 64 ? read_fn<64>(i8) : cache->head_dim == 128 ? read_fn<128>(i8) : read_fn<256>(i8);
+    const int kv = cache->kv_type;
+    const void* fn = cache->head_dim == 64 ? read_fn<64>(kv) : cache->head_dim == 128 ? read_fn<128>(kv) : read_fn<256>(kv);
     void* args[] = {&a};
     launch(fn, (unsigned)grid, KA_NT, 0, (hipStream_t)stream, args);
     return status_of(hipGetLastError());

@@ -15,7 +15,7 @@ struct KvArgs {
     const int32_t* offs;   // [batch + 1] or null
     void* k;
     void* v;
-    float* ks;
+    float* ks;  // (FP4: bytes)
     float* vs;
     int batch, max_rows, total_rows, width;
     int kvh, pages, tpl;  // tiles of a page: 1 << tpl
@@ -39,6 +39,45 @@ __device__ __forceinline__ int v_place(int t, int d) {
     const int lane = 16 * (t >> 3) + (d & 15);
     return I8 ? 1024 * (d >> 5) + 16 * lane + 8 * ((d >> 4) & 1) + (t & 7) : 512 * (d >> 4) + 8 * lane + (t & 7);
 }
+
+// FP4 tiles, in bytes: octet c of token t of a K tile is one word, and so are 8
+// tokens of dim d of a V tile.  A lane's 16 bytes of K are 32 (head_dim 64: 16)
+// consecutive dims of its token, so that they share a power of two.  The first
+// product's k-slots are then dims q4_dim() and not kb * 32 + 8 g, for Q as well.
+template <int D>
+__device__ __forceinline__ int k4_place(int t, int c) {
+    const int s = (t >> 2) & 1, m = 4 * (t >> 3) + (t & 3);
+    return D == 64 ? 16 * (16 * (c >> 1) + m) + 8 * s + 4 * (c & 1)
+                   : 1024 * (2 * (c >> 4) + s) + 16 * (16 * ((c >> 2) & 3) + m) + 4 * (c & 3);
+}
+__device__ __forceinline__ int v4_place(int t, int d) {
+    return 1024 * (d >> 6) + 16 * (16 * (t >> 3) + (d & 15)) + 4 * ((d >> 4) & 3);
+}
+// Byte of block c (of 32 dims) of token t in a tile's powers of two
+template <int D>
+__device__ __forceinline__ int k4_exp_place(int t, int c) {
+    const int s = (t >> 2) & 1, m = 4 * (t >> 3) + (t & 3);
+    return D == 64 ? 2 * (16 * c + m) + s : (16 * (c & 3) + m) * (D / 64) + 2 * (c >> 2) + s;
+}
+template <int D>
+__device__ __forceinline__ int q4_dim(int kb, int g) {
+    return D == 64 ? 16 * g + 8 * kb : 128 * (kb >> 2) + 32 * g + 8 * (kb & 3);
+}
+// 8 codes of a word times the power of two of `scale` (only its exponent counts,
+// NaN's makes NaN), one instruction for two of them; exact
+__device__ __forceinline__ u32x4 fp4_bf16(uint32_t w, float scale) {
+    return u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3))};
+}
+__device__ __forceinline__ void fp4_f32(uint32_t w, float scale, float* f) {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 1),
+               c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, scale, 3);
+    f[0] = a[0], f[1] = a[1], f[2] = b[0], f[3] = b[1], f[4] = c[0], f[5] = c[1], f[6] = d[0], f[7] = d[1];
+}
+// The power of two that a byte of k_scales stands for
+__device__ __forceinline__ float fp4_power(uint32_t byte) { return __uint_as_float(byte << 23); }
 
 // Wave-uniform reads of the arrays through the scalar cache (read-only within a
 // launch), so that a page's number is in scalar registers and its wait does not

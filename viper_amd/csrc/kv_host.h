@@ -8,14 +8,15 @@ namespace vq {
 
 inline int kv_check(const viper_kv_cache* c, const viper_kv_batch* b) {
     if (c == nullptr || b == nullptr) return VIPER_INVALID_ARGUMENT;
-    if (c->kv_type != VIPER_KV_BF16 && c->kv_type != VIPER_KV_INT8) return VIPER_INVALID_ARGUMENT;
+    if (c->kv_type != VIPER_KV_BF16 && c->kv_type != VIPER_KV_INT8 && c->kv_type != VIPER_KV_FP4)
+        return VIPER_INVALID_ARGUMENT;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return VIPER_INVALID_ARGUMENT;
     if (c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
         return VIPER_INVALID_ARGUMENT;
     if (c->kv_heads <= 0 || c->kv_heads > 1024 || c->num_pages <= 0) return VIPER_INVALID_ARGUMENT;
     if (c->k == nullptr || c->v == nullptr || misaligned(c->k, 16) || misaligned(c->v, 16)) return VIPER_INVALID_ARGUMENT;
     const bool scales = c->k_scales != nullptr && c->v_scales != nullptr;
-    if (c->kv_type == VIPER_KV_INT8) {
+    if (c->kv_type != VIPER_KV_BF16) {
         if (!scales || misaligned(c->k_scales, 16) || misaligned(c->v_scales, 16)) return VIPER_INVALID_ARGUMENT;
     } else if (c->k_scales != nullptr || c->v_scales != nullptr) {
         return VIPER_INVALID_ARGUMENT;
@@ -36,7 +37,7 @@ inline KvArgs kv_args(const viper_kv_cache* c, const viper_kv_batch* b) {
     a.offs = b->row_offsets;
     a.k = c->k;
     a.v = c->v;
-    a.ks = c->k_scales;
+    a.ks = (float*)c->k_scales;
     a.vs = c->v_scales;
     a.batch = b->batch;
     a.max_rows = b->max_rows;

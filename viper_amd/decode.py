@@ -27,6 +27,7 @@ from .qlinear import Status, StatusCode, _status, lib, ptr
 class KVType(enum.IntEnum):
     BF16 = 0
     INT8 = 1
+    FP4 = 4
 
 
 class _Fixed:
@@ -52,7 +53,8 @@ class _CBatch(C.Structure):
 class KVCache(_Fixed):
     """Pages of keys and values of one layer: ``k`` and ``v`` bf16 or int8 tensors of num_pages * kv_heads * page_size *
     head_dim elements (their order within a page: include/viper_qlinear.h), ``k_scales`` and ``v_scales`` fp32
-    [num_pages, kv_heads, page_size] for int8."""
+    [num_pages, kv_heads, page_size] for int8.  FP4: two elements to a byte of ``k`` and ``v`` (uint8), ``k_scales`` uint8
+    [num_pages, kv_heads, page_size, head_dim / 32], the exponents of blocks of 32 dimensions, ``v_scales`` as for int8."""
     kv_type: KVType
     k: Any
     v: Any
@@ -64,24 +66,27 @@ class KVCache(_Fixed):
     num_pages: int = field(init=False, default=0)
 
     def __post_init__(self):
-        i8 = KVType(self.kv_type) == KVType.INT8
+        bf16, f4 = KVType(self.kv_type) == KVType.BF16, KVType(self.kv_type) == KVType.FP4
         for t in (self.k, self.v):
-            _typed(t, _INT8 if i8 else _BF16)
-        for t in (self.k_scales, self.v_scales):
-            _typed(t, _FP32)
-        size = 1 if i8 else 2
-        page = self.kv_heads * self.page_size * self.head_dim
+            _typed(t, _BF16 if bf16 else _INT8)
+        _typed(self.k_scales, _INT8 if f4 else _FP32)
+        _typed(self.v_scales, _FP32)
+        size = 2 if bf16 else 1
+        page = self.kv_heads * self.page_size * self.head_dim // (2 if f4 else 1)
         if page <= 0 or self.k.numel() != self.v.numel() or self.k.numel() % page:
             raise ValueError("KVCache: k and v hold whole pages of kv_heads * page_size * head_dim elements")
         self.num_pages = self.k.numel() // page
         if (self.k_scales is None) != (self.v_scales is None):
             raise ValueError("KVCache: k_scales and v_scales go together")
-        if self.k_scales is not None and not all(_laid(t, (self.num_pages, self.kv_heads, self.page_size))
-                                                 for t in (self.k_scales, self.v_scales)):
+        rows = (self.num_pages, self.kv_heads, self.page_size)
+        if self.k_scales is not None and not _laid(self.v_scales, rows):
             raise ValueError("KVCache: one scale for each token and head, [num_pages, kv_heads, page_size]")
+        if self.k_scales is not None and not (_laid(self.k_scales, (*rows, self.head_dim // 32)) if f4 else _laid(self.k_scales, rows)):
+            raise ValueError("KVCache: one scale for each token and head (FP4 keys: and 32 dimensions), [num_pages, kv_heads, "
+                             "page_size] (head_dim / 32)")
         _one_device(self.k, self.v, self.k_scales, self.v_scales)
         self._c = _CCache(int(self.kv_type), self.kv_heads, self.head_dim, self.page_size, self.num_pages, ptr(self.k, size),
-                          ptr(self.v, size), ptr(self.k_scales, 4), ptr(self.v_scales, 4))
+                          ptr(self.v, size), ptr(self.k_scales, 1 if f4 else 4), ptr(self.v_scales, 4))
         self._dev = self.k.get_device()
         self._width = self.kv_heads * self.head_dim
         self._scale = 1.0 / math.sqrt(self.head_dim)
@@ -90,11 +95,18 @@ class KVCache(_Fixed):
     @classmethod
     def empty(cls, kv_type, num_pages, page_size, kv_heads, head_dim, device="cuda"):
         """A cache of zeroed pages."""
-        i8 = int(kv_type) == KVType.INT8
-        shape = (num_pages, kv_heads, page_size // 32, 32 * head_dim)
-        pool = lambda: torch.zeros(shape, dtype=torch.int8 if i8 else torch.bfloat16, device=device)
-        scales = lambda: torch.zeros((num_pages, kv_heads, page_size), dtype=torch.float32, device=device) if i8 else None
-        return cls(KVType(kv_type), pool(), pool(), page_size, kv_heads, head_dim, scales(), scales())
+        kv_type = KVType(kv_type)
+        f4 = kv_type == KVType.FP4
+        shape = (num_pages, kv_heads, page_size // 32, (16 if f4 else 32) * head_dim)
+        dtype = {KVType.BF16: torch.bfloat16, KVType.INT8: torch.int8, KVType.FP4: torch.uint8}[kv_type]
+        pool = lambda: torch.zeros(shape, dtype=dtype, device=device)
+        rows = (num_pages, kv_heads, page_size)
+        ks = vs = None
+        if kv_type != KVType.BF16:
+            vs = torch.zeros(rows, dtype=torch.float32, device=device)
+            # (every exponent's least: blocks of zeros)
+            ks = torch.full((*rows, head_dim // 32), 2, dtype=torch.uint8, device=device) if f4 else torch.zeros_like(vs)
+        return cls(kv_type, pool(), pool(), page_size, kv_heads, head_dim, ks, vs)
 
 
 @dataclass
