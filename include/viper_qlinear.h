@@ -61,6 +61,9 @@
  *                                   (kernels/ops/attn_decode_kernel.cu:35,155,615)
  *                                   over a paged cache, with a window and
  *                                   first tokens that stay visible.
+ *   viper_hip_kv_page_bounds, viper_hip_select_pages, viper_hip_attention_selected
+ *                                   no counterpart: attention over the pages that
+ *                                   a bound on their keys' scores picks.
  *   viper_hip_verify_draft          no counterpart: drafted tokens against the
  *                                   target's probabilities.
  *   viper_hip_qlinear_partials      no counterpart: the same kernels, also writing
@@ -590,6 +593,48 @@ size_t viper_hip_attention_workspace_bytes(const viper_kv_cache* cache, const vi
 int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16,
                               int64_t q_stride, int heads, float scale, int window, int sinks, void* out_bf16,
                               int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Attention over selected pages: viper_hip_kv_page_bounds keeps the range of every
+ * page's keys, viper_hip_select_pages ranks a sequence's pages by it for each new
+ * row and key head, viper_hip_attention_selected looks at the pages of such lists
+ * (of these or others).
+ *
+ * bounds (bf16 [num_pages][kv_heads][2][head_dim], 16-byte aligned, apart from the
+ * cache): of every page that one of the batch's rows (any max_rows) lies on, the
+ * least and the largest value of each dimension over the keys that the sequence
+ * holds there, as kv_read gives them back; both NaN where a key is.  Other pages'
+ * are left as they were, so a call after every kv_append of a batch keeps them all.
+ * A page that two sequences of one call hold unequal parts of gets those of either. */
+int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper_kv_batch* batch, void* bounds_bf16, void* stream);
+
+/* selected int32 [total_rows][kv_heads][count]: the pages that a row at position p
+ * is to look at for the query heads of a key head, as numbers in its sequence
+ * (token j lies on page j / page_size), in order, then -1.  Of its pages 0 ..
+ * p / page_size the first `first` and the last `last` (>= 1) are listed; of the
+ * others those with the largest scores (of equal ones the first) until `count`
+ * (>= first + last) are.  A page's score bounds scale * q . k from above, for
+ * every scale: max over the heads' q of sum_d max(q_d lo_d, q_d hi_d), summed in
+ * 64 bits and rounded to fp32, NaN as +inf; pages that the table lacks have none and
+ * are listed only among the first and last.  Rows at negative positions list none;
+ * pages past the table are not considered.  max_rows <= VIPER_QLINEAR_MAX_M, heads
+ * as for viper_hip_attention_paged, count * page_size < 2^31, batch kv_heads
+ * ceil(table_width head_dim / 2048) < 2^24.  selected and workspace (16-byte
+ * aligned, viper_hip_select_pages_workspace_bytes() bytes, of any content; calls in
+ * flight on one race) overlap neither the inputs nor one another (refused). */
+size_t viper_hip_select_pages_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads, int count);
+int viper_hip_select_pages(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16, int64_t q_stride,
+                           int heads, const void* bounds_bf16, int first, int last, int32_t* selected, int count,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/* viper_hip_attention_paged over the tokens j <= p of the listed pages alone:
+ * selected int32 [total_rows][kv_heads][count], a list for each row and key head, in
+ * any order.  Entries that are negative or past p's page are none; a page listed
+ * twice counts twice; a row whose list has no page is zero.  The rest, the
+ * workspace's rules among it, is as there. */
+size_t viper_hip_attention_selected_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads, int count);
+int viper_hip_attention_selected(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16, int64_t q_stride,
+                                 int heads, float scale, const int32_t* selected, int count, void* out_bf16, int64_t out_stride,
+                                 void* workspace, size_t workspace_bytes, void* stream);
 
 /* Verification of drafted tokens (speculative sampling) for B sequences of up to
  * R - 1 drafted tokens, R <= VIPER_QLINEAR_MAX_M rows of target logits each

@@ -1,0 +1,85 @@
+"""What the calls for selected pages refuse before any launch, and their workspaces (no GPU)."""
+import numpy as np
+import pytest
+
+import pages_ref as P
+import viper_amd as va
+from test_decode_refusals import BAD_BATCH, BAD_CACHE, FAKE, INVALID, OK, batch, cache, ref
+
+torch = pytest.importorskip("torch")
+BIG = 1 << 40  # another place than FAKE
+
+
+def calls(c, b, **kw):
+    L = va.lib()
+    a = dict(q=FAKE, qs=2560, heads=20, bounds=2 * BIG, first=1, last=2, sel=3 * BIG, count=16, ws=BIG, nws=1 << 30, scale=0.1, out=4 * BIG,
+             os=2560)
+    a.update(kw)
+    return [
+        L.viper_hip_kv_page_bounds(ref(c), ref(b), a["bounds"], None),
+        L.viper_hip_select_pages(ref(c), ref(b), a["q"], a["qs"], a["heads"], a["bounds"], a["first"], a["last"], a["sel"], a["count"],
+                                 a["ws"], a["nws"], None),
+        L.viper_hip_attention_selected(ref(c), ref(b), a["q"], a["qs"], a["heads"], a["scale"], a["sel"], a["count"], a["out"], a["os"],
+                                       a["ws"], a["nws"], None)]
+
+
+def sizes(c, b, heads=20, count=16):
+    L = va.lib()
+    return [f(ref(c), ref(b), heads, count) for f in (L.viper_hip_select_pages_workspace_bytes, L.viper_hip_attention_selected_workspace_bytes)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHE)
+def test_bad_cache(bad):
+    assert calls(cache(**bad), batch()) == [INVALID] * 3 and sizes(cache(**bad), batch()) == [0, 0]
+
+
+@pytest.mark.parametrize("bad", BAD_BATCH)
+def test_bad_batch(bad):
+    assert calls(cache(), batch(**bad)) == [INVALID] * 3 and sizes(cache(), batch(**bad)) == [0, 0]
+
+
+def test_null_descriptions_and_no_rows():
+    assert calls(None, batch()) == [INVALID] * 3 and calls(cache(), None) == [INVALID] * 3
+    assert calls(cache(), batch(total_rows=0, row_offsets=FAKE)) == [OK] * 3
+
+
+@pytest.mark.parametrize("bad", [dict(bounds=None), dict(bounds=2 * BIG + 8), dict(bounds=FAKE)])
+def test_bounds_refusals(bad):
+    assert calls(cache(), batch(), **bad)[0] == INVALID  # (FAKE: the cache's keys)
+
+
+@pytest.mark.parametrize("bad", [dict(q=None), dict(q=FAKE + 2), dict(qs=2552), dict(qs=2564), dict(heads=0), dict(heads=18), dict(heads=-4),
+                                 dict(heads=4 * 65, qs=4 * 65 * 128), dict(bounds=None), dict(bounds=2 * BIG + 2), dict(first=-1), dict(last=0),
+                                 dict(last=-1), dict(first=15), dict(first=2 ** 31 - 1, last=2 ** 31 - 1), dict(count=0), dict(count=-1),
+                                 dict(count=1 << 25), dict(sel=None), dict(sel=3 * BIG + 2), dict(ws=None), dict(ws=BIG + 4), dict(nws=16),
+                                 dict(sel=BIG), dict(sel=FAKE), dict(sel=2 * BIG), dict(ws=FAKE), dict(ws=2 * BIG)])
+def test_select_refusals(bad):
+    assert calls(cache(), batch(), **bad)[1] == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(q=None), dict(q=FAKE + 2), dict(qs=2552), dict(heads=0), dict(heads=18), dict(out=None), dict(out=FAKE),
+                                 dict(out=4 * BIG + 8), dict(os=100), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")),
+                                 dict(count=0), dict(count=1 << 25), dict(sel=None), dict(sel=3 * BIG + 1), dict(ws=BIG + 8), dict(nws=16)])
+def test_attention_refusals(bad):
+    # (two rows of 256 listed pages: a call that is split)
+    assert calls(cache(), batch(), **{"count": 256, **bad})[2] == INVALID
+
+
+def test_rows_are_a_verify_steps():
+    b = batch(max_rows=17, total_rows=34)
+    assert calls(cache(), b)[1:] == [INVALID] * 2 and sizes(cache(), b) == [0, 0]
+
+
+def test_workspaces():
+    assert sizes(cache(), batch())[0] == 2 * 4 * 4 * 4  # a score of each row, key head and page
+    c, one, many = cache(), batch(batch=1, total_rows=1), batch(batch=4096, total_rows=4096)
+    assert sizes(c, one, count=1)[1] == 0 and sizes(c, one, count=512)[1] > 8192 and sizes(c, many, count=512)[1] == 0
+
+
+def test_tensors():
+    pool = torch.zeros((8, 4, 2, 32 * 128), dtype=torch.bfloat16)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        va.KVCache(va.KVType.BF16, pool, pool, 64, 4, 128)  # (host memory: no cache to call with)
+    assert P.select(np.ones((1, 2)), np.zeros((9, 2, 2)), [3, -1, 5, 6, 8, 7], 9, 32, 191, 1, 1, 4) == [0, 2, 3, 5]
+    assert i32(1).dtype == torch.int32

@@ -9,5 +9,6 @@ from .qlinear import (GROUP, MAX_M, Prologue, QType, QuantizedWeight, ScaleEnc, 
                       linear_bf16, rmsnorm_quantize, sampling_greedy, greedy_workspace_bytes, swiglu_quantize,
                       workspace_bytes, workspace_layout, frag_bytes, rmsnorm_quantize_frag, swiglu_quantize_frag,
                       linear_prequantized_frag, linear_fused2_prequantized_frag, frag_workspace_bytes)
-from .decode import (KVBatch, KVCache, KVType, attention_paged, attention_workspace_bytes, kv_append, kv_read,  # noqa: F401
-                     verify_draft, verify_workspace_bytes)
+from .decode import (KVBatch, KVCache, KVType, attention_paged, attention_selected,  # noqa: F401
+                     attention_selected_workspace_bytes, attention_workspace_bytes, kv_append, kv_page_bounds, kv_read,
+                     select_pages, select_workspace_bytes, verify_draft, verify_workspace_bytes)

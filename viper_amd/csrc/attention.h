@@ -71,6 +71,29 @@ struct AttnArgs {
     unsigned by_gqa;  // ceil(2^16 / gqa): r / gqa = (r * by_gqa) >> 16 for r < 1024 (gqa <= 64)
     int apart;      // parts are joined by a launch of their own
     float scale;  // times log2 e
+    const int32_t* sel;  // [row][key head][count] pages that are looked at (SEL)
+    int count;
+};
+
+// The list of a row and key head (SEL): tile number vt of it is a tile of the sequence,
+// -1 where the entry is none (negative, or past the row's position p)
+struct AttnList {
+    const int32_t* at;
+    int count, tpl, most;  // most: the page of p
+    __device__ __forceinline__ AttnList(const AttnArgs& a, size_t row, int head, int p)
+        : at(a.sel + (row * a.c.kvh + head) * a.count), count(a.count), tpl(a.c.tpl), most(p >= 0 ? (p / KV_TILE) >> a.c.tpl : -1) {}
+    __device__ __forceinline__ int tile(int e, int vt) const {
+        return e >= 0 && e <= most ? (e << tpl) | (vt & ((1 << tpl) - 1)) : -1;
+    }
+    __device__ __forceinline__ int tile_at(int vt) const { return vt >> tpl < count ? tile(at[vt >> tpl], vt) : -1; }
+    __device__ __forceinline__ int tile_uniform(int vt) const {
+        return vt >> tpl < count ? tile(kv_sload(at, (size_t)(vt >> tpl)), vt) : -1;
+    }
+    __device__ bool empty() const {
+        for (int i = 0; i < count; ++i)
+            if (at[i] >= 0 && at[i] <= most) return false;
+        return true;
+    }
 };
 
 constexpr int at_qt_max(int D) { return D <= 128 ? 4 : 2; }
@@ -137,9 +160,9 @@ __device__ __forceinline__ void again_codes(const u32x2& v, float* f) {
 // looked for first).  One workgroup reads the row's K and V at the latency of its loads, rows
 // side by side where the parts are joined by a launch of their own (65536 tokens of 128 dims
 // 3.6 ms), else one after the other (5 rows of 8192 tokens 0.8 ms).
-template <int D, int KT, int NT>
-__device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, const uint16_t* q, uint16_t* o,
-                                                    int p, float2 ml, float* lds) {
+template <int D, int KT, int NT, bool SEL>
+__device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, size_t row, const uint16_t* q, uint16_t* o, int p,
+                                          float2 ml, float* lds) {
     constexpr int TILES = NT / KV_TILE, G = NT / D;  // tiles of a chunk of tokens; groups of threads over its octets
     constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4;
     const int tid = (int)threadIdx.x;
@@ -150,21 +173,27 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
     int* pages = (int*)(acc + NT);  // [TILES]
     // chunks between the first tokens and the window are skipped
     auto between = [&](int64_t j0, int n) { return a.window != 0 && j0 >= a.sinks && j0 + n - 1 <= (int64_t)p - a.window; };
+    // tokens are walked in order, or (SEL) in the list's, where number j lies in tile turned(j / 32)
+    const AttnList list(a, row, head, p);
+    auto turned = [&](int64_t vt) { return SEL ? list.tile_at((int)vt) : (int)vt; };
+    const int64_t end = SEL ? ((int64_t)a.count << a.c.tpl) * KV_TILE : (int64_t)p + 1;
     bool bad = p >= cap;
     if (!bad) {
-        for (int64_t tile = tid; tile * KV_TILE <= p; tile += NT)
-            if (!between(tile * KV_TILE, KV_TILE) && kv_page(a.c, b, (int)tile) < 0) bad = true;
+        for (int64_t vt = tid; vt * KV_TILE < end; vt += NT) {
+            const int tile = turned(vt);
+            if (tile >= 0 && !between(vt * KV_TILE, KV_TILE) && kv_page(a.c, b, tile) < 0) bad = true;
+        }
     }
     bad = __syncthreads_or(bad);
     // (weights of the mean: a sum of them times finite values stays finite)
     const float il = 1.0f / ml.y;
     float sum = 0.0f;
-    for (int64_t j0 = 0; j0 <= p && !bad; j0 += NT) {
+    for (int64_t j0 = 0; j0 < end && !bad; j0 += NT) {
         if (between(j0, NT)) continue;
-        const bool in = j0 + tid <= p && sight.sees((int)(j0 + tid), p);
+        const int tile = j0 + tid < end ? turned((j0 + tid) / KV_TILE) : -1, t = tid % KV_TILE;
+        const bool in = tile >= 0 && sight.sees(tile * KV_TILE + t, p);
         float e = -1.0f;
         if (in) {
-            const int j = (int)j0 + tid, tile = j / KV_TILE, t = j % KV_TILE;
             const size_t at = kv_tile_at(a.c, kv_page(a.c, b, tile), head, tile), base = at * (KV_TILE * D);
             float s = 0.0f;
 #pragma unroll 2
@@ -184,13 +213,17 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, co
         }
         __syncthreads();
         w[tid] = e;
-        if (tid < TILES) pages[tid] = kv_page(a.c, b, (int)min(j0 / KV_TILE + tid, (int64_t)p / KV_TILE));
+        if (tid < TILES) {
+            const int at = turned(min(j0 / KV_TILE + tid, (end - 1) / KV_TILE));
+            pages[tid] = at >= 0 ? kv_page(a.c, b, at) : -1;
+        }
         __syncthreads();
         const int d = tid % D;
 #pragma unroll 2
         for (int i = tid / D; i < NT / 8; i += G) {
             const int pg = pages[i / 4];  // (4 octets of tokens a tile)
             if (pg < 0) continue;         // (none of its tokens is seen)
+            // (a tile's place in its page is that of its number in the list)
             const size_t at = kv_tile_at(a.c, pg, head, (int)(j0 / KV_TILE) + i / 4), base = at * (KV_TILE * D);
             float v[8];
             if constexpr (I8) {
@@ -231,9 +264,16 @@ struct AttnSeq {
     bool over;       // longer than its table
     __device__ __forceinline__ int tile_of(int v) const { return v < nsink ? v : v - nsink + lo_t; }
 };
-template <int ROWS, int W>
-__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, const KvSeq& sq, int qg) {
+// (SEL: row `row` of the sequence as the only one of a sequence that ends with it)
+template <int ROWS, int W, bool SEL>
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, KvSeq sq, int qg, int row) {
     AttnSeq s;
+    if constexpr (SEL) {
+        const bool in = row < sq.n;
+        sq.len = max(0, max(0, sq.len) - sq.n + row + 1);
+        sq.row0 += in ? row : 0;
+        sq.n = in;
+    }
     s.sq = sq;
     s.rows = min(ROWS, sq.n * a.gqa - qg * ROWS);
     const int cap = (a.c.width << a.c.tpl) * KV_TILE;
@@ -248,31 +288,32 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, const KvSeq& sq, 
         s.nsink = (min(min(a.sinks, from), cap) + KV_TILE - 1) / KV_TILE;
         s.lo_t = max(from / KV_TILE, s.nsink);
     }
-    s.tiles = s.nsink + max(0, (min(s.len, cap) + KV_TILE - 1) / KV_TILE - s.lo_t);
+    s.tiles = SEL ? a.count << a.c.tpl : s.nsink + max(0, (min(s.len, cap) + KV_TILE - 1) / KV_TILE - s.lo_t);
     s.parts = max(1, min(a.splits, (s.tiles + W - 1) / W));
     return s;
 }
 
 // Row rr of group qg as a result; false where it has to be computed again: its weights are
 // numbers, the sums of its values are not finite (0 * x is NaN then)
-template <int D, int ROWS>
+template <int D, int ROWS, bool SEL>
 __device__ __forceinline__ bool attn_store(const AttnArgs& a, const AttnSeq& s, int qg, int head, int rr, int d, at_f32x4 o,
                                            float l) {
     const int r = qg * ROWS + rr, i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
     o = o * (1.0f / l);  // (NaN where l is 0 or NaN)
     bool fine = !(l > 0.0f);
     if (s.pos0 + i < 0) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (SEL && l == 0.0f && AttnList(a, (size_t)s.sq.row0, head, s.pos0).empty()) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     fine |= o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f == 0.0f;
     *(u32x2*)(a.out + (size_t)(s.sq.row0 + i) * a.out_stride + (size_t)(head * a.gqa + hh) * D + d) =
         u32x2{f2bf2(o[0], o[1]), f2bf2(o[2], o[3])};
     return fine;
 }
-template <int D, int KT, int NT, int ROWS>
+template <int D, int KT, int NT, int ROWS, bool SEL>
 __device__ __forceinline__ void attn_again(const AttnArgs& a, const AttnSeq& s, int b, int qg, int head, int rr, float2 ml,
                                            float* lds) {
     const int r = qg * ROWS + rr, i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
     const size_t row = (size_t)s.sq.row0 + i, h = (size_t)(head * a.gqa + hh) * D;
-    row_again<D, KT, NT>(a, b, head, a.q + row * a.q_stride + h, a.out + row * a.out_stride + h, s.pos0 + i, ml, lds);
+    row_again<D, KT, NT, SEL>(a, b, head, row, a.q + row * a.q_stride + h, a.out + row * a.out_stride + h, s.pos0 + i, ml, lds);
 }
 
 // Sums of 8 values (row rr, dims d ..) over parts first, first + step, ...
@@ -318,7 +359,7 @@ __device__ __forceinline__ AttnSum attn_join(__amdgpu_buffer_rsrc_t recs, int rr
 }
 // The groups of threads meet: thread t < 2 * units stores 4 values of unit t % units
 // and leaves the row's maximum and sum in ml
-template <int D, int ROWS>
+template <int D, int ROWS, bool SEL>
 __device__ __forceinline__ bool attn_meet(const AttnArgs& a, const AttnSeq& s, int qg, int head, int rr0, float* lds, int NT,
                                           int units, int G, float2& ml) {
     const at_f32x4* jo = (const at_f32x4*)lds;
@@ -333,7 +374,7 @@ __device__ __forceinline__ bool attn_meet(const AttnArgs& a, const AttnSeq& s, i
         l += lw == lw ? lw * f : lw;
     }
     ml = make_float2(M, l);
-    return attn_store<D, ROWS>(a, s, qg, head, rr0 + u / (D / 8), u % (D / 8) * 8 + 4 * half, o, l);
+    return attn_store<D, ROWS, SEL>(a, s, qg, head, rr0 + u / (D / 8), u % (D / 8) * 8 + 4 * half, o, l);
 }
 __device__ __forceinline__ void attn_lay(float* lds, int NT, const AttnSum& s) {
     at_f32x4* jo = (at_f32x4*)lds;  // [2][NT]
@@ -344,7 +385,7 @@ __device__ __forceinline__ void attn_lay(float* lds, int NT, const AttnSum& s) {
     jm[2 * threadIdx.x + 1] = s.l;
 }
 
-template <int D, int KT, int QT, int W>
+template <int D, int KT, int QT, int W, bool SEL>
 __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(at_two(D, KT != VIPER_KV_BF16, QT) ? 4 : 1)))
 attn_kernel(AttnArgs a) {
     constexpr int NT = W * 64;
@@ -363,7 +404,7 @@ attn_kernel(AttnArgs a) {
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int split = (int)blockIdx.x, b = (int)blockIdx.z;
+    const int b = (int)blockIdx.z, row = SEL ? (int)blockIdx.x / a.splits : 0, split = (int)blockIdx.x - row * a.splits;
     int head = (int)blockIdx.y, qg = 0;
     if (a.qgroups > 1) {
         qg = head / a.c.kvh;
@@ -373,10 +414,12 @@ attn_kernel(AttnArgs a) {
     // depend on the length (but with a window): its page and the sequence's length
     // are asked for together.
     const int v0 = split * W + wave, stride = a.splits * W;
-    int page0 = kv_sload(a.c.table, (size_t)b * a.c.width + min(v0 >> a.c.tpl, a.c.width - 1));
+    int page0 = SEL ? 0 : kv_sload(a.c.table, (size_t)b * a.c.width + min(v0 >> a.c.tpl, a.c.width - 1));
     KvSeq sq = kv_seq(a.c, b);
     asm volatile("" : "+s"(page0), "+s"(sq.len));
-    const AttnSeq s = attn_seq<ROWS, W>(a, sq, qg);
+    const AttnSeq s = attn_seq<ROWS, W, SEL>(a, sq, qg, row);
+    sq = s.sq;
+    const AttnList list(a, (size_t)sq.row0, head, s.pos0);
     const int rows = s.rows, len = s.len, pos0 = s.pos0, tiles = s.tiles, parts = s.parts;
     if (rows <= 0 || split >= parts) return;
 
@@ -448,31 +491,43 @@ attn_kernel(AttnArgs a) {
     // A tile's K is asked for once the products that read the one before are
     // issued, its V likewise, its page two tiles ahead.  A tile whose page is missing
     // reads page 0 and makes the sums of every row of the wave NaN (row_again sorts them out).
-    auto page_of = [&](int v) {
-        const int p = v < tiles ? kv_page_uniform(a.c, b, s.tile_of(v)) : 0;
+    // (SEL: a tile's number is known one tile earlier still; of none, -1, the first of the pool
+    // is read and nothing of it seen)
+    auto page_of = [&](int v, int tile) {
+        const int p = v < tiles && tile >= 0 ? kv_page_uniform(a.c, b, tile) : 0;
         if (p < 0) missing = true;
         return max(p, 0);
     };
+    auto number = [&](int v) { return SEL ? list.tile_uniform(v) : s.tile_of(v); };
+    int tn = number(v0), tnn = number(v0 + stride), t3 = SEL ? number(v0 + 2 * stride) : 0;
     if (v0 < tiles) {
         int p = page0;
-        if (a.window != 0) p = kv_page_uniform(a.c, b, s.tile_of(v0));
+        if (SEL) p = tn >= 0 ? kv_page_uniform(a.c, b, tn) : 0;
+        else if (a.window != 0) p = kv_page_uniform(a.c, b, tn);
         if ((unsigned)p >= (unsigned)a.c.pages) {
             missing = true;
             p = 0;
         }
-        load_k(p, s.tile_of(v0));
-        load_v(p, s.tile_of(v0));
+        load_k(p, max(tn, 0));
+        load_v(p, max(tn, 0));
     }
-    int pn, pnn = page_of(v0 + stride);
+    int pn, pnn = page_of(v0 + stride, tnn);
 #pragma unroll
     for (int k = 0; k < QN; ++k)
         if (QC % NT == 0 || tid + k * NT < QC) lq[tid + k * NT] = qv[k];
     lds_barrier();
     for (int v = v0; v < tiles; v += stride) {
-        const int tile = s.tile_of(v), next = s.tile_of(v + stride);
+        const int tile = SEL ? tn : s.tile_of(v), next = SEL ? max(tnn, 0) : s.tile_of(v + stride);
         const bool more = v + stride < tiles;
         pn = pnn;
-        pnn = page_of(v + 2 * stride);
+        if constexpr (SEL) {
+            tn = tnn;
+            tnn = t3;
+            t3 = number(v + 3 * stride);
+            pnn = page_of(v + 2 * stride, tnn);
+        } else {
+            pnn = page_of(v + 2 * stride, s.tile_of(v + 2 * stride));
+        }
         issue_fence();  // (Q is read again for each tile: its registers go to K and V)
         if constexpr (VS) {  // (codes are not widened before their tile's turn)
 #pragma unroll
@@ -514,7 +569,7 @@ attn_kernel(AttnArgs a) {
         if (more) load_k(pn, next);
         // scores, by token of the lane's eight; tiles that some row does not see whole are masked
         const int j0 = tile * KV_TILE, jl = j0 + 8 * g;
-        const bool whole = j0 + KV_TILE - 1 <= pos0 &&
+        const bool whole = (!SEL || tile >= 0) && j0 + KV_TILE - 1 <= pos0 &&
                            (a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
         at_bf16x8 ph[QT], pl[QT];
 #pragma unroll
@@ -530,7 +585,7 @@ attn_kernel(AttnArgs a) {
                 seen = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
-                    const bool in = sight.sees(jl + e, pos[qt]);
+                    const bool in = (!SEL || tile >= 0) && sight.sees(jl + e, pos[qt]);
                     seen |= in ? 1u << e : 0u;
                     x[e] = in ? x[e] : -__builtin_inff();
                 }
@@ -561,12 +616,12 @@ attn_kernel(AttnArgs a) {
             ph[qt] = __builtin_bit_cast(at_bf16x8, h);
             pl[qt] = __builtin_bit_cast(at_bf16x8, r);
         }
-        if (!VS && j0 + KV_TILE > len) {  // places past the length hold anything
+        if (!VS && (j0 + KV_TILE > len || (SEL && tile < 0))) {  // places past the length hold anything
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    vr[i][e] &= (jl + 2 * e < len ? 0xffffu : 0u) | (jl + 2 * e + 1 < len ? 0xffff0000u : 0u);
+                    vr[i][e] &= SEL && tile < 0 ? 0u : (jl + 2 * e < len ? 0xffffu : 0u) | (jl + 2 * e + 1 < len ? 0xffff0000u : 0u);
             }
         }
         if constexpr (VS) {
@@ -637,14 +692,14 @@ attn_kernel(AttnArgs a) {
     if (tid < (ROWS + 31) / 32) again[tid] = 0u;
     __syncthreads();
 
-    const int rec = (qg * a.c.batch + b) * a.c.kvh + head;
+    const int rec = ((qg * a.c.batch + b) * (SEL ? a.c.max_rows : 1) + row) * a.c.kvh + head;
     constexpr int PF = (int)at_part_floats(D, QT);
     auto once_more = [&](int rr, float2 ml) {  // (threads of one row have the same ml)
         again_ml[rr] = ml;
         atomicOr(&again[rr >> 5], 1u << (rr & 31));
     };
     auto store = [&](int rr, int d, at_f32x4 o, float M, float lt) {
-        if (!attn_store<D, ROWS>(a, s, qg, head, rr, d, o, lt)) once_more(rr, make_float2(M, lt));
+        if (!attn_store<D, ROWS, SEL>(a, s, qg, head, rr, d, o, lt)) once_more(rr, make_float2(M, lt));
     };
     const auto recs = buf(a.part + (size_t)rec * a.splits * PF, (uint32_t)(parts * PF * 4));
     for (int i = tid; i < rows * (D / 4); i += NT) {
@@ -694,75 +749,76 @@ attn_kernel(AttnArgs a) {
         if (G > 1) {
             __syncthreads();
             float2 ml;
-            if (tid < 2 * units && !attn_meet<D, ROWS>(a, s, qg, head, 0, lds, NT, units, G, ml))
+            if (tid < 2 * units && !attn_meet<D, ROWS, SEL>(a, s, qg, head, 0, lds, NT, units, G, ml))
                 once_more((tid >= units ? tid - units : tid) / (D / 8), ml);
         }
     }
     __syncthreads();
     for (int rr = 0; rr < rows; ++rr)
-        if ((again[rr >> 5] >> (rr & 31)) & 1u) attn_again<D, KT, NT, ROWS>(a, s, b, qg, head, rr, again_ml[rr], lds);
+        if ((again[rr >> 5] >> (rr & 31)) & 1u) attn_again<D, KT, NT, ROWS, SEL>(a, s, b, qg, head, rr, again_ml[rr], lds);
 }
 
 // The join as a launch of its own: a workgroup per row and group of rows, its
 // threads D / 8 values wide and G parts deep.
 constexpr int AT_JNT = 256;
-template <int D, int KT, int QT, int W>
+template <int D, int KT, int QT, int W, bool SEL>
 __global__ void __launch_bounds__(AT_JNT)
 attn_join_kernel(AttnArgs a) {
     constexpr int ROWS = QT * 16, U = D / 8, G = AT_JNT / U;
     __shared__ __align__(16) float lds[AT_JNT * 10];
     __shared__ int again;
     __shared__ float2 again_ml;
-    const int b = (int)blockIdx.z, rr = (int)blockIdx.x, tid = (int)threadIdx.x;
+    const int b = (int)blockIdx.z, row = SEL ? (int)blockIdx.x / a.lrows : 0, rr = (int)blockIdx.x - row * a.lrows;
+    const int tid = (int)threadIdx.x;
     int head = (int)blockIdx.y, qg = 0;
     if (a.qgroups > 1) {
         qg = head / a.c.kvh;
         head -= qg * a.c.kvh;
     }
-    const AttnSeq s = attn_seq<ROWS, W>(a, kv_seq(a.c, b), qg);
+    const AttnSeq s = attn_seq<ROWS, W, SEL>(a, kv_seq(a.c, b), qg, row);
     if (rr >= s.rows || s.parts == 1) return;
-    const int rec = (qg * a.c.batch + b) * a.c.kvh + head;
+    const int rec = ((qg * a.c.batch + b) * (SEL ? a.c.max_rows : 1) + row) * a.c.kvh + head;
     constexpr int PF = (int)at_part_floats(D, QT);
     const auto recs = buf(a.part + (size_t)rec * a.splits * PF, (uint32_t)(s.parts * PF * 4));
     attn_lay(lds, AT_JNT, attn_join<D, ROWS>(recs, rr, tid % U * 8, tid / U, G, s.parts));
     if (tid == 0) again = 0;
     __syncthreads();
     float2 ml;
-    if (tid < 2 * U && !attn_meet<D, ROWS>(a, s, qg, head, rr, lds, AT_JNT, U, G, ml)) {
+    if (tid < 2 * U && !attn_meet<D, ROWS, SEL>(a, s, qg, head, rr, lds, AT_JNT, U, G, ml)) {
         again_ml = ml;
         again = 1;
     }
     __syncthreads();
-    if (again) attn_again<D, KT, AT_JNT, ROWS>(a, s, b, qg, head, rr, again_ml, lds);
+    if (again) attn_again<D, KT, AT_JNT, ROWS, SEL>(a, s, b, qg, head, rr, again_ml, lds);
 }
 
 struct AttnFn {
     const void* attn;
     const void* join;
 };
-template <int D, int KT, int QT, int W>
+template <int D, int KT, int QT, int W, bool SEL>
 inline AttnFn attn_pair() {
-    return AttnFn{(const void*)attn_kernel<D, KT, QT, W>, (const void*)attn_join_kernel<D, KT, QT, W>};
+    return AttnFn{(const void*)attn_kernel<D, KT, QT, W, SEL>, (const void*)attn_join_kernel<D, KT, QT, W, SEL>};
 }
-template <int D, int KT, int QT>
+template <int D, int KT, int QT, bool SEL>
 inline AttnFn attn_of(int W) {
     if constexpr (at_waves(D, QT) == 8)
-        if (W == 8) return attn_pair<D, KT, QT, 8>();
-    return attn_pair<D, KT, QT, 4>();
+        if (W == 8) return attn_pair<D, KT, QT, 8, SEL>();
+    return attn_pair<D, KT, QT, 4, SEL>();
 }
-template <int KT>
+template <int KT, bool SEL = false>
 inline AttnFn attn_fn(int D, int qt, int W) {
     switch (D * 8 + qt) {
-        case 64 * 8 + 1: return attn_of<64, KT, 1>(W);
-        case 64 * 8 + 2: return attn_of<64, KT, 2>(W);
-        case 64 * 8 + 3: return attn_of<64, KT, 3>(W);
-        case 64 * 8 + 4: return attn_of<64, KT, 4>(W);
-        case 128 * 8 + 1: return attn_of<128, KT, 1>(W);
-        case 128 * 8 + 2: return attn_of<128, KT, 2>(W);
-        case 128 * 8 + 3: return attn_of<128, KT, 3>(W);
-        case 128 * 8 + 4: return attn_of<128, KT, 4>(W);
-        case 256 * 8 + 1: return attn_of<256, KT, 1>(W);
-        case 256 * 8 + 2: return attn_of<256, KT, 2>(W);
+        case 64 * 8 + 1: return attn_of<64, KT, 1, SEL>(W);
+        case 64 * 8 + 2: return attn_of<64, KT, 2, SEL>(W);
+        case 64 * 8 + 3: return attn_of<64, KT, 3, SEL>(W);
+        case 64 * 8 + 4: return attn_of<64, KT, 4, SEL>(W);
+        case 128 * 8 + 1: return attn_of<128, KT, 1, SEL>(W);
+        case 128 * 8 + 2: return attn_of<128, KT, 2, SEL>(W);
+        case 128 * 8 + 3: return attn_of<128, KT, 3, SEL>(W);
+        case 128 * 8 + 4: return attn_of<128, KT, 4, SEL>(W);
+        case 256 * 8 + 1: return attn_of<256, KT, 1, SEL>(W);
+        case 256 * 8 + 2: return attn_of<256, KT, 2, SEL>(W);
         default: return AttnFn{nullptr, nullptr};
     }
 }

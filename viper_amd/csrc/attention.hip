@@ -7,6 +7,9 @@ namespace vq {
 AttnFn attn_kernels_bf16(int D, int qt, int W);
 AttnFn attn_kernels_int8(int D, int qt, int W);
 AttnFn attn_kernels_fp4(int D, int qt, int W);
+AttnFn attn_selected_bf16(int D, int qt, int W);
+AttnFn attn_selected_int8(int D, int qt, int W);
+AttnFn attn_selected_fp4(int D, int qt, int W);
 
 // One row of 20 heads over 4 key heads, 128 dims:
 //  * 8 waves a CU (one workgroup, each wave a tile in use and one in flight): 131072
@@ -29,20 +32,20 @@ struct AttnPlan {
     size_t bytes;  // of workspace; 0: one part
 };
 
-static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int heads) {
+// `units` sequences of `rows` rows that look at up to `tiles` tiles each
+static AttnPlan attn_plan(const viper_kv_cache* c, int rows, int64_t units, int64_t tiles, int heads) {
     AttnPlan p;
     const int gqa = heads / c->kv_heads, most = at_qt_max(c->head_dim);
-    const int t16 = (b->max_rows * gqa + 15) / 16;
+    const int t16 = (rows * gqa + 15) / 16;
     p.qgroups = (t16 + most - 1) / most;
     p.qt = (t16 + p.qgroups - 1) / p.qgroups;
-    p.lrows = b->max_rows * gqa < p.qt * 16 ? b->max_rows * gqa : p.qt * 16;
-    const int64_t base = (int64_t)b->batch * c->kv_heads * p.qgroups;
-    const int64_t tiles = (int64_t)b->table_width * (c->page_size / KV_TILE);
+    p.lrows = rows * gqa < p.qt * 16 ? rows * gqa : p.qt * 16;
+    const int64_t base = units * c->kv_heads * p.qgroups;
     p.waves = at_waves(c->head_dim, p.qt);
     if (tiles <= AT_SHORT) p.waves = 4;
     int64_t s = 1;
     if (base <= AT_CNT) {
-        const bool two = b->batch > 1 && at_two(c->head_dim, c->kv_type != VIPER_KV_BF16, p.qt);
+        const bool two = units > 1 && at_two(c->head_dim, c->kv_type != VIPER_KV_BF16, p.qt);
         const int64_t wgs = (int64_t)device_cus() * AT_WAVES * (two ? 2 : 1) / p.waves;
         s = (wgs + base - 1) / base;
         const int64_t fit = (tiles + p.waves - 1) / p.waves;
@@ -53,6 +56,13 @@ static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int 
     p.bytes = s > 1 ? AT_CNT * 4 + (size_t)base * s * at_part_floats(c->head_dim, p.qt) * 4 : 0;
     return p;
 }
+static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int heads) {
+    return attn_plan(c, b->max_rows, b->batch, (int64_t)b->table_width * (c->page_size / KV_TILE), heads);
+}
+// (over lists, every row is a sequence of its own)
+static AttnPlan attn_plan_selected(const viper_kv_cache* c, const viper_kv_batch* b, int heads, int count) {
+    return attn_plan(c, 1, (int64_t)b->batch * b->max_rows, (int64_t)count * (c->page_size / KV_TILE), heads);
+}
 
 static int attn_check(const viper_kv_cache* c, const viper_kv_batch* b, int heads) {
     const int rc = kv_check(c, b);
@@ -62,23 +72,19 @@ static int attn_check(const viper_kv_cache* c, const viper_kv_batch* b, int head
     return VIPER_OK;
 }
 
-}  // namespace vq
-
-extern "C" size_t viper_hip_attention_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads) {
-    if (vq::attn_check(cache, batch, heads) != VIPER_OK) return 0;
-    return vq::attn_plan(cache, batch, heads).bytes;
+static int selected_check(const viper_kv_cache* c, const viper_kv_batch* b, int heads, int count) {
+    const int rc = attn_check(c, b, heads);
+    if (rc != VIPER_OK) return rc;
+    return count > 0 && (int64_t)count * c->page_size <= INT32_MAX ? VIPER_OK : VIPER_INVALID_ARGUMENT;
 }
 
-extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16,
-                                         int64_t q_stride, int heads, float scale, int window, int sinks, void* out_bf16,
-                                         int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
-    using namespace vq;
-    const int rc = attn_check(cache, batch, heads);
-    if (rc != VIPER_OK) return rc;
+// One call: over the whole sequences, or over the pages of lists (sel)
+static int attn_call(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16, int64_t q_stride, int heads,
+                     float scale, int window, int sinks, const int32_t* sel, int count, void* out_bf16, int64_t out_stride,
+                     void* workspace, size_t workspace_bytes, AttnPlan p, void* stream) {
     const int64_t width = (int64_t)heads * cache->head_dim;
     if (bad_rows(q_bf16, q_stride, width) || bad_rows(out_bf16, out_stride, width)) return VIPER_INVALID_ARGUMENT;
     if (!(scale > 0.0f) || scale > 1e30f || window < 0 || sinks < 0) return VIPER_INVALID_ARGUMENT;
-    AttnPlan p = attn_plan(cache, batch, heads);
     if (workspace == nullptr) {
         p.splits = 1;
     } else if (misaligned(workspace, 16) || workspace_bytes < p.bytes) {
@@ -103,21 +109,57 @@ extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const vipe
     a.window = window > INT32_MAX - VIPER_QLINEAR_MAX_M ? 0 : window;
     a.sinks = sinks;
     a.scale = scale * 1.44269504088896340736f;
-    const int D = cache->head_dim;
-    const AttnFn fn = cache->kv_type == VIPER_KV_INT8  ? attn_kernels_int8(D, p.qt, p.waves)
-                      : cache->kv_type == VIPER_KV_FP4 ? attn_kernels_fp4(D, p.qt, p.waves)
-                                                       : attn_kernels_bf16(D, p.qt, p.waves);
+    a.sel = sel;
+    a.count = count;
+    const int D = cache->head_dim, rows = sel != nullptr ? batch->max_rows : 1;
+    const int kind = (cache->kv_type == VIPER_KV_INT8 ? 1 : cache->kv_type == VIPER_KV_FP4 ? 2 : 0) + (sel != nullptr ? 3 : 0);
+    static AttnFn (*const of[])(int, int, int) = {attn_kernels_bf16,  attn_kernels_int8,  attn_kernels_fp4,
+                                                  attn_selected_bf16, attn_selected_int8, attn_selected_fp4};
+    const AttnFn fn = of[kind](D, p.qt, p.waves);
     if (fn.attn == nullptr) return VIPER_INTERNAL;
     a.by_gqa = (65536u + (unsigned)a.gqa - 1) / (unsigned)a.gqa;
     a.apart = p.splits > 1 && (int64_t)p.splits * p.lrows * D * 4 >= AT_APART;
     void* args[] = {&a};
-    const dim3 grid((unsigned)p.splits, (unsigned)(cache->kv_heads * p.qgroups), (unsigned)batch->batch);
+    const dim3 grid((unsigned)(p.splits * rows), (unsigned)(cache->kv_heads * p.qgroups), (unsigned)batch->batch);
     (void)hipLaunchKernel(fn.attn, grid, dim3((unsigned)p.waves * 64), args, at_lds_bytes(D, p.qt, p.waves, p.lrows),
                           (hipStream_t)stream);
     if (a.apart) {
         const int rc2 = status_of(hipGetLastError());
         if (rc2 != VIPER_OK) return rc2;
-        (void)hipLaunchKernel(fn.join, dim3((unsigned)p.lrows, grid.y, grid.z), dim3(AT_JNT), args, 0, (hipStream_t)stream);
+        (void)hipLaunchKernel(fn.join, dim3((unsigned)(p.lrows * rows), grid.y, grid.z), dim3(AT_JNT), args, 0, (hipStream_t)stream);
     }
     return status_of(hipGetLastError());
+}
+
+}  // namespace vq
+
+extern "C" size_t viper_hip_attention_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads) {
+    if (vq::attn_check(cache, batch, heads) != VIPER_OK) return 0;
+    return vq::attn_plan(cache, batch, heads).bytes;
+}
+
+extern "C" int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16,
+                                         int64_t q_stride, int heads, float scale, int window, int sinks, void* out_bf16,
+                                         int64_t out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+    const int rc = vq::attn_check(cache, batch, heads);
+    if (rc != VIPER_OK) return rc;
+    return vq::attn_call(cache, batch, q_bf16, q_stride, heads, scale, window, sinks, nullptr, 0, out_bf16, out_stride, workspace,
+                         workspace_bytes, vq::attn_plan(cache, batch, heads), stream);
+}
+
+extern "C" size_t viper_hip_attention_selected_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads,
+                                                               int count) {
+    if (vq::selected_check(cache, batch, heads, count) != VIPER_OK) return 0;
+    return vq::attn_plan_selected(cache, batch, heads, count).bytes;
+}
+
+extern "C" int viper_hip_attention_selected(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16,
+                                            int64_t q_stride, int heads, float scale, const int32_t* selected, int count,
+                                            void* out_bf16, int64_t out_stride, void* workspace, size_t workspace_bytes,
+                                            void* stream) {
+    const int rc = vq::selected_check(cache, batch, heads, count);
+    if (rc != VIPER_OK) return rc;
+    if (selected == nullptr || vq::misaligned(selected, 4)) return VIPER_INVALID_ARGUMENT;
+    return vq::attn_call(cache, batch, q_bf16, q_stride, heads, scale, 0, 0, selected, count, out_bf16, out_stride, workspace,
+                         workspace_bytes, vq::attn_plan_selected(cache, batch, heads, count), stream);
 }

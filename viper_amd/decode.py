@@ -305,10 +305,7 @@ def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int
     0 where the batch alone fills the GPU."""
     if not _int32(heads):
         return 0
-    if cache._dev != torch.cuda.current_device():  # (the plan counts a device's CUs)
-        with torch.cuda.device(cache._dev):
-            return int(lib().viper_hip_attention_workspace_bytes(cache._ref, batch._ref, heads))
-    return int(lib().viper_hip_attention_workspace_bytes(cache._ref, batch._ref, heads))
+    return _on_device(cache, lib().viper_hip_attention_workspace_bytes, cache._ref, batch._ref, heads)
 
 
 def attention_paged(cache: KVCache, batch: KVBatch, q, out, scale: Optional[float] = None, window: int = 0, sinks: int = 0,
@@ -336,6 +333,103 @@ def attention_paged(cache: KVCache, batch: KVBatch, q, out, scale: Optional[floa
             ws = _flat(workspace, None, dev)
     return _call(lib().viper_hip_attention_paged, what, dev, stream, cache._ref, ref, qp, qs, heads,
                  cache._scale if scale is None else scale, window, sinks, op, os, ws, nws)
+
+
+def kv_page_bounds(cache: KVCache, batch: KVBatch, bounds, stream=None) -> Status:
+    """The least and largest key value of every dimension of each page that a row of the batch lies on, into bounds (bf16
+    [num_pages, kv_heads, 2, head_dim]); other pages' are left as they were.  After kv_append of a batch (total_rows known)."""
+    what = "viper_hip_kv_page_bounds"
+    dev = cache._dev
+    if not _laid(bounds, (cache.num_pages, cache.kv_heads, 2, cache.head_dim)):
+        return _mismatch(what, "bounds is [num_pages, kv_heads, 2, head_dim]")
+    if batch.total_rows is None and batch.row_offsets is not None:
+        ref = batch._rows(min(batch.batch * batch.max_rows, (1 << 31) - 1), dev)  # (an upper limit: offsets past it do not fit)
+    else:
+        ref = batch._rows(batch.total_rows, dev)
+    return _call(lib().viper_hip_kv_page_bounds, what, dev, stream, cache._ref, ref, _flat(bounds, _BF16, dev))
+
+
+def _on_device(cache, fn, *args):
+    if cache._dev != torch.cuda.current_device():  # (plans count a device's CUs)
+        with torch.cuda.device(cache._dev):
+            return int(fn(*args))
+    return int(fn(*args))
+
+
+def select_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int, count: int) -> int:
+    """Bytes of workspace that select_pages takes."""
+    if not (_int32(heads) and _int32(count)):
+        return 0
+    return _on_device(cache, lib().viper_hip_select_pages_workspace_bytes, cache._ref, batch._ref, heads, count)
+
+
+def select_pages(cache: KVCache, batch: KVBatch, q, bounds, selected, first: int = 1, last: int = 1, workspace=None,
+                 stream=None) -> Status:
+    """For each row of q ([rows, heads * head_dim]) and key head the pages to look at, into selected (int32 [rows, kv_heads,
+    count], in order, then -1): the sequence's first `first` and last `last` pages and, of the others, those whose bounds
+    (kv_page_bounds) allow the largest scores.  workspace: select_workspace_bytes(...) bytes."""
+    what = "viper_hip_select_pages"
+    dev, width = cache._dev, _row_width(q)
+    heads = width // cache.head_dim
+    if heads * cache.head_dim != width:
+        return _mismatch(what, "q rows are not whole heads")
+    qp, qs, rows = _row_view(q, width, dev)
+    ref = batch._rows(rows, dev)
+    if ref is None:
+        return _mismatch(what, "the rows do not match the batch")
+    count = _lists(cache, selected, rows)
+    if count is None or not _laid(bounds, (cache.num_pages, cache.kv_heads, 2, cache.head_dim)):
+        return _mismatch(what, "selected is [rows, kv_heads, count], bounds [num_pages, kv_heads, 2, head_dim]")
+    if not (_int32(first) and _int32(last)):
+        return Status(StatusCode.INVALID_ARGUMENT, f"{what}: first and last are 32-bit")
+    if rows == 0:
+        return _OK
+    nws = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    return _call(lib().viper_hip_select_pages, what, dev, stream, cache._ref, ref, qp, qs, heads, _flat(bounds, _BF16, dev), first, last,
+                 _flat(selected, _INT32, dev), count, _flat(workspace, None, dev) if nws else None, nws)
+
+
+def _lists(cache, selected, rows):
+    """The entries of each list of selected, None where it is not [rows, kv_heads, count]."""
+    if selected.dim() != 3 or selected.shape[0] != rows or selected.shape[1] != cache.kv_heads or selected.shape[2] == 0:
+        return None
+    return selected.shape[2]
+
+
+def attention_selected_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int, count: int) -> int:
+    """Bytes of workspace (zero before its first use) that lets attention_selected split lists over workgroups; 0 where the
+    rows alone fill the GPU."""
+    if not (_int32(heads) and _int32(count)):
+        return 0
+    return _on_device(cache, lib().viper_hip_attention_selected_workspace_bytes, cache._ref, batch._ref, heads, count)
+
+
+def attention_selected(cache: KVCache, batch: KVBatch, q, selected, out, scale: Optional[float] = None, workspace=None,
+                       stream=None) -> Status:
+    """attention_paged of each row over the pages of its list alone: selected int32 [rows, kv_heads, count], numbers of pages
+    in the row's sequence as select_pages leaves them; negative entries are none."""
+    what = "viper_hip_attention_selected"
+    dev, width = cache._dev, _row_width(q)
+    heads = width // cache.head_dim
+    if heads * cache.head_dim != width:
+        return _mismatch(what, "q rows are not whole heads")
+    qp, qs, rows = _row_view(q, width, dev)
+    op, os, orows = _row_view(out, width, dev)
+    ref = batch._rows(rows, dev)
+    if orows != rows or ref is None:
+        return _mismatch(what, "the rows do not match the batch")
+    count = _lists(cache, selected, rows)
+    if count is None:
+        return _mismatch(what, "selected is [rows, kv_heads, count]")
+    if rows == 0:
+        return _OK
+    ws, nws = None, 0
+    if workspace is not None:
+        nws = workspace.numel() * workspace.element_size()
+        if nws:
+            ws = _flat(workspace, None, dev)
+    return _call(lib().viper_hip_attention_selected, what, dev, stream, cache._ref, ref, qp, qs, heads,
+                 cache._scale if scale is None else scale, _flat(selected, _INT32, dev), count, op, os, ws, nws)
 
 
 def verify_workspace_bytes(B: int, R: int, V: int) -> int:

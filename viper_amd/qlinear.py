@@ -149,6 +149,11 @@ _SYMBOLS = (
     "viper_hip_kv_read",
     "viper_hip_attention_workspace_bytes",
     "viper_hip_attention_paged",
+    "viper_hip_kv_page_bounds",
+    "viper_hip_select_pages_workspace_bytes",
+    "viper_hip_select_pages",
+    "viper_hip_attention_selected_workspace_bytes",
+    "viper_hip_attention_selected",
     "viper_hip_verify_workspace_bytes",
     "viper_hip_verify_draft",
 )
@@ -243,6 +248,14 @@ def lib():
     L.viper_hip_attention_workspace_bytes.restype = sz
     L.viper_hip_attention_paged.argtypes = [vp, vp, vp, i64, i32, C.c_float, i32, i32, vp, i64, vp, sz, vp]
     L.viper_hip_attention_paged.restype = i32
+    L.viper_hip_kv_page_bounds.argtypes = [vp, vp, vp, vp]
+    L.viper_hip_kv_page_bounds.restype = i32
+    for f in (L.viper_hip_select_pages_workspace_bytes, L.viper_hip_attention_selected_workspace_bytes):
+        f.argtypes, f.restype = [vp, vp, i32, i32], sz
+    L.viper_hip_select_pages.argtypes = [vp, vp, vp, i64, i32, vp, i32, i32, vp, i32, vp, sz, vp]
+    L.viper_hip_select_pages.restype = i32
+    L.viper_hip_attention_selected.argtypes = [vp, vp, vp, i64, i32, C.c_float, vp, i32, vp, i64, vp, sz, vp]
+    L.viper_hip_attention_selected.restype = i32
     L.viper_hip_verify_workspace_bytes.argtypes = [i32, i32, i32]
     L.viper_hip_verify_workspace_bytes.restype = sz
     L.viper_hip_verify_draft.argtypes = [vp, vp, vp, vp, vp, vp, i32, i32, i32, vp, vp, vp, vp, sz, vp]
