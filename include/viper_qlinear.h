@@ -618,7 +618,7 @@ int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper_kv_batch* 
  * are listed only among the first and last.  Rows at negative positions list none;
  * pages past the table are not considered.  max_rows <= VIPER_QLINEAR_MAX_M, heads
  * as for viper_hip_attention_paged, count * page_size < 2^31, batch kv_heads
- * ceil(table_width head_dim / 2048) < 2^24.  selected and workspace (16-byte
+ * ceil(table_width / 64) < 2^24.  selected and workspace (16-byte
  * aligned, viper_hip_select_pages_workspace_bytes() bytes, of any content; calls in
  * flight on one race) overlap neither the inputs nor one another (refused). */
 size_t viper_hip_select_pages_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads, int count);

@@ -135,6 +135,39 @@ def test_select(D, page, kvh, heads, lens, rows, counts, first, last, count):
     assert np.all(got[total:] == 77)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("alike", [2, 9, 60, 300])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -110, 2.0 ** 100])
+def test_select_near_the_border(D, alike, scale):
+    """Pages at the border whose scores differ by a part in 2^20 and less, or not at all, amid others far from it."""
+    page, kvh, heads, pages = 32, 2, 6, 700
+    rng = np.random.default_rng(alike + D)
+    table = rng.permutation(pages).astype(np.int32)[None, :]
+    near = np.sort(rng.standard_normal((pages, kvh, 2, D)), 2)
+    order = rng.permutation(pages)
+    near[order[:100]] += 1.5                                        # in
+    like = order[100:100 + alike]
+    near[like] = near[like[0]] + np.array([0.5, 0.7])[:, None]      # at the border
+    q = rng.standard_normal((3, heads, D))
+    q[:, :, 5] = 2.0 ** -14
+    near[like, :, 1, 5] += rng.integers(0, 4, (alike, kvh)) * 2.0 ** -7
+    q, near = R.bf16_bits(q.reshape(3, heads * D)), R.bf16_bits(near * scale)
+    g = va.KVCache.empty(va.KVType.BF16, pages, page, kvh, D)
+    n = pages * page - 7
+    batch = va.KVBatch(dev(table), dev(np.array([n], np.int32)), 3)
+    f = R.bf16_val(near).astype(np.float64)
+    for count in (101, 102 + alike // 2, 101 + alike, 400):
+        sel = dev(np.zeros((3, kvh, count), np.int32))
+        ws = ws_of(va.select_workspace_bytes(g, batch, heads, count))
+        for _ in range(2):
+            assert va.select_pages(g, batch, dev(q), dev(near), sel, first=0, last=1, workspace=ws).ok()
+        got = back(sel)
+        for r in range(3):
+            x = R.bf16_val(q[r]).astype(np.float64).reshape(kvh, heads // kvh, D)
+            for h in range(kvh):
+                assert got[r, h].tolist() == P.select(x[h], f[:, h], table[0], pages, page, n - 3 + r, 0, 1, count), (count, r, h)
+
+
 def test_select_among_missing_pages_and_scores_that_are_not_finite():
     D, page, kvh, pages, n = 64, 32, 1, 40, 30
     rng = np.random.default_rng(5)

@@ -70,8 +70,13 @@ def test_rows_are_a_verify_steps():
     assert calls(cache(), b)[1:] == [INVALID] * 2 and sizes(cache(), b) == [0, 0]
 
 
+def test_largest_selection():
+    c, b = cache(page_size=32, kv_heads=1024, num_pages=1), batch(batch=1, total_rows=1, table_width=1 << 20)
+    assert calls(c, b, heads=1024, qs=1024 * 128, os=1024 * 128, nws=1 << 40)[1] == INVALID  # 2^24 workgroups
+
+
 def test_workspaces():
-    assert sizes(cache(), batch())[0] == 2 * 4 * 4 * 4  # a score of each row, key head and page
+    assert sizes(cache(), batch())[0] == 2 * 4 * (4 + 1) * 4  # a score of each row, key head and page, and how far 16 may be off
     c, one, many = cache(), batch(batch=1, total_rows=1), batch(batch=4096, total_rows=4096)
     assert sizes(c, one, count=1)[1] == 0 and sizes(c, one, count=512)[1] > 8192 and sizes(c, many, count=512)[1] == 0
 

@@ -124,9 +124,6 @@ page_bounds_kernel(BoundsArgs a) {
 
 // ----------------------------------------------------------------- scores
 
-constexpr int PS_NT = 256;
-constexpr int PS_LDS = 32768;  // bytes of q that a workgroup keeps at a time
-
 struct SelectArgs {
     KvArgs c;
     const uint16_t* q;
@@ -134,7 +131,10 @@ struct SelectArgs {
     const uint16_t* bounds;
     int32_t* out;
     uint32_t* keys;  // [batch * max_rows][key head][width]
-    int gqa, count, first, last, chunks;
+    uint32_t* off;   // [batch * max_rows][key head][tiles]: how far the scores of 16 pages may be off (fp32 patterns)
+    int gqa, count, first, last;
+    int cols, shift;  // columns of a row: its gqa queries, padded to 2^shift (to 5: a multiple of 16)
+    int tiles;  // of 16 pages
 };
 
 // Pages of the row at position p (0: no token)
@@ -142,190 +142,464 @@ __device__ __forceinline__ int ps_pages(const KvArgs& c, int64_t p) {
     return p < 0 ? 0 : (int)min((int64_t)c.width, (p >> (c.tpl + 5)) + 1);
 }
 // A score as an integer in its order, above 0; NaN as +inf
+constexpr uint32_t PS_INF = 0xff800000u, PS_NINF = 0x007fffffu;
 __device__ __forceinline__ uint32_t ps_key(float v) {
     if (v != v) v = __builtin_inff();
     const uint32_t u = __float_as_uint(v);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-template <int L>
-__device__ __forceinline__ double ps_sum(double v) {
-    auto step = [&](auto dpp) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const uint32_t lo = (uint32_t)dpp((int)(uint32_t)u), hi = (uint32_t)dpp((int)(u >> 32));
-        v += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-    };
-    step([](int x) { return dpp_i<DPP_SWAP1>(x); });
-    step([](int x) { return dpp_i<DPP_SWAP2>(x); });
-    step([](int x) { return dpp_i<DPP_HALF_MIRROR>(x); });
-    if constexpr (L >= 16) step([](int x) { return dpp_i<DPP_MIRROR>(x); });
-    if constexpr (L >= 32) {
-        const uint64_t u = __builtin_bit_cast(uint64_t, v);
-        const auto l = __builtin_amdgcn_permlane16_swap((uint32_t)u, (uint32_t)u, false, false);
-        const auto h = __builtin_amdgcn_permlane16_swap((uint32_t)(u >> 32), (uint32_t)(u >> 32), false, false);
-        v = __builtin_bit_cast(double, (uint64_t)h[0] << 32 | l[0]) + __builtin_bit_cast(double, (uint64_t)h[1] << 32 | l[1]);
-    }
-    return v;
+__device__ __forceinline__ float ps_score(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
+__device__ __forceinline__ size_t ps_row(const SelectArgs& a, int b, int r, int head) {
+    return (size_t)(b * a.c.max_rows + r) * a.c.kvh + head;
 }
 
-// D / 8 lanes to a page, each with 8 dims of it; the rows' queries come from LDS
+// Scores in 32 bits, sum_d max(q_d, 0) hi_d + min(q_d, 0) lo_d, as products of 16 pages and
+// 16 queries over 32 dims at a time whose sums are added one after the other.  In whatever
+// order a product adds its 32 terms, and if it truncates, a sum is off by at most 32 2^-23 of
+// the sum of its terms' magnitudes; the 2 D / 32 <= 16 additions add 16 2^-24 of all.
+// PS_OFF is above these 40 2^-23 by a fifth, which covers the rounding of the magnitudes' sum
+// and of what a score is compared with.  Values and products under 2^-126 may count as zero:
+// magnitudes are taken as 2^-100 at least, and 2^-117 is added.  page_pick_kernel computes
+// the few pages that are too near to the border for that in 64 bits.
+constexpr float PS_OFF = 48 * 0x1p-23f, PS_OFF_MIN = 0x1p-117f;
+typedef __bf16 ps_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float ps_f32x4 __attribute__((ext_vector_type(4)));
+constexpr int PS_NT = 256;
+
+// A wave takes 16 pages and all rows of its sequence.
 template <int D>
 __global__ void __launch_bounds__(PS_NT)
 page_score_kernel(SelectArgs a) {
-    constexpr int L = D / 8, PP = PS_NT / L;
-    extern __shared__ __align__(16) uint16_t lq[];  // [rows of a turn][gqa][D]
-    const int tid = (int)threadIdx.x, l = tid % L;
-    const int head = (int)blockIdx.y, b = (int)blockIdx.z;
+    constexpr int NKB = D / 32;
+    const int tid = (int)threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int chunk = (int)blockIdx.x / a.c.kvh, head = (int)blockIdx.x - chunk * a.c.kvh, b = (int)blockIdx.z;
+    const int tile = chunk * (PS_NT / 64) + wave;
+    const int entry = tile * 16 + m < a.c.width ? a.c.table[(size_t)b * a.c.width + tile * 16 + m] : -1;
     const KvSeq s = kv_seq(a.c, b);
     const int64_t pos0 = (int64_t)s.len - s.n;
-    const int all = ps_pages(a.c, (int64_t)s.len - 1), p = (int)blockIdx.x * PP + tid / L;
-    if (s.n == 0 || (int)blockIdx.x * PP >= all) return;
-    const int page = p < all ? a.c.table[(size_t)b * a.c.width + p] : -1;
-    const bool there = (unsigned)page < (unsigned)a.c.pages;
-    float lo[8], hi[8];
-    {
-        u32x4 x = {0u, 0u, 0u, 0u}, y = x;
-        if (there) {
-            const uint16_t* at = a.bounds + ((size_t)page * a.c.kvh + head) * (2 * D) + 8 * l;
-            x = *(const u32x4*)at;
-            y = *(const u32x4*)(at + D);
+    if (s.n == 0 || tile * 16 >= ps_pages(a.c, (int64_t)s.len - 1)) return;
+    // the rows' queries are the columns, 16 at a time; of a row of more than 16 the running maximum is kept
+    const int shift = a.shift, per = min(a.cols, 16), turns = (s.n * a.cols + 15) / 16;
+    auto column = [&](int turn, int& r, int& h) {
+        if (shift <= 4) {
+            r = (turn * 16 + m) >> shift;
+            h = (turn * 16 + m) & (a.cols - 1);
+        } else {  // (turns of one row)
+            r = turn / (a.cols / 16);
+            h = (turn - r * (a.cols / 16)) * 16 + m;
         }
+    };
+    u32x4 q[NKB], lo[NKB], hi[NKB];
+    bool in = false;
+    auto load_q = [&](int turn) {
+        int r, h;
+        column(turn, r, h);
+        in = r < s.n && h < a.gqa;
+        const uint16_t* const at = a.q + (size_t)(s.row0 + (in ? r : 0)) * a.q_stride + (size_t)(head * a.gqa + (in ? h : 0)) * D + 8 * g;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo[i] = bf16f(x[i >> 1] >> (16 * (i & 1)) & 0xffffu);
-            hi[i] = bf16f(y[i >> 1] >> (16 * (i & 1)) & 0xffffu);
+        for (int kb = 0; kb < NKB; ++kb) q[kb] = *(const u32x4*)(at + 32 * kb);
+    };
+    load_q(0);
+    const bool there = (unsigned)entry < (unsigned)a.c.pages;
+    const uint32_t present = (uint32_t)__ballot(there);
+    {
+        const uint16_t* const at = a.bounds + ((size_t)(there ? entry : 0) * a.c.kvh + head) * (2 * D) + 8 * g;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+            lo[kb] = *(const u32x4*)(at + 32 * kb);
+            hi[kb] = *(const u32x4*)(at + D + 32 * kb);
         }
     }
-    const int turn = max(1, PS_LDS / (a.gqa * D * 2));  // (64 heads of 256 dims: one row)
-    for (int r0 = 0; r0 < s.n; r0 += turn) {
-        const int rows = min(turn, s.n - r0);
-        if (r0) __syncthreads();
-        for (int i = tid; i < rows * a.gqa * L; i += PS_NT) {
-            const int r = i / (a.gqa * L), x = i % (a.gqa * L);
-            *(u32x4*)(lq + (size_t)i * 8) =
-                *(const u32x4*)(a.q + (size_t)(s.row0 + r0 + r) * a.q_stride + (size_t)head * a.gqa * D + 8 * x);
-        }
-        __syncthreads();
-        for (int r = 0; r < rows; ++r) {
-            if (p >= ps_pages(a.c, pos0 + r0 + r)) continue;
-            double best = -__builtin_inf();
-            bool nan = false;
-            for (int h = 0; h < a.gqa; ++h) {
-                const u32x4 w = *(const u32x4*)(lq + (size_t)(r * a.gqa + h) * D + 8 * l);
-                double sum = 0.0;
+    constexpr uint32_t LEAST = 0x0d800d80u;  // 2^-100
+    auto of = [](const u32x4& v) { return __builtin_bit_cast(ps_bf16x8, v); };
+    ps_f32x4 best;
+    uint32_t off = 0;
+    for (int turn = 0; turn < turns; ++turn) {
+        const ps_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        ps_f32x4 S = zero, Q = zero;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float x = bf16f(w[i >> 1] >> (16 * (i & 1)) & 0xffffu);
-                    // (NaN where either product is: an infinite bound under a zero)
-                    const float u = x * lo[i], v = x * hi[i];
-                    sum += (double)(u != u || v != v ? __builtin_nanf("") : fmaxf(u, v));
-                }
-                sum = ps_sum<L>(sum);
-                nan |= sum != sum;
-                best = fmax(best, sum);
+        for (int kb = 0; kb < NKB; ++kb) {
+            u32x4 up, dn, mag, most;  // most: the larger magnitude of either bound
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // (as integers, values with a sign are under 0)
+                up[i] = pb_max(q[kb][i], 0u);
+                dn[i] = pb_min(q[kb][i], 0u);
+                mag[i] = pb_max(q[kb][i] & 0x7fff7fffu, LEAST);
+                most[i] = pb_max(pb_max(lo[kb][i] & 0x7fff7fffu, hi[kb][i] & 0x7fff7fffu), LEAST);
             }
-            if (l == 0)
-                a.keys[((size_t)(b * a.c.max_rows + r0 + r) * a.c.kvh + head) * a.c.width + p] =
-                    there ? ps_key(nan ? __builtin_inff() : (float)best) : 0u;
+            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(hi[kb]), of(up), zero, 0, 0, 0);
+            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(lo[kb]), of(dn), zero, 0, 0, 0);
+            Q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(most), of(mag), Q, 0, 0, 0);
         }
+        const bool was = in;
+        int r, h;
+        column(turn, r, h);
+        if (turn + 1 < turns) load_q(turn + 1);
+        const bool begins = shift <= 4 || h < 16, ends = shift <= 4 || h + 16 - m >= a.cols;
+        // over the columns of a row.  A score that is no number has a Q that is not finite, and
+        // as patterns NaN and infinity are the largest of these: pages in 64 bits then.
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v = was ? S[i] : -__builtin_inff();
+            if (per >= 2) v = fmaxf(v, dpp_f<DPP_SWAP1>(v));
+            if (per >= 4) v = fmaxf(v, dpp_f<DPP_SWAP2>(v));
+            if (per >= 8) v = fmaxf(v, dpp_f<DPP_HALF_MIRROR>(v));
+            if (per >= 16) v = fmaxf(v, dpp_f<DPP_MIRROR>(v));
+            best[i] = begins ? v : fmaxf(best[i], v);
+        }
+        uint32_t e = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e = max(e, (present >> (4 * g + i)) & 1u ? __float_as_uint(Q[i]) & 0x7fffffffu : 0u);
+        e = was ? e : 0u;
+        if (per >= 2) e = max(e, (uint32_t)dpp_i<DPP_SWAP1>((int)e));
+        if (per >= 4) e = max(e, (uint32_t)dpp_i<DPP_SWAP2>((int)e));
+        if (per >= 8) e = max(e, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)e));
+        if (per >= 16) e = max(e, (uint32_t)dpp_i<DPP_MIRROR>((int)e));
+        auto w = __builtin_amdgcn_permlane16_swap(e, e, false, false);
+        e = max(w[0], w[1]);
+        w = __builtin_amdgcn_permlane32_swap(e, e, false, false);
+        e = max(w[0], w[1]);
+        off = begins ? e : max(off, e);
+        const int p = tile * 16 + 4 * g, pages = ps_pages(a.c, pos0 + r);
+        if (!ends || m % per != 0 || r >= s.n || p >= pages) continue;
+        const size_t row = ps_row(a, b, r, head);
+        uint32_t* const keys = a.keys + row * a.c.width + p;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (p + i < pages) keys[i] = (present >> (4 * g + i)) & 1u ? ps_key(best[i]) : 0u;
+        if (g == 0) a.off[row * a.tiles + tile] = __float_as_uint(__uint_as_float(off) * PS_OFF + PS_OFF_MIN);
     }
 }
 
 // ----------------------------------------------------------------- selection
 
-constexpr int PK_NT = 512, PK_KPT = 8, PK_W = PK_NT / 64;
+constexpr int PK_NT = 512, PK_W = PK_NT / 64, PK_BINS = 1024, PK_LIST = 64;
 
-// A workgroup per row and key head; a thread holds PK_KPT consecutive pages (rows of more
-// pages than that are walked again at each step).
+__device__ __forceinline__ double wave_sum(double v) {
+    auto step = [&](auto f) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        uint32_t a[2], b[2];
+        f((uint32_t)u, a);
+        f((uint32_t)(u >> 32), b);
+        v = __builtin_bit_cast(double, (uint64_t)b[0] << 32 | a[0]) + __builtin_bit_cast(double, (uint64_t)b[1] << 32 | a[1]);
+    };
+    auto dpp = [&](auto f) { step([&](uint32_t x, uint32_t* y) { y[0] = x; y[1] = (uint32_t)f((int)x); }); };
+    dpp([](int x) { return dpp_i<DPP_SWAP1>(x); });
+    dpp([](int x) { return dpp_i<DPP_SWAP2>(x); });
+    dpp([](int x) { return dpp_i<DPP_HALF_MIRROR>(x); });
+    dpp([](int x) { return dpp_i<DPP_MIRROR>(x); });
+    step([](uint32_t x, uint32_t* y) {
+        const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+        y[0] = r[0], y[1] = r[1];
+    });
+    step([](uint32_t x, uint32_t* y) {
+        const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+        y[0] = r[0], y[1] = r[1];
+    });
+    return v;
+}
+// The score of a page for one query head by a wave: products are exact in 32 bits, sums in 64
+__device__ __forceinline__ uint32_t page_exact(const uint16_t* at, const uint16_t* q, int D) {
+    const int lane = (int)threadIdx.x & 63;
+    uint32_t x[4], lo[4], hi[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int d = lane + 64 * i;
+        x[i] = lo[i] = hi[i] = 0u;
+        if (d < D) {
+            x[i] = q[d];
+            lo[i] = at[d];
+            hi[i] = at[D + d];
+        }
+    }
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double y = (double)bf16f(x[i]), u = y * (double)bf16f(lo[i]), v = y * (double)bf16f(hi[i]);
+        sum += u != u || v != v ? __builtin_nan("") : fmax(u, v);
+    }
+    return ps_key((float)wave_sum(sum));
+}
+
+// Least / largest / sum of the lanes before and the lane's own, over a wave
+template <bool MAX>
+__device__ __forceinline__ uint32_t wave_most(uint32_t v) {
+    auto of = [](uint32_t x, uint32_t y) { return MAX ? max(x, y) : min(x, y); };
+    v = of(v, (uint32_t)dpp_i<DPP_SWAP1>((int)v));
+    v = of(v, (uint32_t)dpp_i<DPP_SWAP2>((int)v));
+    v = of(v, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)v));
+    v = of(v, (uint32_t)dpp_i<DPP_MIRROR>((int)v));
+    auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = of(r[0], r[1]);
+    r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return of(r[0], r[1]);
+}
+__device__ __forceinline__ unsigned wave_upto(unsigned v) {
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes back in the row
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // a row's last lane to the row behind it
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // the lower half's to the upper half
+    return v;
+}
+
+// A workgroup per row and key head.  A wave holds KPT 64 consecutive pages, a lane every
+// 64th of them, so that ballots count and number them in order (MULTI: there are more
+// pages than the workgroup holds, and keys are read again at each step).  The border is
+// found through a histogram of the keys between the least and the largest, then within
+// the bin that holds it; once few keys are left they are ranked.  Every wave does so for
+// itself from what is in LDS: each step costs one barrier.  Bound by the latency of its
+// steps; run once and straight on, also by that of its own code: hence small variants.
+template <int KPT, bool MULTI>
 __global__ void __launch_bounds__(PK_NT)
-page_pick_kernel(SelectArgs a) {
-    __shared__ unsigned part[2][PK_W];
-    const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+page_pick_kernel(SelectArgs a, int D) {
+    __shared__ __align__(16) unsigned hist[3][PK_BINS];  // (one is cleared while another may still be read)
+    __shared__ uint32_t part[2][4][PK_W];
+    __shared__ uint32_t list_key[PK_LIST];
+    __shared__ int list_page[PK_LIST];
+    __shared__ unsigned listed;
+    constexpr int ALL = PK_NT * KPT;
+    const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r = (int)blockIdx.x, head = (int)blockIdx.y, b = (int)blockIdx.z;
+    uint32_t* const keys = a.keys + ps_row(a, b, r, head) * a.c.width;
+    const auto kbuf = buf(keys, (uint32_t)a.c.width * 4);  // (past the end: 0)
+    const uint32_t* const offs = a.off + ps_row(a, b, r, head) * a.tiles;
+    // the first keys are asked for before the sequence's length is known
+    uint32_t key[KPT];
+    const int at0 = wave * (KPT * 64) + lane;
+#pragma unroll
+    for (int k = 0; k < KPT; ++k) key[k] = bload4(kbuf, (at0 + 64 * k) * 4);
+    uint32_t err = bload4(buf(offs, (uint32_t)a.tiles * 4), tid * 4);
     const KvSeq s = kv_seq(a.c, b);
     if (r >= s.n) return;
-    const int64_t p = (int64_t)s.len - s.n + r;
-    const int n = ps_pages(a.c, p);
-    const int first = min(a.first, n), last = max(first, n - a.last);  // first and last are in, [first, last) is ranked
-    int32_t* const out = a.out + ((size_t)(s.row0 + r) * a.c.kvh + head) * a.count;
-    const uint32_t* const keys = a.keys + ((size_t)(b * a.c.max_rows + r) * a.c.kvh + head) * a.c.width;
+    const int n = ps_pages(a.c, (int64_t)s.len - s.n + r);
+    const int first = min(a.first, n), last = max(first, n - a.last);  // [first, last) is ranked, the others are in
+    const size_t row = (size_t)s.row0 + r;
+    int32_t* const out = a.out + (row * a.c.kvh + head) * a.count;
     const unsigned want = (unsigned)(a.count - (n - (last - first)));  // of the ranked ones (first + last <= count)
-    const int turns = (n + PK_NT * PK_KPT - 1) / (PK_NT * PK_KPT);
-    uint32_t key[PK_KPT];
-    auto load = [&](int turn) {
+    const int turns = MULTI ? (n + ALL - 1) / ALL : 1;
+    auto ranked = [&](int at) { return (unsigned)(at - first) < (unsigned)(last - first); };
 #pragma unroll
-        for (int k = 0; k < PK_KPT; ++k) {
-            const int at = (turn * PK_NT + tid) * PK_KPT + k;
-            key[k] = at >= first && at < last ? keys[at] : 0u;
+    for (int k = 0; k < KPT; ++k) key[k] = ranked(at0 + 64 * k) ? key[k] : 0u;
+    // (patterns of values that are not under 0 are in their order, NaN the largest)
+    err = tid * 16 < n ? err : 0u;
+    if (MULTI)
+        for (int i = PK_NT + tid; i * 16 < n; i += PK_NT) err = max(err, offs[i]);
+    auto each = [&](auto f) {  // over the thread's keys of all turns: f(k, page)
+        for (int turn = 0; turn < turns; ++turn) {
+#pragma unroll
+            for (int k = 0; k < KPT; ++k) {
+                const int at = turn * ALL + at0 + 64 * k;
+                if (MULTI) key[k] = ranked(at) ? bload4(kbuf, at * 4) : 0u;
+            }
+#pragma unroll
+            for (int k = 0; k < KPT; ++k) f(k, turn * ALL + at0 + 64 * k);
         }
     };
     int side = 0;
-    auto total = [&](unsigned mine) {  // (of the waves' counts)
-        if (lane == 0) part[side][wave] = mine;
+    // A wave's two counts as all waves': those of the waves before it and of all
+    auto meet = [&](unsigned x, unsigned y, unsigned* before, unsigned* all) {
+        if (lane == 0) {
+            part[side][0][wave] = x;
+            part[side][1][wave] = y;
+        }
         __syncthreads();
-        unsigned t = 0;
 #pragma unroll
-        for (int w = 0; w < PK_W; ++w) t += part[side][w];
-        side ^= 1;
-        return t;
-    };
-    if (turns == 1) load(0);
-    auto count_from = [&](uint32_t t) {
-        unsigned c = 0;
-        for (int turn = 0; turn < turns; ++turn) {
-            if (turns > 1) load(turn);
-#pragma unroll
-            for (int k = 0; k < PK_KPT; ++k) c += (unsigned)__popcll(__ballot(key[k] >= t));
-        }
-        return total(c);
-    };
-    // the largest t that `want` keys reach; 0: there are not so many
-    uint32_t t = 0;
-    for (int bit = 31; bit >= 0; --bit)
-        if (count_from(t | 1u << bit) >= want) t |= 1u << bit;
-    const unsigned ties = t == 0u || t == 0xffffffffu ? 0u : want - count_from(t + 1);  // of the keys that are t
-    // their numbers in order: what is in for certain and how many ties come before a thread's
-    unsigned sure0 = 0, tie0 = 0;
-    for (int turn = 0; turn < turns; ++turn) {
-        if (turns > 1) load(turn);
-        const int at0 = (turn * PK_NT + tid) * PK_KPT;
-        unsigned mine = 0;  // sure ones, and ties in the upper half
-#pragma unroll
-        for (int k = 0; k < PK_KPT; ++k) {
-            const int at = at0 + k;
-            const bool in = at < n && (at < first || at >= last || key[k] > t);
-            mine += in ? 1u : at < n && t != 0u && key[k] == t ? 1u << 16 : 0u;
-        }
-        unsigned before = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const unsigned v = (unsigned)__shfl_up((int)before, d);
-            if (lane >= d) before += v;
-        }
-        const unsigned wave_sum = (unsigned)__shfl((int)before, 63);
-        before -= mine;
-        if (lane == 0) part[side][wave] = wave_sum;
-        __syncthreads();
-        unsigned sum = 0;
-#pragma unroll
-        for (int w = 0; w < PK_W; ++w) {
-            if (w < wave) before += part[side][w];
-            sum += part[side][w];
+        for (int i = 0; i < 2; ++i) {  // (a lane to each wave's)
+            const unsigned c = part[side][i][lane & (PK_W - 1)], upto = wave_upto(c);
+            before[i] = wave == 0 ? 0u : (unsigned)__builtin_amdgcn_readlane((int)upto, (wave - 1) & (PK_W - 1));
+            all[i] = (unsigned)__builtin_amdgcn_readlane((int)upto, PK_W - 1);
         }
         side ^= 1;
-        unsigned sure = sure0 + (before & 0xffffu), tie = tie0 + (before >> 16);
+    };
+
+    const unsigned all_want = want + (unsigned)(n - (last - first));
+    // keys over `above` are in, and of those from `from` on so many as to have `want`
+    uint32_t above = 0u, from = 1u;
+    for (bool exact = false, settled = false;; exact = true) {
+        bool fine = true;
+        if (!settled) {
+            uint32_t least = 0xffffffffu, most = 0;
+            unsigned there = 0;
+            each([&](int k, int) {
+                least = key[k] != 0u ? min(least, key[k]) : least;
+                most = max(most, key[k]);
+                there += (unsigned)__popcll(__ballot(key[k] != 0u));
+            });
+            least = wave_most<false>(least);
+            most = wave_most<true>(most);
+            err = wave_most<true>(err);
+            if (lane == 0) {
+                part[side][0][wave] = least;
+                part[side][1][wave] = most;
+                part[side][2][wave] = err;
+                part[side][3][wave] = there;
+            }
+            for (int i = tid; i < PK_BINS; i += PK_NT) hist[0][i] = 0u;
+            if (tid == 0) listed = 0u;
+            __syncthreads();
+            const int w = lane & (PK_W - 1);
+            least = wave_most<false>(part[side][0][w]);
+            most = wave_most<true>(part[side][1][w]);
+            err = wave_most<true>(part[side][2][w]);
+            there = (unsigned)__builtin_amdgcn_readlane((int)wave_upto(part[side][3][w]), PK_W - 1);
+            side ^= 1;
+            const float e2 = 2.0f * __uint_as_float(err);
+            if (want == 0u) {
+                above = from = 0xffffffffu;
+            } else if (there > want) {  // (else all that are there)
+                // (sums that are not finite: all pages in 64 bits)
+                fine = exact || (least > PS_NINF && most < PS_INF && e2 < 0x1p100f);
+                uint32_t lo = least, hi = fine ? most : least;
+                unsigned left = want;  // of the keys lo .. hi
+                for (int level = 0; lo != hi; ++level) {
+                    unsigned* const h = hist[level % 3];
+                    const int shift = max(0, 22 - (int)__clz((int)((hi - lo) | 1u)));
+                    each([&](int k, int) {
+                        if (key[k] >= lo && key[k] <= hi) atomicAdd(&h[(key[k] - lo) >> shift], 1u);
+                    });
+                    for (int i = tid; i < PK_BINS; i += PK_NT) hist[(level + 1) % 3][i] = 0u;
+                    __syncthreads();
+                    // the bin of the left-th key from above: 16 bins to a lane, then a lane to each of those
+                    constexpr int BPL = PK_BINS / 64;
+                    const u32x4* const mine = (const u32x4*)&h[PK_BINS - BPL * (lane + 1)];
+                    unsigned sum = 0;
 #pragma unroll
-        for (int k = 0; k < PK_KPT; ++k) {
-            const int at = at0 + k;
-            const bool in = at < n && (at < first || at >= last || key[k] > t);
-            const bool eq = !in && at < n && t != 0u && key[k] == t;
-            if (in || (eq && tie < ties)) out[sure + min(tie, ties)] = at;
-            sure += in;
-            tie += eq;
+                    for (int i = 0; i < BPL / 4; ++i) sum += mine[i].x + mine[i].y + mine[i].z + mine[i].w;
+                    unsigned upto = wave_upto(sum);
+                    int src = __ffsll((long long)__ballot(upto >= left)) - 1;
+                    left -= (unsigned)__builtin_amdgcn_readlane((int)(upto - sum), src);
+                    const int top = PK_BINS - 1 - BPL * src;
+                    const unsigned one = lane < BPL ? h[top - lane] : 0u;
+                    upto = wave_upto(one);
+                    src = __ffsll((long long)__ballot(upto >= left)) - 1;
+                    const unsigned held = (unsigned)__builtin_amdgcn_readlane((int)one, src);
+                    left -= (unsigned)__builtin_amdgcn_readlane((int)upto, src) - held;
+                    lo += (uint32_t)(top - src) << shift;
+                    hi = shift == 0 ? lo : min(hi, lo + (1u << shift) - 1u);
+                    if (lo != hi && held <= PK_LIST) {
+                        each([&](int k, int) {
+                            if (key[k] >= lo && key[k] <= hi) list_key[atomicAdd(&listed, 1u)] = key[k];
+                        });
+                        __syncthreads();
+                        const uint32_t v = lane < (int)held ? list_key[lane] : 0u;
+                        unsigned higher = 0, same = 0;
+                        for (unsigned i = 0; i < held; ++i) {
+                            const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+                            higher += x > v;
+                            same += x == v;
+                        }
+                        const uint64_t is = __ballot(lane < (int)held && higher < left && higher + same >= left);
+                        lo = hi = (uint32_t)__builtin_amdgcn_readlane((int)v, __ffsll((long long)is) - 1);
+                    }
+                }
+                // lo is the want-th key, and the want-th score differs from it by e2 / 2 at most
+                above = exact ? lo : ps_key(ps_score(lo) + e2);
+                from = exact ? lo : ps_key(ps_score(lo) - e2);
+            }
         }
-        sure0 += sum & 0xffffu;
-        tie0 += sum >> 16;
+        auto is_in = [&](int k, int at) { return at < n && (!ranked(at) || key[k] > above); };
+        auto may_be = [&](int k) { return key[k] >= from && key[k] <= above; };
+        unsigned sure = 0, may = 0, before[2], all[2];
+        auto count = [&](int k, int at) {
+            sure += (unsigned)__popcll(__ballot(is_in(k, at)));
+            may += (unsigned)__popcll(__ballot(may_be(k)));
+        };
+        each(count);
+        meet(sure, may, before, all);
+        const unsigned need = min(all[1], all_want - all[0]), doubt = all[1];
+        if (fine && (exact || need == doubt)) {  // numbers in order; of equal scores the first
+            unsigned in0 = 0, may0 = 0, turn_all[2] = {0, 0};
+            for (int turn = 0; turn < turns; ++turn) {
+                if (MULTI) {
+#pragma unroll
+                    for (int k = 0; k < KPT; ++k) {
+                        const int at = turn * ALL + at0 + 64 * k;
+                        key[k] = ranked(at) ? bload4(kbuf, at * 4) : 0u;
+                    }
+                    sure = may = 0;
+#pragma unroll
+                    for (int k = 0; k < KPT; ++k) count(k, turn * ALL + at0 + 64 * k);
+                    meet(sure, may, before, turn_all);
+                }
+                unsigned x = in0 + before[0], y = may0 + before[1];
+#pragma unroll
+                for (int k = 0; k < KPT; ++k) {
+                    const int at = turn * ALL + at0 + 64 * k;
+                    const bool i = is_in(k, at), e = may_be(k);
+                    const uint64_t bi = __ballot(i), be = __ballot(e), under = (1ull << lane) - 1;
+                    const unsigned xi = x + (unsigned)__popcll(bi & under), yi = y + (unsigned)__popcll(be & under);
+                    if (i || (e && yi < need)) out[xi + min(yi, need)] = at;
+                    x += (unsigned)__popcll(bi);
+                    y += (unsigned)__popcll(be);
+                }
+                in0 += turn_all[0];
+                may0 += turn_all[1];
+            }
+            for (unsigned i = all[0] + need + tid; i < (unsigned)a.count; i += PK_NT) out[i] = -1;
+            return;
+        }
+        // scores in 64 bits, of the pages in doubt or, where those are too many, of all; a wave takes
+        // a page for one head at a time, and the largest counts
+        settled = fine && doubt <= PK_LIST;
+        const int items = settled ? (int)doubt : last - first;
+        if (settled) {
+            if (tid == 0) listed = 0u;
+            if (tid < PK_LIST) list_key[tid] = 0u;
+            __syncthreads();
+            each([&](int k, int at) {
+                if (may_be(k)) list_page[atomicAdd(&listed, 1u)] = at;
+            });
+        } else {
+            for (int i = tid; i < items; i += PK_NT) keys[first + i] = 0u;
+        }
+        __syncthreads();
+        for (int i = 0, h = wave;; h += PK_W) {
+            for (; h >= a.gqa; h -= a.gqa) ++i;
+            if (i >= items) break;
+            const int c = settled ? list_page[i] : first + i;
+            const int page = a.c.table[(size_t)b * a.c.width + c];
+            if ((unsigned)page >= (unsigned)a.c.pages) continue;
+            const uint32_t v = page_exact(a.bounds + ((size_t)page * a.c.kvh + head) * (2 * D),
+                                          a.q + row * a.q_stride + (size_t)(head * a.gqa + h) * D, D);
+            if (lane != 0) continue;
+            if (settled) atomicMax(&list_key[i], v);
+            else atomicMax(&keys[c], v);
+        }
+        if (!settled) __threadfence();  // (keys are read back past the atomics)
+        __syncthreads();
+        if (settled) {  // in or out, by score and number
+            const uint32_t v = lane < (int)doubt ? list_key[lane] : 0u;
+            const int p = lane < (int)doubt ? list_page[lane] : 0x7fffffff;
+            unsigned higher = 0;
+            for (unsigned i = 0; i < doubt; ++i) {
+                const uint32_t x = (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+                const int o = __builtin_amdgcn_readlane(p, i);
+                higher += x > v || (x == v && o < p);
+            }
+            const uint64_t chosen = __ballot(lane < (int)doubt && higher < need);
+            for (unsigned i = 0; i < doubt; ++i) {
+                const int o = __builtin_amdgcn_readlane(p, i);
+                const uint32_t x = (chosen >> i) & 1ull ? 0xffffffffu : 0u;
+                if (MULTI) {
+                    if (tid == 0) keys[o] = x;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < KPT; ++k) key[k] = at0 + 64 * k == o ? x : key[k];
+                }
+            }
+            from = 0xffffffffu;
+            above = min(above, 0xfffffffeu);
+        }
+        if (MULTI) {
+            __syncthreads();
+        } else if (!settled) {
+#pragma unroll
+            for (int k = 0; k < KPT; ++k) key[k] = ranked(at0 + 64 * k) ? bload4(kbuf, (at0 + 64 * k) * 4) : 0u;
+        }
     }
-    for (unsigned i = sure0 + min(tie0, ties) + tid; i < (unsigned)a.count; i += PK_NT) out[i] = -1;
 }
 
 template <int D>
@@ -348,7 +622,7 @@ static int select_check(const viper_kv_cache* c, const viper_kv_batch* b, int he
     return count > 0 && (int64_t)count * c->page_size <= INT32_MAX ? VIPER_OK : VIPER_INVALID_ARGUMENT;
 }
 static size_t select_bytes(const viper_kv_cache* c, const viper_kv_batch* b) {
-    return (size_t)b->batch * b->max_rows * c->kv_heads * b->table_width * 4;
+    return (size_t)b->batch * b->max_rows * c->kv_heads * (b->table_width + ((size_t)b->table_width + 15) / 16) * 4;
 }
 
 }  // namespace vq
@@ -406,20 +680,30 @@ extern "C" int viper_hip_select_pages(const viper_kv_cache* cache, const viper_k
     a.bounds = (const uint16_t*)bounds_bf16;
     a.out = selected;
     a.keys = (uint32_t*)workspace;
+    a.off = a.keys + (size_t)batch->batch * batch->max_rows * cache->kv_heads * batch->table_width;
+    a.tiles = (batch->table_width + 15) / 16;
     a.gqa = heads / cache->kv_heads;
     a.count = count;
     a.first = first;
     a.last = last;
-    const int pp = PS_NT / (D / 8), turn = PS_LDS / (a.gqa * D * 2) > 1 ? PS_LDS / (a.gqa * D * 2) : 1;
-    const int held = turn < batch->max_rows ? turn : batch->max_rows;
-    void* args[] = {&a};
-    const dim3 grid((unsigned)((batch->table_width + pp - 1) / pp), (unsigned)cache->kv_heads, (unsigned)batch->batch);
-    if ((int64_t)grid.x * grid.y * grid.z >= 1 << 24) return VIPER_INVALID_ARGUMENT;
-    const void* fn = D == 64 ? (const void*)page_score_kernel<64> : D == 128 ? (const void*)page_score_kernel<128> : (const void*)page_score_kernel<256>;
-    (void)hipLaunchKernel(fn, grid, dim3(PS_NT), args, (size_t)held * a.gqa * D * 2, (hipStream_t)stream);
+    a.shift = 0;
+    while (a.shift <= 4 && 1 << a.shift < a.gqa) ++a.shift;
+    a.cols = a.shift <= 4 ? 1 << a.shift : (a.gqa + 15) / 16 * 16;
+    int d = D;
+    void* args[] = {&a, &d};
+    const int64_t chunks = (a.tiles + PS_NT / 64 - 1) / (PS_NT / 64);
+    if (chunks * cache->kv_heads * batch->batch >= 1 << 24) return VIPER_INVALID_ARGUMENT;
+    const dim3 grid((unsigned)(chunks * cache->kv_heads), 1, (unsigned)batch->batch);
+    const void* score = D == 64 ? (const void*)page_score_kernel<64> : D == 128 ? (const void*)page_score_kernel<128> : (const void*)page_score_kernel<256>;
+    (void)hipLaunchKernel(score, grid, dim3(PS_NT), args, 0, (hipStream_t)stream);
     rc = status_of(hipGetLastError());
     if (rc != VIPER_OK) return rc;
-    (void)hipLaunchKernel((const void*)page_pick_kernel, dim3((unsigned)batch->max_rows, grid.y, grid.z), dim3(PK_NT), args, 0,
-                          (hipStream_t)stream);
+    const int w = batch->table_width;
+    const void* pick = w <= PK_NT       ? (const void*)page_pick_kernel<1, false>
+                       : w <= 2 * PK_NT ? (const void*)page_pick_kernel<2, false>
+                       : w <= 4 * PK_NT ? (const void*)page_pick_kernel<4, false>
+                       : w <= 8 * PK_NT ? (const void*)page_pick_kernel<8, false>
+                                        : (const void*)page_pick_kernel<8, true>;
+    (void)hipLaunchKernel(pick, dim3((unsigned)batch->max_rows, (unsigned)cache->kv_heads, grid.z), dim3(PK_NT), args, 0, (hipStream_t)stream);
     return status_of(hipGetLastError());
 }
