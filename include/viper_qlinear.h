@@ -562,7 +562,8 @@ typedef struct viper_kv_batch {
  * otherwise overlaps neither q nor k nor v (refused);
  * rope_theta = 0: k is stored as it is, q must be NULL.  Strides are multiples
  * of 8 elements, all pointers 16-byte aligned.  Two rows of one call must not be
- * one token. */
+ * one token, nor (FP4, whose values of 8 tokens share words) rows of two sequences
+ * lie among the same 8 tokens of a page. */
 int viper_hip_kv_append(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* k_bf16,
                         const void* v_bf16, int64_t kv_stride, const void* q_bf16, int64_t q_stride, int heads,
                         void* q_out_bf16, int64_t q_out_stride, double rope_theta, void* stream);

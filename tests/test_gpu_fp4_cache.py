@@ -88,6 +88,37 @@ def test_append_and_read(D, page, kvh, heads, lens, counts, rows, theta):
         np.testing.assert_array_equal(getattr(n, name)[kept[name]], getattr(c, name)[kept[name]])
 
 
+def test_every_mantissa_of_a_value_under_every_mantissa_of_a_row_s_largest():
+    """All 128 mantissas of the largest value times all values down to 2^-6 of it, at three exponents: codes, scales, exponents.
+    (Quotients depend on the exponents' difference alone, and values under 2^-6 are under a tenth of the least step.)"""
+    D, page = 128, 256
+    amax = 1 + np.arange(128) / 128
+    x = np.concatenate([amax * 2.0 ** -e for e in range(7)] + [np.zeros(1)])
+    rows = []
+    for a in amax:
+        v = np.concatenate([x[x < a], -x[x < a]])
+        v = np.concatenate([v, np.zeros(-len(v) % (D - 1))]).reshape(-1, D - 1)
+        rows.append(np.concatenate([np.full((len(v), 1), a), v], 1))
+    rows = np.concatenate(rows)
+    print(len(rows), "rows", flush=True)
+    for e in (0, -20, 100):
+        y = rows * 2.0 ** e
+        bits = R.bf16_bits(y.astype(np.float32))
+        np.testing.assert_array_equal(R.bf16_val(bits), y)
+        n = len(y)
+        pages = -(-n // page)
+        g = va.KVCache.empty(va.KVType.FP4, pages, page, 1, D)
+        table = dev(np.arange(pages, dtype=np.int32)[None, :])
+        batch = va.KVBatch(table, dev(np.array([n], np.int32)), n)
+        assert va.kv_append(g, batch, dev(bits), dev(bits)).ok()
+        ko, vo = (dev(np.zeros((n, 1, D), np.uint16)) for _ in range(2))
+        assert va.kv_read(g, batch, ko, vo).ok()
+        np.testing.assert_array_equal(R.bf16_val(back(ko))[:, 0], F.quantize_k(y)[0])
+        s = np.maximum(np.abs(y).max(1).astype(np.float32) / np.float32(6), np.float32(1e-8))
+        held = F.nearest(y.astype(np.float32) / s[:, None]).astype(np.float32) * s[:, None]
+        np.testing.assert_array_equal(R.bf16_val(back(vo))[:, 0], R.bf16_val(R.bf16_bits(held)))
+
+
 def test_blocks_and_rows_that_are_not_finite_and_ends_of_the_range():
     D, page = 128, 32
     c = F.Cache4(2, page, 1, D)
@@ -109,16 +140,16 @@ def test_blocks_and_rows_that_are_not_finite_and_ends_of_the_range():
         np.testing.assert_array_equal(R.bf16_val(back(vo)[r, 0]), R.bf16_val(R.bf16_bits(vh.astype(np.float32) * s)))
 
 
-def test_tokens_of_one_octet_written_by_two_sequences_and_by_steps():
-    """A shared page whose octet two sequences of one call write at different tokens, and single tokens one call after the other."""
+def test_tokens_written_by_steps_and_by_two_sequences_of_a_page():
+    """Single tokens one call after the other, and a shared page of which two sequences of one call write different octets."""
     D, page, rng = 64, 32, np.random.default_rng(2)
     c = F.Cache4(1, page, 2, D, rng)
     g = F.gpu_cache(c, va, dev)
     x = R.bf16_bits(rng.standard_normal((32, 2 * D)))
-    lens = dev(np.array([3, 6], np.int32))
     table = dev(np.zeros((2, 1), np.int32))
-    assert va.kv_append(g, va.KVBatch(table, lens, 2), dev(x[[1, 2, 4, 5]]), dev(x[[1, 2, 4, 5]])).ok()
-    for t in (0, 3, 6, 7, 8, 31):
+    assert va.kv_append(g, va.KVBatch(table, dev(np.array([3, 20], np.int32)), 2), dev(x[[1, 2, 18, 19]]), dev(x[[1, 2, 18, 19]])).ok()
+    steps = (0, 3, 6, 7, 8, 31)
+    for t in steps:
         one = va.KVBatch(table[:1].contiguous(), dev(np.array([t + 1], np.int32)), 1)
         assert va.kv_append(g, one, dev(x[t:t + 1]), dev(x[t:t + 1])).ok()
     n = F.Cache4(1, page, 2, D)
@@ -126,7 +157,7 @@ def test_tokens_of_one_octet_written_by_two_sequences_and_by_steps():
     for t in range(32):
         for h in range(2):
             for is_k in (True, False):
-                if t > 8 and t != 31:
+                if t not in steps and t not in (1, 2, 18, 19):
                     want = c.held(0, t, h, is_k)
                 else:
                     y = R.bf16_val(x[t, h * D:(h + 1) * D]).astype(np.float64)
