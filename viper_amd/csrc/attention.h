@@ -58,6 +58,7 @@ __host__ __device__ constexpr bool at_halves(int D, int qt, int W) { return (siz
 __host__ __device__ constexpr int at_slots(int D, int qt, int W) { return W / (at_halves(D, qt, W) ? 2 : 1); }
 constexpr int AT_CNT = 2048;  // counters at the head of the workspace
 constexpr int AT_GP = 6;      // parts whose loads a thread has in flight
+constexpr int AT_PARTS = 64;  // of a sequence at most
 
 struct AttnArgs {
     KvArgs c;
@@ -73,6 +74,7 @@ struct AttnArgs {
     float scale;  // times log2 e
     const int32_t* sel;  // [row][key head][count] pages that are looked at (SEL)
     int count;
+    int share;  // parts are shared out by the sequences' lengths (splits: of all sequences together)
 };
 
 // The list of a row and key head (SEL): tile number vt of it is a tile of the sequence,
@@ -254,6 +256,55 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, si
     __syncthreads();
 }
 
+// Whose part workgroup x of a group of rows is.  Parts of equal numbers for sequences of
+// unequal lengths leave most workgroups waiting for the longest sequence's, so with `share`
+// a sequence has as many as its length asks for: the least number of steps (a tile to
+// every wave) to a part with which all parts of all sequences (up to 64, a lane to each)
+// run at once.
+struct AttnShare {
+    int b, split, splits, first;  // first: the sequence's part 0 among all of them
+};
+__device__ __forceinline__ AttnShare attn_share(const AttnArgs& a, int W, int x, int b) {
+    const int lane = (int)threadIdx.x & 63;
+    const int cap = (a.c.width << a.c.tpl) * KV_TILE;
+    int steps = 0;
+    if (lane < a.c.batch) {
+        int n = a.c.max_rows;
+        if (a.c.offs != nullptr) {
+            const int o = a.c.offs[lane], e = a.c.offs[lane + 1];
+            n = o >= 0 && o <= e && e <= a.c.total_rows && e - o <= a.c.max_rows ? e - o : 0;
+        }
+        const int tiles = (min(max(0, a.c.lens[lane]), cap) + KV_TILE - 1) / KV_TILE;
+        steps = n > 0 ? max(1, (tiles + W - 1) / W) : 0;
+    }
+    auto sum = [](int v) { return __builtin_amdgcn_readlane((int)wave_upto((unsigned)v), 63); };
+    int most = steps;
+    most = max(most, dpp_i<DPP_SWAP1>(most));
+    most = max(most, dpp_i<DPP_SWAP2>(most));
+    most = max(most, dpp_i<DPP_HALF_MIRROR>(most));
+    most = max(most, dpp_i<DPP_MIRROR>(most));
+    most = max(max(__builtin_amdgcn_readlane(most, 0), __builtin_amdgcn_readlane(most, 16)),
+               max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
+    const int held = (int)__popcll(__ballot(steps > 0)), room = max(1, a.splits - held / 2);
+    int k = max(max((sum(steps) + room - 1) / room, (most + AT_PARTS - 1) / AT_PARTS), 1), parts, upto;
+    for (;; ++k) {  // (ends: with k = most each has one part, and there are at least as many as sequences)
+        parts = (steps + k - 1) / k;
+        upto = (int)wave_upto((unsigned)parts);
+        if (__builtin_amdgcn_readlane(upto, 63) <= a.splits) break;
+    }
+    if (x >= 0) {
+        const uint64_t over = __ballot(upto > x);
+        if (over == 0) return AttnShare{-1, 0, 1, 0};
+        b = __ffsll((long long)over) - 1;
+    }
+    AttnShare s;
+    s.b = b;
+    s.splits = __builtin_amdgcn_readlane(parts, b);
+    s.first = __builtin_amdgcn_readlane(upto, b) - s.splits;
+    s.split = x - s.first;
+    return s;
+}
+
 // What a group of rows of a sequence has to look at
 struct AttnSeq {
     KvSeq sq;
@@ -266,7 +317,7 @@ struct AttnSeq {
 };
 // (SEL: row `row` of the sequence as the only one of a sequence that ends with it)
 template <int ROWS, int W, bool SEL>
-__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, KvSeq sq, int qg, int row) {
+__device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, KvSeq sq, int qg, int row, int splits) {
     AttnSeq s;
     if constexpr (SEL) {
         const bool in = row < sq.n;
@@ -289,8 +340,13 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, KvSeq sq, int qg,
         s.lo_t = max(from / KV_TILE, s.nsink);
     }
     s.tiles = SEL ? a.count << a.c.tpl : s.nsink + max(0, (min(s.len, cap) + KV_TILE - 1) / KV_TILE - s.lo_t);
-    s.parts = max(1, min(a.splits, (s.tiles + W - 1) / W));
+    s.parts = max(1, min(splits, (s.tiles + W - 1) / W));
     return s;
+}
+
+// The first part of record rec (of a group of rows, sequence and key head), or of a shared sequence
+__device__ __forceinline__ size_t part_at(const AttnArgs& a, int rec, int first, int qg, int head) {
+    return first < 0 ? (size_t)rec * a.splits : (size_t)(qg * a.c.kvh + head) * a.splits + first;
 }
 
 // Row rr of group qg as a result; false where it has to be computed again: its weights are
@@ -389,7 +445,7 @@ template <int D, int KT, int QT, int W, bool SEL>
 __global__ void __launch_bounds__(W * 64) __attribute__((amdgpu_waves_per_eu(at_two(D, KT != VIPER_KV_BF16, QT) ? 4 : 1)))
 attn_kernel(AttnArgs a) {
     constexpr int NT = W * 64;
-    constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4, VS = I8 || F4;  // VS: values have scales
+    constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4;
     constexpr int NKB = D / 32, NDB = D / 16, ROWS = QT * 16, ST = D + 4;
     constexpr int NK = F4 ? D / 64 : I8 ? NKB : 2 * NKB, NV = F4 ? D / 64 : I8 ? NDB / 2 : NDB;  // 16-byte loads of a lane per tile
     constexpr int SLOTS = at_slots(D, QT, W);
@@ -404,7 +460,18 @@ attn_kernel(AttnArgs a) {
 
     const int tid = (int)threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int l16 = lane & 15, g = lane >> 4;
-    const int b = (int)blockIdx.z, row = SEL ? (int)blockIdx.x / a.splits : 0, split = (int)blockIdx.x - row * a.splits;
+    const int row = SEL ? (int)blockIdx.x / a.splits : 0;
+    int b = (int)blockIdx.z, split = (int)blockIdx.x - row * a.splits, splits = a.splits, first = -1;
+    if constexpr (F4 && !SEL) {
+        if (a.share) {
+            const AttnShare sh = attn_share(a, W, split, 0);
+            if (sh.b < 0) return;
+            b = sh.b;
+            split = sh.split;
+            splits = sh.splits;
+            first = sh.first;
+        }
+    }
     int head = (int)blockIdx.y, qg = 0;
     if (a.qgroups > 1) {
         qg = head / a.c.kvh;
@@ -413,11 +480,11 @@ attn_kernel(AttnArgs a) {
     // Part p of P takes tiles (p + k P) W + wave, so that its first tile does not
     // depend on the length (but with a window): its page and the sequence's length
     // are asked for together.
-    const int v0 = split * W + wave, stride = a.splits * W;
+    const int v0 = split * W + wave, stride = splits * W;
     int page0 = SEL ? 0 : kv_sload(a.c.table, (size_t)b * a.c.width + min(v0 >> a.c.tpl, a.c.width - 1));
     KvSeq sq = kv_seq(a.c, b);
     asm volatile("" : "+s"(page0), "+s"(sq.len));
-    const AttnSeq s = attn_seq<ROWS, W, SEL>(a, sq, qg, row);
+    const AttnSeq s = attn_seq<ROWS, W, SEL>(a, sq, qg, row, splits);
     sq = s.sq;
     const AttnList list(a, (size_t)sq.row0, head, s.pos0);
     const int rows = s.rows, len = s.len, pos0 = s.pos0, tiles = s.tiles, parts = s.parts;
@@ -453,199 +520,331 @@ attn_kernel(AttnArgs a) {
     }
     bool missing = s.over;
 
-    u32x4 kr[NK], vr[NV];
-    u32x4 ksc[2], vsc[2];
-    uint32_t kex = 0;  // FP4: the lane's powers of two, byte 2 (kb / 4) + h
-    constexpr int TB = F4 ? KV_TILE * D / 2 : KV_TILE * D * (I8 ? 1 : 2);  // bytes of a tile
-    // A tile that one workgroup reads is not kept (131072 tokens, one row: 58 us
-    // instead of 68); several groups of rows read it again from L2.
-    constexpr int AUX = QT < at_qt_max(D) && QT <= 2 ? AUX_NT : 0;
-    auto load_tile = [&](const void* pool, size_t at, u32x4* r, auto n) {
-        const auto t = buf((const uint8_t*)pool + at * TB, TB);
+    if constexpr (F4) {
+        // FP4: a tile's K is asked for once the products that read the one before are issued, its
+        // V likewise (past the last tile: a buffer of no bytes, so that the waits count the
+        // loads exactly and K's do not wait for V), its page a tile earlier, its place in a list
+        // two.  The maximum that weights refer to follows the running one only once that has
+        // grown by 2^8: until then they are at most that, and neither sums nor weights are turned
+        // to another one.
+        u32x4 kr[NK], vr[NV], vsc[2];
+        uint32_t ex = 0;  // the lane's powers of two, byte 2 (kb / 4) + h
+        constexpr int TB = KV_TILE * D / 2;
+        constexpr int AUX = QT < at_qt_max(D) && QT <= 2 ? AUX_NT : 0;
+        constexpr float LAG = 8.0f;
+        auto column = [&](int tile) { return min(max(tile, 0) >> a.c.tpl, a.c.width - 1); };
+        auto raw_of = [&](int tile) { return kv_sload(a.c.table, (size_t)b * a.c.width + column(tile)); };
+        auto entry = [&](int v) { return SEL ? kv_sload(list.at, (size_t)min(v >> a.c.tpl, a.count - 1)) : 0; };
+        auto number = [&](int v, int e) { return SEL ? list.tile(e, v) : s.tile_of(v); };
+        struct Place {
+            size_t at;  // the tile's number in the pool
+            bool want;
+        };
+        auto place = [&](int v, int tile, int raw) {
+            const bool want = v < tiles && tile >= 0;
+            const bool fits = (unsigned)raw < (unsigned)a.c.pages && (!SEL || tile >> a.c.tpl < a.c.width);
+            missing |= want && !fits;
+            return Place{kv_tile_at(a.c, want && fits ? raw : 0, head, max(tile, 0)), want};
+        };
+        auto load_k = [&](const Place& p) {
+            const auto kb = buf((const uint8_t*)a.c.k + p.at * TB, p.want ? TB : 0);
+            const auto eb = buf((const uint8_t*)a.c.ks + p.at * D, p.want ? D : 0);
 #pragma unroll
-        for (int i = 0; i < n(); ++i) {
-            const i32x4 w = __builtin_amdgcn_raw_buffer_load_b128(t, lane * 16 + (i & 3) * 1024, (i >> 2) * 4096, AUX);
-            r[i] = u32x4{(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
-        }
-    };
-    auto load_scales = [&](const float* pool, size_t at, u32x4* r) {
-        const auto t = buf(pool + at * KV_TILE, KV_TILE * 4);
-        r[0] = bload16(t, g * 32);
-        r[1] = bload16(t, g * 32 + 16);
-    };
-    auto load_k = [&](int page, int tile) {
-        const size_t at = kv_tile_at(a.c, page, head, tile);
-        load_tile(a.c.k, at, kr, [] { return NK; });
-        if constexpr (I8) load_scales(a.c.ks, at, ksc);
-        if constexpr (F4) {
-            const auto t = buf((const uint8_t*)a.c.ks + at * D, D);
-            kex = D == 256 ? bload4(t, lane * 4) : bload2(t, D == 64 ? (16 * (g >> 1) + l16) * 2 : lane * 2);
-        }
-    };
-    auto load_v = [&](int page, int tile) {
-        const size_t at = kv_tile_at(a.c, page, head, tile);
-        load_tile(a.c.v, at, vr, [] { return NV; });
-        if constexpr (VS) load_scales(a.c.vs, at, vsc);
-    };
-
-    // A tile's K is asked for once the products that read the one before are
-    // issued, its V likewise, its page two tiles ahead.  A tile whose page is missing
-    // reads page 0 and makes the sums of every row of the wave NaN (row_again sorts them out).
-    // (SEL: a tile's number is known one tile earlier still; of none, -1, the first of the pool
-    // is read and nothing of it seen)
-    auto page_of = [&](int v, int tile) {
-        const int p = v < tiles && tile >= 0 ? kv_page_uniform(a.c, b, tile) : 0;
-        if (p < 0) missing = true;
-        return max(p, 0);
-    };
-    auto number = [&](int v) { return SEL ? list.tile_uniform(v) : s.tile_of(v); };
-    int tn = number(v0), tnn = number(v0 + stride), t3 = SEL ? number(v0 + 2 * stride) : 0;
-    if (v0 < tiles) {
-        int p = page0;
-        if (SEL) p = tn >= 0 ? kv_page_uniform(a.c, b, tn) : 0;
-        else if (a.window != 0) p = kv_page_uniform(a.c, b, tn);
-        if ((unsigned)p >= (unsigned)a.c.pages) {
-            missing = true;
-            p = 0;
-        }
-        load_k(p, max(tn, 0));
-        load_v(p, max(tn, 0));
-    }
-    int pn, pnn = page_of(v0 + stride, tnn);
+            for (int i = 0; i < NK; ++i) kr[i] = bload16<AUX>(kb, lane * 16 + i * 1024);
+            ex = D == 256 ? bload4(eb, lane * 4) : bload2(eb, D == 64 ? (16 * (g >> 1) + l16) * 2 : lane * 2);
+        };
+        auto load_v = [&](const Place& p) {
+            const auto vb = buf((const uint8_t*)a.c.v + p.at * TB, p.want ? TB : 0);
+            const auto sb = buf(a.c.vs + p.at * KV_TILE, p.want ? KV_TILE * 4 : 0);
+            vsc[0] = bload16(sb, g * 32);
+            vsc[1] = bload16(sb, g * 32 + 16);
 #pragma unroll
-    for (int k = 0; k < QN; ++k)
-        if (QC % NT == 0 || tid + k * NT < QC) lq[tid + k * NT] = qv[k];
-    lds_barrier();
-    for (int v = v0; v < tiles; v += stride) {
-        const int tile = SEL ? tn : s.tile_of(v), next = SEL ? max(tnn, 0) : s.tile_of(v + stride);
-        const bool more = v + stride < tiles;
-        pn = pnn;
-        if constexpr (SEL) {
-            tn = tnn;
-            tnn = t3;
-            t3 = number(v + 3 * stride);
-            pnn = page_of(v + 2 * stride, tnn);
-        } else {
-            pnn = page_of(v + 2 * stride, s.tile_of(v + 2 * stride));
-        }
-        issue_fence();  // (Q is read again for each tile: its registers go to K and V)
-        if constexpr (VS) {  // (codes are not widened before their tile's turn)
+            for (int i = 0; i < NV; ++i) vr[i] = bload16<AUX>(vb, lane * 16 + i * 1024);
+        };
+        int v = v0, tile = number(v, entry(v)), t1 = number(v + stride, entry(v + stride));
+        int e2 = entry(v + 2 * stride), raw = raw_of(t1);
+        Place next = place(v, tile, !SEL && a.window == 0 ? page0 : raw_of(tile));
+        load_k(next);
+        load_v(next);
 #pragma unroll
-            for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(kr[i]));
-        }
-        at_f32x4 S[QT][2];
+        for (int k = 0; k < QN; ++k)
+            if (QC % NT == 0 || tid + k * NT < QC) lq[tid + k * NT] = qv[k];
+        lds_barrier();
+        for (; v < tiles; v += stride) {
+            next = place(v + stride, t1, raw);
+            const int t2 = number(v + 2 * stride, e2);
+            raw = raw_of(t2);
+            e2 = entry(v + 3 * stride);
+            issue_fence();  // (Q is read again for each tile: its registers go to K and V)
 #pragma unroll
-        for (int qt = 0; qt < QT; ++qt) S[qt][0] = S[qt][1] = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(kr[i]));  // (codes are not widened before their tile's turn)
+            at_f32x4 S[QT][2];
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-            at_bf16x8 qf[QT];
+            for (int qt = 0; qt < QT; ++qt) S[qt][0] = S[qt][1] = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int qt = 0; qt < QT; ++qt) qf[qt] = __builtin_bit_cast(at_bf16x8, lq[(qt * NKB + kb) * 64 + lane]);
+            for (int kb = 0; kb < NKB; ++kb) {
+                at_bf16x8 qf[QT];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                at_bf16x8 k;
-                if constexpr (I8) {
-                    const u32x4 w = kr[(kb >> 1) * 2 + h];
-                    k = kb & 1 ? codes_bf16(w.z, w.w) : codes_bf16(w.x, w.y);
-                } else if constexpr (F4) {
+                for (int qt = 0; qt < QT; ++qt) qf[qt] = __builtin_bit_cast(at_bf16x8, lq[(qt * NKB + kb) * 64 + lane]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
                     const uint32_t w = D == 64 ? kr[0][2 * h + kb] : kr[2 * (kb >> 2) + h][kb & 3];
-                    k = __builtin_bit_cast(at_bf16x8, fp4_bf16(w, fp4_power((kex >> (8 * (2 * (kb >> 2) + h))) & 0xffu)));
-                } else {
-                    k = __builtin_bit_cast(at_bf16x8, kr[kb * 2 + h]);
-                }
+                    const at_bf16x8 k = __builtin_bit_cast(at_bf16x8, fp4_bf16(w, fp4_power((ex >> (8 * (2 * (kb >> 2) + h))) & 0xffu)));
 #pragma unroll
-                for (int qt = 0; qt < QT; ++qt)
-                    S[qt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[qt], S[qt][h], 0, 0, 0);
-            }
-        }
-        float kscale[8], vscale[8];
-        if constexpr (VS) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                if constexpr (I8) kscale[e] = __uint_as_float(ksc[e >> 2][e & 3]) * a.scale;
-                vscale[e] = __uint_as_float(vsc[e >> 2][e & 3]);
-            }
-        }
-        if (more) load_k(pn, next);
-        // scores, by token of the lane's eight; tiles that some row does not see whole are masked
-        const int j0 = tile * KV_TILE, jl = j0 + 8 * g;
-        const bool whole = (!SEL || tile >= 0) && j0 + KV_TILE - 1 <= pos0 &&
-                           (a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
-        at_bf16x8 ph[QT], pl[QT];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt) {
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                x[e] = S[qt][e >> 2][e & 3] * (I8 ? kscale[e] : a.scale);
-            }
-            uint32_t seen = 0xffu;
-            if (!whole) {
-                const Sight sight{a.window, a.sinks};
-                seen = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool in = (!SEL || tile >= 0) && sight.sees(jl + e, pos[qt]);
-                    seen |= in ? 1u << e : 0u;
-                    x[e] = in ? x[e] : -__builtin_inff();
+                    for (int qt = 0; qt < QT; ++qt)
+                        S[qt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[qt], S[qt][h], 0, 0, 0);
                 }
             }
-            float mt = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-            mt = fmaxf(m[qt], max_over_groups(mt));
-            const float ms = mt == -__builtin_inff() ? 0.0f : mt;
-            const float f = __builtin_amdgcn_exp2f(m[qt] - ms);
-            m[qt] = mt;
-            float sum = 0.0f;
-            float p[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(x[e] - ms);
-                sum += p[e];
-                if constexpr (VS) p[e] = (seen >> e) & 1 ? p[e] * vscale[e] : 0.0f;
-            }
-            l[qt] = l[qt] * f + sum;
-#pragma unroll
-            for (int db = 0; db < NDB; ++db) O[qt][db] *= f;
-            u32x4 h, r;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t w = f2bf2(p[2 * e], p[2 * e + 1]);
-                h[e] = w;
-                r[e] = f2bf2(p[2 * e] - bf16f(w & 0xffffu), p[2 * e + 1] - bf16f(w >> 16));
-            }
-            ph[qt] = __builtin_bit_cast(at_bf16x8, h);
-            pl[qt] = __builtin_bit_cast(at_bf16x8, r);
-        }
-        if (!VS && (j0 + KV_TILE > len || (SEL && tile < 0))) {  // places past the length hold anything
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    vr[i][e] &= SEL && tile < 0 ? 0u : (jl + 2 * e < len ? 0xffffu : 0u) | (jl + 2 * e + 1 < len ? 0xffff0000u : 0u);
-            }
-        }
-        if constexpr (VS) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(vr[i]));
-        }
-#pragma unroll
-        for (int db = 0; db < NDB; ++db) {
-            at_bf16x8 vv;
-            if constexpr (I8) {
-                const u32x4 w = vr[db >> 1];
-                vv = db & 1 ? codes_bf16(w.z, w.w) : codes_bf16(w.x, w.y);
-            } else if constexpr (F4) {
-                vv = __builtin_bit_cast(at_bf16x8, fp4_bf16(vr[db >> 2][db & 3], 1.0f));
-            } else {
-                vv = __builtin_bit_cast(at_bf16x8, vr[db]);
-            }
+            load_k(next);
+            const int j0 = tile * KV_TILE, jl = j0 + 8 * g;
+            const bool whole = (!SEL || tile >= 0) && j0 + KV_TILE - 1 <= pos0 &&
+                               (a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
+            at_bf16x8 ph[QT], pl[QT];
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
-                O[qt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, ph[qt], O[qt][db], 0, 0, 0);
-                O[qt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pl[qt], O[qt][db], 0, 0, 0);
+                float x[8], vs[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = S[qt][e >> 2][e & 3];
+                    vs[e] = __uint_as_float(vsc[e >> 2][e & 3]);
+                }
+                if (!whole) {
+                    const Sight sight{a.window, a.sinks};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const bool in = (!SEL || tile >= 0) && sight.sees(jl + e, pos[qt]);
+                        x[e] = in ? x[e] : -__builtin_inff();
+                        vs[e] = in ? vs[e] : 0.0f;
+                    }
+                }
+                auto larger = [](float u, float v) { return __builtin_amdgcn_fmed3f(u, v, __builtin_inff()); };
+                const float mt = larger(larger(larger(x[0], x[1]), larger(x[2], x[3])), larger(larger(x[4], x[5]), larger(x[6], x[7])));
+                const float top = max_over_groups(mt) * a.scale;
+                if (__any(top > m[qt] + LAG)) {
+                    const float M = fmaxf(m[qt], top), f = part_weight(m[qt], M);
+                    l[qt] *= f;
+#pragma unroll
+                    for (int db = 0; db < NDB; ++db) O[qt][db] *= f;
+                    m[qt] = M;
+                }
+                const float ms = m[qt] == -__builtin_inff() ? 0.0f : m[qt];
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], a.scale, -ms));
+                    l[qt] += p[e];
+                    p[e] *= vs[e];
+                }
+                u32x4 h, r;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = f2bf2(p[2 * e], p[2 * e + 1]);
+                    h[e] = w;
+                    r[e] = f2bf2(p[2 * e] - bf16f(w & 0xffffu), p[2 * e + 1] - bf16f(w >> 16));
+                }
+                ph[qt] = __builtin_bit_cast(at_bf16x8, h);
+                pl[qt] = __builtin_bit_cast(at_bf16x8, r);
             }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(vr[i]));
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) {
+                const at_bf16x8 vv = __builtin_bit_cast(at_bf16x8, fp4_bf16(vr[db >> 2][db & 3], 1.0f));
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    O[qt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, ph[qt], O[qt][db], 0, 0, 0);
+                    O[qt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pl[qt], O[qt][db], 0, 0, 0);
+                }
+            }
+            load_v(next);
+            tile = t1;
+            t1 = t2;
         }
-        if (more) load_v(pn, next);
+    } else {
+        u32x4 kr[NK], vr[NV];
+        u32x4 ksc[2], vsc[2];
+        constexpr int TB = KV_TILE * D * (I8 ? 1 : 2);  // bytes of a tile
+        // A tile that one workgroup reads is not kept (131072 tokens, one row: 58 us
+        // instead of 68); several groups of rows read it again from L2.
+        constexpr int AUX = QT < at_qt_max(D) && QT <= 2 ? AUX_NT : 0;
+        auto load_tile = [&](const void* pool, size_t at, u32x4* r, auto n) {
+            const auto t = buf((const uint8_t*)pool + at * TB, TB);
+#pragma unroll
+            for (int i = 0; i < n(); ++i) {
+                const i32x4 w = __builtin_amdgcn_raw_buffer_load_b128(t, lane * 16 + (i & 3) * 1024, (i >> 2) * 4096, AUX);
+                r[i] = u32x4{(uint32_t)w.x, (uint32_t)w.y, (uint32_t)w.z, (uint32_t)w.w};
+            }
+        };
+        auto load_scales = [&](const float* pool, size_t at, u32x4* r) {
+            const auto t = buf(pool + at * KV_TILE, KV_TILE * 4);
+            r[0] = bload16(t, g * 32);
+            r[1] = bload16(t, g * 32 + 16);
+        };
+        auto load_k = [&](int page, int tile) {
+            const size_t at = kv_tile_at(a.c, page, head, tile);
+            load_tile(a.c.k, at, kr, [] { return NK; });
+            if constexpr (I8) load_scales(a.c.ks, at, ksc);
+        };
+        auto load_v = [&](int page, int tile) {
+            const size_t at = kv_tile_at(a.c, page, head, tile);
+            load_tile(a.c.v, at, vr, [] { return NV; });
+            if constexpr (I8) load_scales(a.c.vs, at, vsc);
+        };
+
+        // A tile's K is asked for once the products that read the one before are
+        // issued, its V likewise, its page two tiles ahead.  A tile whose page is missing
+        // reads page 0 and makes the sums of every row of the wave NaN (row_again sorts them out).
+        // (SEL: a tile's number is known one tile earlier still; of none, -1, the first of the pool
+        // is read and nothing of it seen)
+        auto page_of = [&](int v, int tile) {
+            const int p = v < tiles && tile >= 0 ? kv_page_uniform(a.c, b, tile) : 0;
+            if (p < 0) missing = true;
+            return max(p, 0);
+        };
+        auto number = [&](int v) { return SEL ? list.tile_uniform(v) : s.tile_of(v); };
+        int tn = number(v0), tnn = number(v0 + stride), t3 = SEL ? number(v0 + 2 * stride) : 0;
+        if (v0 < tiles) {
+            int p = page0;
+            if (SEL) p = tn >= 0 ? kv_page_uniform(a.c, b, tn) : 0;
+            else if (a.window != 0) p = kv_page_uniform(a.c, b, tn);
+            if ((unsigned)p >= (unsigned)a.c.pages) {
+                missing = true;
+                p = 0;
+            }
+            load_k(p, max(tn, 0));
+            load_v(p, max(tn, 0));
+        }
+        int pn, pnn = page_of(v0 + stride, tnn);
+#pragma unroll
+        for (int k = 0; k < QN; ++k)
+            if (QC % NT == 0 || tid + k * NT < QC) lq[tid + k * NT] = qv[k];
+        lds_barrier();
+        for (int v = v0; v < tiles; v += stride) {
+            const int tile = SEL ? tn : s.tile_of(v), next = SEL ? max(tnn, 0) : s.tile_of(v + stride);
+            const bool more = v + stride < tiles;
+            pn = pnn;
+            if constexpr (SEL) {
+                tn = tnn;
+                tnn = t3;
+                t3 = number(v + 3 * stride);
+                pnn = page_of(v + 2 * stride, tnn);
+            } else {
+                pnn = page_of(v + 2 * stride, s.tile_of(v + 2 * stride));
+            }
+            issue_fence();  // (Q is read again for each tile: its registers go to K and V)
+            if constexpr (I8) {  // (codes are not widened before their tile's turn)
+#pragma unroll
+                for (int i = 0; i < NK; ++i) asm volatile("" : "+v"(kr[i]));
+            }
+            at_f32x4 S[QT][2];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) S[qt][0] = S[qt][1] = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb) {
+                at_bf16x8 qf[QT];
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) qf[qt] = __builtin_bit_cast(at_bf16x8, lq[(qt * NKB + kb) * 64 + lane]);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    at_bf16x8 k;
+                    if constexpr (I8) {
+                        const u32x4 w = kr[(kb >> 1) * 2 + h];
+                        k = kb & 1 ? codes_bf16(w.z, w.w) : codes_bf16(w.x, w.y);
+                    } else {
+                        k = __builtin_bit_cast(at_bf16x8, kr[kb * 2 + h]);
+                    }
+#pragma unroll
+                    for (int qt = 0; qt < QT; ++qt)
+                        S[qt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k, qf[qt], S[qt][h], 0, 0, 0);
+                }
+            }
+            float kscale[8], vscale[8];
+            if constexpr (I8) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    kscale[e] = __uint_as_float(ksc[e >> 2][e & 3]) * a.scale;
+                    vscale[e] = __uint_as_float(vsc[e >> 2][e & 3]);
+                }
+            }
+            if (more) load_k(pn, next);
+            // scores, by token of the lane's eight; tiles that some row does not see whole are masked
+            const int j0 = tile * KV_TILE, jl = j0 + 8 * g;
+            const bool whole = (!SEL || tile >= 0) && j0 + KV_TILE - 1 <= pos0 &&
+                               (a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
+            at_bf16x8 ph[QT], pl[QT];
+#pragma unroll
+            for (int qt = 0; qt < QT; ++qt) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = S[qt][e >> 2][e & 3] * (I8 ? kscale[e] : a.scale);
+                }
+                uint32_t seen = 0xffu;
+                if (!whole) {
+                    const Sight sight{a.window, a.sinks};
+                    seen = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const bool in = (!SEL || tile >= 0) && sight.sees(jl + e, pos[qt]);
+                        seen |= in ? 1u << e : 0u;
+                        x[e] = in ? x[e] : -__builtin_inff();
+                    }
+                }
+                float mt = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
+                mt = fmaxf(m[qt], max_over_groups(mt));
+                const float ms = mt == -__builtin_inff() ? 0.0f : mt;
+                const float f = __builtin_amdgcn_exp2f(m[qt] - ms);
+                m[qt] = mt;
+                float sum = 0.0f;
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f(x[e] - ms);
+                    sum += p[e];
+                    if constexpr (I8) p[e] = (seen >> e) & 1 ? p[e] * vscale[e] : 0.0f;
+                }
+                l[qt] = l[qt] * f + sum;
+#pragma unroll
+                for (int db = 0; db < NDB; ++db) O[qt][db] *= f;
+                u32x4 h, r;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t w = f2bf2(p[2 * e], p[2 * e + 1]);
+                    h[e] = w;
+                    r[e] = f2bf2(p[2 * e] - bf16f(w & 0xffffu), p[2 * e + 1] - bf16f(w >> 16));
+                }
+                ph[qt] = __builtin_bit_cast(at_bf16x8, h);
+                pl[qt] = __builtin_bit_cast(at_bf16x8, r);
+            }
+            if (!I8 && (j0 + KV_TILE > len || (SEL && tile < 0))) {  // places past the length hold anything
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        vr[i][e] &= SEL && tile < 0 ? 0u : (jl + 2 * e < len ? 0xffffu : 0u) | (jl + 2 * e + 1 < len ? 0xffff0000u : 0u);
+                }
+            }
+            if constexpr (I8) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) asm volatile("" : "+v"(vr[i]));
+            }
+#pragma unroll
+            for (int db = 0; db < NDB; ++db) {
+                at_bf16x8 vv;
+                if constexpr (I8) {
+                    const u32x4 w = vr[db >> 1];
+                    vv = db & 1 ? codes_bf16(w.z, w.w) : codes_bf16(w.x, w.y);
+                } else {
+                    vv = __builtin_bit_cast(at_bf16x8, vr[db]);
+                }
+#pragma unroll
+                for (int qt = 0; qt < QT; ++qt) {
+                    O[qt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, ph[qt], O[qt][db], 0, 0, 0);
+                    O[qt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, pl[qt], O[qt][db], 0, 0, 0);
+                }
+            }
+            if (more) load_v(pn, next);
+        }
     }
 
     // the waves meet
@@ -701,7 +900,7 @@ attn_kernel(AttnArgs a) {
     auto store = [&](int rr, int d, at_f32x4 o, float M, float lt) {
         if (!attn_store<D, ROWS, SEL>(a, s, qg, head, rr, d, o, lt)) once_more(rr, make_float2(M, lt));
     };
-    const auto recs = buf(a.part + (size_t)rec * a.splits * PF, (uint32_t)(parts * PF * 4));
+    const auto recs = buf(a.part + part_at(a, rec, first, qg, head) * PF, (uint32_t)(parts * PF * 4));
     for (int i = tid; i < rows * (D / 4); i += NT) {
         const int rr = i / (D / 4), d = i % (D / 4) * 4;
         float M = lml[2 * rr];
@@ -775,11 +974,19 @@ attn_join_kernel(AttnArgs a) {
         qg = head / a.c.kvh;
         head -= qg * a.c.kvh;
     }
-    const AttnSeq s = attn_seq<ROWS, W, SEL>(a, kv_seq(a.c, b), qg, row);
+    int splits = a.splits, first = -1;
+    if constexpr (KT == VIPER_KV_FP4 && !SEL) {
+        if (a.share) {
+            const AttnShare sh = attn_share(a, W, -1, b);
+            splits = sh.splits;
+            first = sh.first;
+        }
+    }
+    const AttnSeq s = attn_seq<ROWS, W, SEL>(a, kv_seq(a.c, b), qg, row, splits);
     if (rr >= s.rows || s.parts == 1) return;
     const int rec = ((qg * a.c.batch + b) * (SEL ? a.c.max_rows : 1) + row) * a.c.kvh + head;
     constexpr int PF = (int)at_part_floats(D, QT);
-    const auto recs = buf(a.part + (size_t)rec * a.splits * PF, (uint32_t)(s.parts * PF * 4));
+    const auto recs = buf(a.part + part_at(a, rec, first, qg, head) * PF, (uint32_t)(s.parts * PF * 4));
     attn_lay(lds, AT_JNT, attn_join<D, ROWS>(recs, rr, tid % U * 8, tid / U, G, s.parts));
     if (tid == 0) again = 0;
     __syncthreads();

@@ -25,15 +25,16 @@ AttnFn attn_selected_fp4(int D, int qt, int W);
 // Parts of equal steps dealt out over all sequences of a batch, whatever their
 // lengths, were slower (32 x 8192 tokens 92.9 us against 85.7, 256 x 600 76 against
 // 36): a part that ends one sequence and begins another waits at both.
-constexpr int AT_WAVES = 8, AT_PARTS = 64, AT_SHORT = 4096 / KV_TILE, AT_APART = 80000;
+constexpr int AT_WAVES = 8, AT_SHORT = 4096 / KV_TILE, AT_APART = 80000;
 
 struct AttnPlan {
     int qt, qgroups, waves, splits, lrows;
+    int shared;  // parts of all sequences together where they are shared out by length, 0: not
     size_t bytes;  // of workspace; 0: one part
 };
 
 // `units` sequences of `rows` rows that look at up to `tiles` tiles each
-static AttnPlan attn_plan(const viper_kv_cache* c, int rows, int64_t units, int64_t tiles, int heads) {
+static AttnPlan attn_plan(const viper_kv_cache* c, int rows, int64_t units, int64_t tiles, int heads, bool share) {
     AttnPlan p;
     const int gqa = heads / c->kv_heads, most = at_qt_max(c->head_dim);
     const int t16 = (rows * gqa + 15) / 16;
@@ -44,24 +45,31 @@ static AttnPlan attn_plan(const viper_kv_cache* c, int rows, int64_t units, int6
     p.waves = at_waves(c->head_dim, p.qt);
     if (tiles <= AT_SHORT) p.waves = 4;
     int64_t s = 1;
+    p.shared = 0;
     if (base <= AT_CNT) {
         const bool two = units > 1 && at_two(c->head_dim, c->kv_type != VIPER_KV_BF16, p.qt);
         const int64_t wgs = (int64_t)device_cus() * AT_WAVES * (two ? 2 : 1) / p.waves;
         s = (wgs + base - 1) / base;
         const int64_t fit = (tiles + p.waves - 1) / p.waves;
+        if (share && units > 1 && units <= 64 && s > 1 && fit > 1) {
+            const int64_t all = wgs / (c->kv_heads * p.qgroups);  // (at least one to a sequence)
+            p.shared = (int)(all < units * fit ? all : units * fit);
+        }
         if (s > fit) s = fit;
         if (s > AT_PARTS) s = AT_PARTS;
     }
     p.splits = (int)s;
-    p.bytes = s > 1 ? AT_CNT * 4 + (size_t)base * s * at_part_floats(c->head_dim, p.qt) * 4 : 0;
+    const int64_t parts = base * s, shared = (int64_t)p.shared * c->kv_heads * p.qgroups;
+    p.bytes = s > 1 ? AT_CNT * 4 + (size_t)(parts > shared ? parts : shared) * at_part_floats(c->head_dim, p.qt) * 4 : 0;
     return p;
 }
 static AttnPlan attn_plan(const viper_kv_cache* c, const viper_kv_batch* b, int heads) {
-    return attn_plan(c, b->max_rows, b->batch, (int64_t)b->table_width * (c->page_size / KV_TILE), heads);
+    return attn_plan(c, b->max_rows, b->batch, (int64_t)b->table_width * (c->page_size / KV_TILE), heads,
+                     c->kv_type == VIPER_KV_FP4);
 }
 // (over lists, every row is a sequence of its own)
 static AttnPlan attn_plan_selected(const viper_kv_cache* c, const viper_kv_batch* b, int heads, int count) {
-    return attn_plan(c, 1, (int64_t)b->batch * b->max_rows, (int64_t)count * (c->page_size / KV_TILE), heads);
+    return attn_plan(c, 1, (int64_t)b->batch * b->max_rows, (int64_t)count * (c->page_size / KV_TILE), heads, false);
 }
 
 static int attn_check(const viper_kv_cache* c, const viper_kv_batch* b, int heads) {
@@ -111,6 +119,8 @@ static int attn_call(const viper_kv_cache* cache, const viper_kv_batch* batch, c
     a.scale = scale * 1.44269504088896340736f;
     a.sel = sel;
     a.count = count;
+    a.share = p.splits > 1 && p.shared > 0 && a.window == 0;
+    if (a.share) a.splits = p.shared;
     const int D = cache->head_dim, rows = sel != nullptr ? batch->max_rows : 1;
     const int kind = (cache->kv_type == VIPER_KV_INT8 ? 1 : cache->kv_type == VIPER_KV_FP4 ? 2 : 0) + (sel != nullptr ? 3 : 0);
     static AttnFn (*const of[])(int, int, int) = {attn_kernels_bf16,  attn_kernels_int8,  attn_kernels_fp4,
@@ -120,13 +130,13 @@ static int attn_call(const viper_kv_cache* cache, const viper_kv_batch* batch, c
     a.by_gqa = (65536u + (unsigned)a.gqa - 1) / (unsigned)a.gqa;
     a.apart = p.splits > 1 && (int64_t)p.splits * p.lrows * D * 4 >= AT_APART;
     void* args[] = {&a};
-    const dim3 grid((unsigned)(p.splits * rows), (unsigned)(cache->kv_heads * p.qgroups), (unsigned)batch->batch);
+    const dim3 grid((unsigned)(a.splits * rows), (unsigned)(cache->kv_heads * p.qgroups), a.share ? 1u : (unsigned)batch->batch);
     (void)hipLaunchKernel(fn.attn, grid, dim3((unsigned)p.waves * 64), args, at_lds_bytes(D, p.qt, p.waves, p.lrows),
                           (hipStream_t)stream);
     if (a.apart) {
         const int rc2 = status_of(hipGetLastError());
         if (rc2 != VIPER_OK) return rc2;
-        (void)hipLaunchKernel(fn.join, dim3((unsigned)(p.lrows * rows), grid.y, grid.z), dim3(AT_JNT), args, 0, (hipStream_t)stream);
+        (void)hipLaunchKernel(fn.join, dim3((unsigned)(p.lrows * rows), grid.y, (unsigned)batch->batch), dim3(AT_JNT), args, 0, (hipStream_t)stream);
     }
     return status_of(hipGetLastError());
 }

@@ -85,6 +85,17 @@ __device__ __forceinline__ float fp4_power(uint32_t byte) { return __uint_as_flo
 typedef const __attribute__((address_space(4))) int32_t* kv_cptr;
 __device__ __forceinline__ int kv_sload(const int32_t* p, size_t i) { return ((kv_cptr)(uintptr_t)p)[i]; }
 
+// Sum over the lanes of a wave up to the lane's own
+__device__ __forceinline__ unsigned wave_upto(unsigned v) {
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes back in the row
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // a row's last lane to the row behind it
+    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // the lower half's to the upper half
+    return v;
+}
+
 // Sequence b's rows: the first, their count (0 where the offsets do not fit)
 // and the sequence's length.
 struct KvSeq {

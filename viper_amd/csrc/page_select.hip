@@ -322,7 +322,7 @@ __device__ __forceinline__ uint32_t page_exact(const uint16_t* at, const uint16_
     return ps_key((float)wave_sum(sum));
 }
 
-// Least / largest / sum of the lanes before and the lane's own, over a wave
+// Least / largest over a wave
 template <bool MAX>
 __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
     auto of = [](uint32_t x, uint32_t y) { return MAX ? max(x, y) : min(x, y); };
@@ -334,15 +334,6 @@ __device__ __forceinline__ uint32_t wave_most(uint32_t v) {
     v = of(r[0], r[1]);
     r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return of(r[0], r[1]);
-}
-__device__ __forceinline__ unsigned wave_upto(unsigned v) {
-    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes back in the row
-    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, false);
-    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, false);
-    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, false);
-    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);  // a row's last lane to the row behind it
-    v += (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);  // the lower half's to the upper half
-    return v;
 }
 
 // A workgroup per row and key head.  A wave holds KPT 64 consecutive pages, a lane every
