@@ -605,7 +605,8 @@ int viper_hip_attention_paged(const viper_kv_cache* cache, const viper_kv_batch*
  * least and the largest value of each dimension over the keys that the sequence
  * holds there, as kv_read gives them back; both NaN where a key is.  Other pages'
  * are left as they were, so a call after every kv_append of a batch keeps them all.
- * A page that two sequences of one call hold unequal parts of gets those of either. */
+ * A page that two sequences of one call hold unequal parts of gets those of either.
+ * batch kv_heads (ceil((min(max_rows, total_rows) - 1) / page_size) + 1) < 2^24. */
 int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper_kv_batch* batch, void* bounds_bf16, void* stream);
 
 /* selected int32 [total_rows][kv_heads][count]: the pages that a row at position p

@@ -35,90 +35,127 @@ __device__ __forceinline__ uint32_t pb_min(uint32_t a, uint32_t b) {
 __device__ __forceinline__ uint32_t pb_max(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(pb_i16x2, a), __builtin_bit_cast(pb_i16x2, b)));
 }
-template <int CTRL>
-__device__ __forceinline__ void pb_step(uint32_t* lo, uint32_t* hi) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        lo[i] = pb_min(lo[i], (uint32_t)dpp_i<CTRL>((int)lo[i]));
-        hi[i] = pb_max(hi[i], (uint32_t)dpp_i<CTRL>((int)hi[i]));
-    }
-}
+constexpr int DPP_ROR8 = 0x128;  // lane i <- i ^ 8 within 16
 
-// A workgroup per page and head; a wave takes chunks of 32 dims of all tiles, a lane the
-// octet of the token that the tile's order gives it.
+// A wave takes a page of a key head (of pages of several tiles two or four waves, which
+// meet in LDS) with the tile's 16-byte loads.  The least and, complemented, the largest of a
+// lane's token are R registers; each step of the way over the 16 lanes of other tokens
+// halves them, a lane keeping the half that one bit of its number says.  3 prompts of
+// 20000 tokens in pages of 32, int8: 4 pages to a workgroup of one wave for each 32 dims took 11.5 us.
 template <int D, int KT>
 __global__ void __launch_bounds__(PB_NT)
 page_bounds_kernel(BoundsArgs a) {
-    constexpr int NKB = D / 32, W = NKB < 4 ? NKB : 4;
+    constexpr int NKB = D / 32, R = 8 * NKB, N = R / 16;
+    __shared__ uint32_t lv[PB_NT / 64][64][N];
     const int tid = (int)threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    int id = (int)blockIdx.x;
-    const int head = id % a.c.kvh;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wl = min(a.c.tpl, 2), part = wave & ((1 << wl) - 1);
+    int64_t id = ((int64_t)blockIdx.x * (PB_NT / 64) + wave) >> wl;
+    const int head = (int)(id % a.c.kvh);
     id /= a.c.kvh;
-    const int b = id / a.span;
-    const KvSeq s = kv_seq(a.c, b);
-    if (s.n == 0 || s.len <= 0) return;
+    const int b = (int)(id / a.span);
+    const KvSeq s = b < a.c.batch ? kv_seq(a.c, b) : KvSeq{0, 0, 0};
     const int from = max(0, s.len - s.n), shift = a.c.tpl + 5;
     const int64_t page64 = (int64_t)(from >> shift) + id % a.span;
-    if (page64 << shift >= s.len) return;
-    const int tile0 = (int)(page64 << a.c.tpl), tiles = min(1 << a.c.tpl, (s.len - 1) / KV_TILE - tile0 + 1);
-    const int page = kv_page_uniform(a.c, b, tile0);
-    if (page < 0) return;
-    for (int kb = wave; kb < NKB; kb += W) {
-        uint32_t lo[4], hi[4];
+    const bool live = s.n > 0 && page64 << shift < s.len;
+    const int tile0 = live ? (int)(page64 << a.c.tpl) : 0;
+    const int tiles = live ? min(1 << a.c.tpl, (s.len - 1) / KV_TILE - tile0 + 1) : 0;
+    const int page = live ? kv_page_uniform(a.c, b, tile0) : -1;
+    // words [side][32 dims][pair of dims], of the largest the complement: all are made smaller
+    uint32_t v[R];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            lo[i] = 0x7fff7fffu;
-            hi[i] = 0x80008000u;
-        }
-#pragma unroll 2
-        for (int tl = 0; tl < tiles; ++tl) {
-            const size_t at = kv_tile_at(a.c, page, head, tl);
+    for (int i = 0; i < R; ++i) v[i] = 0x7fff7fffu;
+    for (int tl = part; tl < tiles && page >= 0; tl += 1 << wl) {
+        const size_t at = kv_tile_at(a.c, page, head, tl);
+        u32x4 x[NKB][2];
+        if constexpr (KT == VIPER_KV_BF16) {
+            const u32x4* const p = (const u32x4*)((const uint16_t*)a.c.k + at * (KV_TILE * D)) + lane;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int t = 8 * (m >> 2) + 4 * h + (m & 3), c = 4 * kb + g;
-                u32x4 x;
-                if constexpr (KT == VIPER_KV_BF16) {
-                    x = *(const u32x4*)((const uint16_t*)a.c.k + at * (KV_TILE * D) + k_place<false>(t, c));
-                } else if constexpr (KT == VIPER_KV_INT8) {
-                    const u32x2 w = *(const u32x2*)((const int8_t*)a.c.k + at * (KV_TILE * D) + k_place<true>(t, c));
-                    const float sc = a.c.ks[at * KV_TILE + t];
+            for (int i = 0; i < 2 * NKB; ++i) x[i >> 1][i & 1] = p[64 * i];
+        } else if constexpr (KT == VIPER_KV_INT8) {
+            const u32x4* const p = (const u32x4*)((const int8_t*)a.c.k + at * (KV_TILE * D)) + lane;
+            u32x4 w[NKB];
+#pragma unroll
+            for (int i = 0; i < NKB; ++i) w[i] = p[64 * i];
+            float sc[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) sc[h] = a.c.ks[at * KV_TILE + 8 * (m >> 2) + 4 * h + (m & 3)];
+#pragma unroll
+            for (int i = 0; i < NKB; ++i) {
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {  // dims 64 (i / 2) + 32 k + 8 g ..
                     float y[8];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] = (float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))) * sc;
-                    x = u32x4{f2bf2(y[0], y[1]), f2bf2(y[2], y[3]), f2bf2(y[4], y[5]), f2bf2(y[6], y[7])};
-                } else {
-                    const uint32_t w = *(const uint32_t*)((const uint8_t*)a.c.k + at * (KV_TILE * D / 2) + k4_place<D>(t, c));
-                    x = fp4_bf16(w, fp4_power(((const uint8_t*)a.c.ks)[at * D + k4_exp_place<D>(t, kb)]));
+                    for (int j = 0; j < 8; ++j) y[j] = (float)(int8_t)(w[i][2 * k + (j >> 2)] >> (8 * (j & 3))) * sc[i & 1];
+                    x[2 * (i >> 1) + k][i & 1] = u32x4{f2bf2(y[0], y[1]), f2bf2(y[2], y[3]), f2bf2(y[4], y[5]), f2bf2(y[6], y[7])};
                 }
-                const bool held = (tile0 + tl) * KV_TILE + t < s.len;
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            }
+        } else {
+            const u32x4* const p = (const u32x4*)((const uint8_t*)a.c.k + at * (KV_TILE * D / 2)) + lane;
+            const uint8_t* const e = (const uint8_t*)a.c.ks + at * D;
+            u32x4 w[D / 64];
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) w[i] = p[64 * i];
+            const uint32_t ex = D == 256 ? *(const uint32_t*)(e + 4 * lane) : *(const uint16_t*)(e + (D == 64 ? 2 * (16 * (g >> 1) + m) : 2 * lane));
+#pragma unroll
+            for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    x[kb][h] = fp4_bf16(D == 64 ? w[0][2 * h + kb] : w[2 * (kb >> 2) + h][kb & 3],
+                                        fp4_power((ex >> (8 * (2 * (kb >> 2) + h))) & 0xffu));
+            }
+        }
+        const bool whole = (tile0 + tl + 1) * KV_TILE <= s.len;
+#pragma unroll
+        for (int kb = 0; kb < NKB; ++kb) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const bool held = whole || (tile0 + tl) * KV_TILE + 8 * (m >> 2) + 4 * h + (m & 3) < s.len;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t v = pb_order(w[i]);
-                    lo[i] = pb_min(lo[i], held ? v : 0x7fff7fffu);
-                    hi[i] = pb_max(hi[i], held ? v : 0x80008000u);
+                    const uint32_t u = pb_order(x[kb][h][i]);
+                    v[4 * kb + i] = pb_min(v[4 * kb + i], held ? u : 0x7fff7fffu);
+                    v[4 * (NKB + kb) + i] = pb_min(v[4 * (NKB + kb) + i], held ? ~u : 0x7fff7fffu);
                 }
             }
         }
-        pb_step<DPP_SWAP1>(lo, hi);
-        pb_step<DPP_SWAP2>(lo, hi);
-        pb_step<DPP_HALF_MIRROR>(lo, hi);
-        pb_step<DPP_MIRROR>(lo, hi);
-        if (m < 2) {  // one lane stores the least, one the largest values
-            u32x4 v;
+    }
+    auto halve = [&](auto dpp, bool upper, int half) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t l = pb_order(lo[i]), u = pb_order(hi[i]);
-                v[i] = m == 0 ? l : u;
-                // a NaN key makes both NaN
-                const uint32_t n0 = (l & 0x7fffu) > 0x7f80u || (u & 0x7fffu) > 0x7f80u ? 0x7fc0u : 0u;
-                const uint32_t n1 = (l >> 16 & 0x7fffu) > 0x7f80u || (u >> 16 & 0x7fffu) > 0x7f80u ? 0x7fc00000u : 0u;
-                v[i] = n0 != 0u ? (v[i] & 0xffff0000u) | n0 : v[i];
-                v[i] = n1 != 0u ? (v[i] & 0xffffu) | n1 : v[i];
-            }
-            *(u32x4*)(a.out + (((size_t)page * a.c.kvh + head) * 2 + m) * D + 32 * kb + 8 * g) = v;
+        for (int i = 0; i < R / 2; ++i) {
+            if (i >= half) continue;
+            const uint32_t keep = upper ? v[i + half] : v[i], send = upper ? v[i] : v[i + half];
+            v[i] = pb_min(keep, (uint32_t)dpp((int)send));
         }
+    };
+    // (the half mirror turns the lower bits too: it comes before they choose)
+    halve([](int x) { return dpp_i<DPP_ROR8>(x); }, m & 8, R / 2);
+    halve([](int x) { return dpp_i<DPP_HALF_MIRROR>(x); }, m & 4, R / 4);
+    halve([](int x) { return dpp_i<DPP_SWAP2>(x); }, m & 2, R / 8);
+    halve([](int x) { return dpp_i<DPP_SWAP1>(x); }, m & 1, R / 16);
+    if (wl > 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) lv[wave][lane][i] = v[i];
+        __syncthreads();
+        if (part != 0) return;
+        for (int w = 1; w < 1 << wl; ++w) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) v[i] = pb_min(v[i], lv[wave + w][lane][i]);
+        }
+    }
+    if (page < 0) return;
+    // word `first` of the lane's N: its side, 32 dims and pair
+    const int first = (m >> 2 & 1) * (R / 4) + (m >> 1 & 1) * (R / 8) + (m & 1) * (R / 16), kb = first / 4;
+    const int dim = (KT == VIPER_KV_FP4 ? q4_dim<D>(kb, g) : 32 * kb + 8 * g) + 2 * (first & 3);
+    uint32_t* const out = (uint32_t*)(a.out + (((size_t)page * a.c.kvh + head) * 2 + (m >> 3)) * D + dim);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t mine = pb_order(m & 8 ? ~v[i] : v[i]), other = (uint32_t)dpp_i<DPP_ROR8>((int)mine);
+        // a NaN key makes both NaN
+        auto nan = [](uint32_t w) { return (w & 0x7fffu) > 0x7f80u; };
+        uint32_t w = mine;
+        if (nan(mine) || nan(other)) w = (w & 0xffff0000u) | 0x7fc0u;
+        if (nan(mine >> 16) || nan(other >> 16)) w = (w & 0xffffu) | 0x7fc00000u;
+        out[i] = w;
     }
 }
 
@@ -632,11 +669,12 @@ extern "C" int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper
     a.c.max_rows = batch->max_rows < batch->total_rows ? batch->max_rows : batch->total_rows;
     a.out = (uint16_t*)bounds_bf16;
     a.span = (int)(((int64_t)a.c.max_rows + cache->page_size - 2) / cache->page_size + 1);
-    const int64_t grid = (int64_t)batch->batch * a.span * cache->kv_heads;
-    if (grid >= 1 << 24) return VIPER_INVALID_ARGUMENT;
+    const int64_t units = (int64_t)batch->batch * a.span * cache->kv_heads;
+    if (units >= 1 << 24) return VIPER_INVALID_ARGUMENT;
+    const int waves = PB_NT / 64, per = waves >> (a.c.tpl < 2 ? a.c.tpl : 2);
     const int D = cache->head_dim, kv = cache->kv_type;
     void* args[] = {&a};
-    launch(D == 64 ? bounds_fn<64>(kv) : D == 128 ? bounds_fn<128>(kv) : bounds_fn<256>(kv), (unsigned)grid, D == 64 ? 128 : 256, 0,
+    launch(D == 64 ? bounds_fn<64>(kv) : D == 128 ? bounds_fn<128>(kv) : bounds_fn<256>(kv), (unsigned)((units + per - 1) / per), PB_NT, 0,
            (hipStream_t)stream, args);
     return status_of(hipGetLastError());
 }
