@@ -33,7 +33,10 @@ o projection q and k are rotated, k and v stored and the new token attends over
 its sequence (two launches more, kv_append and attention_paged), in place of the
 fixed activation.  The sequence's length is on the device and grows by one in
 each step, a captured step's replays included; past `capacity` tokens results
-are NaN.
+are NaN.  With `select` > 0 the new token attends over that many pages of each
+slot's cache alone: the first `keep_first`, the last `keep_last` and those whose
+keys' bounds promise most (kv_page_bounds, select_pages and attention_selected in
+place of attention_paged).
 """
 import ctypes as C
 import math
@@ -47,7 +50,7 @@ Q4 = int(_q.QType.Q4_G64)
 class Stack:
     def __init__(self, torch, hidden=2560, inter=10240, n_heads=20, n_kv_heads=4, head_dim=128,
                  layers=22, passes=2, vocab=166144, seed=0x5EED0003, eps=1e-6, context=0, kv_type=_d.KVType.BF16, page_size=64,
-                 rope_theta=10000.0, window=0, sinks=0):
+                 rope_theta=10000.0, window=0, sinks=0, select=0, keep_first=1, keep_last=2):
         self.torch = torch
         self.H, self.I = hidden, inter
         self.nQ, self.nKV = n_heads * head_dim, n_kv_heads * head_dim
@@ -135,15 +138,33 @@ class Stack:
             self.rows = _d.KVBatch(table, self.seq_len)
             # one workspace: the slots' launches follow one another
             nws = _d.attention_workspace_bytes(self.kv[0], self.rows, n_heads)
+            self.select, self.keep = select, dict(first=keep_first, last=keep_last)
+            if select:
+                if window:
+                    raise ValueError("Stack: select and window exclude each other")
+                nws = _d.attention_selected_workspace_bytes(self.kv[0], self.rows, n_heads, select)
+                self.bounds = [torch.zeros((pages, n_kv_heads, 2, head_dim), dtype=torch.bfloat16, device="cuda")
+                               for _ in range(layers * passes)]
+                self.selected = torch.empty((1, n_kv_heads, select), dtype=torch.int32, device="cuda")
+                self.select_ws = torch.empty((_d.select_workspace_bytes(self.kv[0], self.rows, n_heads, select),),
+                                             dtype=torch.uint8, device="cuda")
             self.attn_ws = torch.zeros((max(nws, 16),), dtype=torch.uint8, device="cuda")
         L = _q.lib()
         self.L = L
 
     def attend(self, l):
         """Slot l's attention: q and k of self.qkv rotated, k and v stored, the row's attention left in self.attn."""
-        for st in (_d.kv_append(self.kv[l], self.rows, self.k, self.v, q=self.q, q_out=self.q, rope_theta=self.rope_theta),
-                   _d.attention_paged(self.kv[l], self.rows, self.q, self.attn, window=self.window, sinks=self.sinks,
-                                      workspace=self.attn_ws)):
+        calls = [lambda: _d.kv_append(self.kv[l], self.rows, self.k, self.v, q=self.q, q_out=self.q, rope_theta=self.rope_theta)]
+        if self.select:
+            calls += [lambda: _d.kv_page_bounds(self.kv[l], self.rows, self.bounds[l]),
+                      lambda: _d.select_pages(self.kv[l], self.rows, self.q, self.bounds[l], self.selected, workspace=self.select_ws,
+                                              **self.keep),
+                      lambda: _d.attention_selected(self.kv[l], self.rows, self.q, self.selected, self.attn, workspace=self.attn_ws)]
+        else:
+            calls += [lambda: _d.attention_paged(self.kv[l], self.rows, self.q, self.attn, window=self.window, sinks=self.sinks,
+                                                 workspace=self.attn_ws)]
+        for call in calls:
+            st = call()
             if not st.ok():
                 raise RuntimeError(st.message)
 
