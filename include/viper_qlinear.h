@@ -631,8 +631,8 @@ int viper_hip_select_pages(const viper_kv_cache* cache, const viper_kv_batch* ba
 /* viper_hip_attention_paged over the tokens j <= p of the listed pages alone:
  * selected int32 [total_rows][kv_heads][count], a list for each row and key head, in
  * any order.  Entries that are negative or past p's page are none; a page listed
- * twice counts twice; a row whose list has no page is zero.  The rest, the
- * workspace's rules among it, is as there. */
+ * twice counts twice; a row whose list has no page is zero.  out overlaps neither
+ * q nor selected (refused).  The rest, the workspace's rules among it, is as there. */
 size_t viper_hip_attention_selected_workspace_bytes(const viper_kv_cache* cache, const viper_kv_batch* batch, int heads, int count);
 int viper_hip_attention_selected(const viper_kv_cache* cache, const viper_kv_batch* batch, const void* q_bf16, int64_t q_stride,
                                  int heads, float scale, const int32_t* selected, int count, void* out_bf16, int64_t out_stride,

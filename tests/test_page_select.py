@@ -48,18 +48,24 @@ def test_bounds_refusals(bad):
     assert calls(cache(), batch(), **bad)[0] == INVALID  # (FAKE: the cache's keys)
 
 
+def test_bounds_over_scales_are_refused():
+    assert calls(cache(kv_type=1, k_scales=2 * BIG + 16, v_scales=FAKE), batch())[0] == INVALID
+    assert calls(cache(kv_type=4, k_scales=2 * BIG + 16, v_scales=FAKE), batch())[0] == INVALID
+
+
 @pytest.mark.parametrize("bad", [dict(q=None), dict(q=FAKE + 2), dict(qs=2552), dict(qs=2564), dict(heads=0), dict(heads=18), dict(heads=-4),
                                  dict(heads=4 * 65, qs=4 * 65 * 128), dict(bounds=None), dict(bounds=2 * BIG + 2), dict(first=-1), dict(last=0),
                                  dict(last=-1), dict(first=15), dict(first=2 ** 31 - 1, last=2 ** 31 - 1), dict(count=0), dict(count=-1),
                                  dict(count=1 << 25), dict(sel=None), dict(sel=3 * BIG + 2), dict(ws=None), dict(ws=BIG + 4), dict(nws=16),
-                                 dict(sel=BIG), dict(sel=FAKE), dict(sel=2 * BIG), dict(ws=FAKE), dict(ws=2 * BIG)])
+                                 dict(sel=BIG), dict(sel=FAKE), dict(sel=2 * BIG), dict(ws=FAKE), dict(ws=2 * BIG), dict(qs=1 << 48), dict(qs=1 << 62)])
 def test_select_refusals(bad):
     assert calls(cache(), batch(), **bad)[1] == INVALID
 
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(q=FAKE + 2), dict(qs=2552), dict(heads=0), dict(heads=18), dict(out=None), dict(out=FAKE),
                                  dict(out=4 * BIG + 8), dict(os=100), dict(scale=0.0), dict(scale=float("nan")), dict(scale=float("inf")),
-                                 dict(count=0), dict(count=1 << 25), dict(sel=None), dict(sel=3 * BIG + 1), dict(ws=BIG + 8), dict(nws=16)])
+                                 dict(count=0), dict(count=1 << 25), dict(sel=None), dict(sel=3 * BIG + 1), dict(ws=BIG + 8), dict(nws=16),
+                                 dict(sel=4 * BIG), dict(sel=4 * BIG + 5000), dict(sel=4 * BIG - 8)])
 def test_attention_refusals(bad):
     # (two rows of 256 listed pages: a call that is split)
     assert calls(cache(), batch(), **{"count": 256, **bad})[2] == INVALID

@@ -287,7 +287,7 @@ __device__ __forceinline__ AttnShare attn_share(const AttnArgs& a, int W, int x,
                max(__builtin_amdgcn_readlane(most, 32), __builtin_amdgcn_readlane(most, 48)));
     const int held = (int)__popcll(__ballot(steps > 0)), room = max(1, a.splits - held / 2);
     int k = max(max((sum(steps) + room - 1) / room, (most + AT_PARTS - 1) / AT_PARTS), 1), parts, upto;
-    for (;; ++k) {  // (ends: with k = most each has one part, and there are at least as many as sequences)
+    for (;; k += 1 + k / 16) {  // (ends: with k >= most each has one part, and there are at least as many as sequences)
         parts = (steps + k - 1) / k;
         upto = (int)wave_upto((unsigned)parts);
         if (__builtin_amdgcn_readlane(upto, 63) <= a.splits) break;
@@ -357,8 +357,7 @@ __device__ __forceinline__ bool attn_store(const AttnArgs& a, const AttnSeq& s, 
     const int r = qg * ROWS + rr, i = (int)((unsigned)r * a.by_gqa >> 16), hh = r - i * a.gqa;
     o = o * (1.0f / l);  // (NaN where l is 0 or NaN)
     bool fine = !(l > 0.0f);
-    if (s.pos0 + i < 0) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (SEL && l == 0.0f && AttnList(a, (size_t)s.sq.row0, head, s.pos0).empty()) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (s.pos0 + i < 0 || (SEL && l == 0.0f && AttnList(a, (size_t)s.sq.row0, head, s.pos0).empty())) o = at_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     fine |= o[0] * 0.0f + o[1] * 0.0f + o[2] * 0.0f + o[3] * 0.0f == 0.0f;
     *(u32x2*)(a.out + (size_t)(s.sq.row0 + i) * a.out_stride + (size_t)(head * a.gqa + hh) * D + d) =
         u32x2{f2bf2(o[0], o[1]), f2bf2(o[2], o[3])};

@@ -101,6 +101,9 @@ static int attn_call(const viper_kv_cache* cache, const viper_kv_batch* batch, c
     if (batch->total_rows == 0) return VIPER_OK;
     // (rows may be read again after others are written)
     if (rows_meet(q_bf16, q_stride, width, out_bf16, out_stride, width, batch->total_rows)) return VIPER_INVALID_ARGUMENT;
+    if (sel != nullptr && ranges_meet(out_bf16, ((size_t)(batch->total_rows - 1) * out_stride + width) * 2, sel,
+                                      (size_t)batch->total_rows * cache->kv_heads * count * 4))
+        return VIPER_INVALID_ARGUMENT;
     AttnArgs a;
     a.c = kv_args(cache, batch);
     a.q = (const uint16_t*)q_bf16;

@@ -54,6 +54,11 @@ inline bool bad_rows(const void* p, int64_t stride, int64_t width) {
     return p == nullptr || misaligned(p, 16) || stride < width || stride % 8 != 0 || stride > (int64_t)1 << 40;
 }
 
+// Whether two ranges of bytes have one in common
+inline bool ranges_meet(const void* p, size_t n, const void* o, size_t m) {
+    return n != 0 && m != 0 && (uintptr_t)p < (uintptr_t)o + m && (uintptr_t)o < (uintptr_t)p + n;
+}
+
 // Whether two tensors of n rows (dense rows of pw and ow bf16 values, their strides
 // in elements) have a value in common, or reach further than any memory.  Columns of
 // one wider matrix have one stride and need no walk.

@@ -638,10 +638,6 @@ static const void* bounds_fn(int kv) {
 }
 
 static size_t bounds_bytes(const viper_kv_cache* c) { return (size_t)c->num_pages * c->kv_heads * c->head_dim * 4; }
-static bool ranges_meet(const void* p, size_t n, const void* o, size_t m) {
-    return n != 0 && m != 0 && (uintptr_t)p < (uintptr_t)o + m && (uintptr_t)o < (uintptr_t)p + n;
-}
-
 static int select_check(const viper_kv_cache* c, const viper_kv_batch* b, int heads, int count) {
     const int rc = kv_check(c, b);
     if (rc != VIPER_OK) return rc;
@@ -662,7 +658,11 @@ extern "C" int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper
     if (bounds_bf16 == nullptr || misaligned(bounds_bf16, 16)) return VIPER_INVALID_ARGUMENT;
     const size_t keys = bounds_bytes(cache) / 4 * cache->page_size * (cache->kv_type == VIPER_KV_BF16 ? 2 : 1) /
                         (cache->kv_type == VIPER_KV_FP4 ? 2 : 1);
-    if (ranges_meet(bounds_bf16, bounds_bytes(cache), cache->k, keys)) return VIPER_INVALID_ARGUMENT;
+    const size_t rows = (size_t)cache->num_pages * cache->kv_heads * cache->page_size;
+    const size_t scales = cache->kv_type == VIPER_KV_FP4 ? rows * (cache->head_dim / 32) : rows * 4;
+    if (ranges_meet(bounds_bf16, bounds_bytes(cache), cache->k, keys) ||
+        (cache->k_scales != nullptr && ranges_meet(bounds_bf16, bounds_bytes(cache), cache->k_scales, scales)))
+        return VIPER_INVALID_ARGUMENT;
     if (batch->total_rows == 0) return VIPER_OK;
     BoundsArgs a;
     a.c = kv_args(cache, batch);
@@ -697,6 +697,7 @@ extern "C" int viper_hip_select_pages(const viper_kv_cache* cache, const viper_k
     const size_t need = select_bytes(cache, batch);
     if (workspace == nullptr || misaligned(workspace, 16) || workspace_bytes < need) return VIPER_INVALID_ARGUMENT;
     if (batch->total_rows == 0) return VIPER_OK;
+    if (q_stride > ((int64_t)1 << 48) / batch->total_rows) return VIPER_INVALID_ARGUMENT;  // (further than any memory)
     const size_t n = (size_t)batch->total_rows, lists = n * cache->kv_heads * count * 4, rows = ((n - 1) * q_stride + width) * 2;
     if (ranges_meet(selected, lists, q_bf16, rows) || ranges_meet(selected, lists, bounds_bf16, bounds_bytes(cache)) ||
         ranges_meet(selected, lists, workspace, need) || ranges_meet(workspace, need, q_bf16, rows) ||

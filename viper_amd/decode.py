@@ -393,6 +393,8 @@ def _lists(cache, selected, rows):
     """The entries of each list of selected, None where it is not [rows, kv_heads, count]."""
     if selected.dim() != 3 or selected.shape[0] != rows or selected.shape[1] != cache.kv_heads or selected.shape[2] == 0:
         return None
+    if not _int32(selected.shape[2]):
+        raise ValueError("viper_amd: lists of 2^31 entries and more")
     return selected.shape[2]
 
 
