@@ -170,7 +170,7 @@ struct SelectArgs {
     uint32_t* keys;  // [batch * max_rows][key head][width]
     uint32_t* off;   // [batch * max_rows][key head][tiles]: how far the scores of 16 pages may be off (fp32 patterns)
     int gqa, count, first, last;
-    int cols, shift;  // columns of a row: its gqa queries, padded to 2^shift (to 5: a multiple of 16)
+    int cols, shift;  // a row's gqa queries, padded to 2^shift from 4 (shift 5: to a multiple of 16)
     int tiles;  // of 16 pages
 };
 
@@ -216,30 +216,23 @@ page_score_kernel(SelectArgs a) {
     const KvSeq s = kv_seq(a.c, b);
     const int64_t pos0 = (int64_t)s.len - s.n;
     if (s.n == 0 || tile * 16 >= ps_pages(a.c, (int64_t)s.len - 1)) return;
-    // the rows' queries are the columns, 16 at a time; of a row of more than 16 the running maximum is kept
-    const int shift = a.shift, per = min(a.cols, 16), turns = (s.n * a.cols + 15) / 16;
-    auto column = [&](int turn, int& r, int& h) {
-        if (shift <= 4) {
-            r = (turn * 16 + m) >> shift;
-            h = (turn * 16 + m) & (a.cols - 1);
-        } else {  // (turns of one row)
-            r = turn / (a.cols / 16);
-            h = (turn - r * (a.cols / 16)) * 16 + m;
-        }
+    // a row's queries, padded with its last one, are the rows of the products, 16 to a turn
+    const int shift = a.shift, turns = (s.n * a.cols + 15) / 16;
+    auto row_of = [&](int turn, int i, int& column) {
+        const int r = shift <= 4 ? (turn * 16 + i) >> shift : turn / (a.cols / 16);
+        column = turn * 16 + i - r * a.cols;
+        return r;
     };
     u32x4 q[NKB], lo[NKB], hi[NKB];
-    bool in = false;
     auto load_q = [&](int turn) {
-        int r, h;
-        column(turn, r, h);
-        in = r < s.n && h < a.gqa;
-        const uint16_t* const at = a.q + (size_t)(s.row0 + (in ? r : 0)) * a.q_stride + (size_t)(head * a.gqa + (in ? h : 0)) * D + 8 * g;
+        int h;
+        const int r = min(row_of(turn, m, h), s.n - 1);
+        const uint16_t* const at = a.q + (size_t)(s.row0 + r) * a.q_stride + (size_t)(head * a.gqa + min(h, a.gqa - 1)) * D + 8 * g;
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) q[kb] = *(const u32x4*)(at + 32 * kb);
     };
     load_q(0);
     const bool there = (unsigned)entry < (unsigned)a.c.pages;
-    const uint32_t present = (uint32_t)__ballot(there);
     {
         const uint16_t* const at = a.bounds + ((size_t)(there ? entry : 0) * a.c.kvh + head) * (2 * D) + 8 * g;
 #pragma unroll
@@ -250,7 +243,7 @@ page_score_kernel(SelectArgs a) {
     }
     constexpr uint32_t LEAST = 0x0d800d80u;  // 2^-100
     auto of = [](const u32x4& v) { return __builtin_bit_cast(ps_bf16x8, v); };
-    ps_f32x4 best;
+    float best = 0.0f;
     uint32_t off = 0;
     for (int turn = 0; turn < turns; ++turn) {
         const ps_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -265,47 +258,49 @@ page_score_kernel(SelectArgs a) {
                 mag[i] = pb_max(q[kb][i] & 0x7fff7fffu, LEAST);
                 most[i] = pb_max(pb_max(lo[kb][i] & 0x7fff7fffu, hi[kb][i] & 0x7fff7fffu), LEAST);
             }
-            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(hi[kb]), of(up), zero, 0, 0, 0);
-            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(lo[kb]), of(dn), zero, 0, 0, 0);
-            Q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(most), of(mag), Q, 0, 0, 0);
+            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(up), of(hi[kb]), zero, 0, 0, 0);
+            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(dn), of(lo[kb]), zero, 0, 0, 0);
+            Q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(mag), of(most), Q, 0, 0, 0);
         }
-        const bool was = in;
-        int r, h;
-        column(turn, r, h);
         if (turn + 1 < turns) load_q(turn + 1);
-        const bool begins = shift <= 4 || h < 16, ends = shift <= 4 || h + 16 - m >= a.cols;
-        // over the columns of a row.  A score that is no number has a Q that is not finite, and
-        // as patterns NaN and infinity are the largest of these: pages in 64 bits then.
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v = was ? S[i] : -__builtin_inff();
-            if (per >= 2) v = fmaxf(v, dpp_f<DPP_SWAP1>(v));
-            if (per >= 4) v = fmaxf(v, dpp_f<DPP_SWAP2>(v));
-            if (per >= 8) v = fmaxf(v, dpp_f<DPP_HALF_MIRROR>(v));
-            if (per >= 16) v = fmaxf(v, dpp_f<DPP_MIRROR>(v));
-            best[i] = begins ? v : fmaxf(best[i], v);
-        }
+        // The lane's four queries are of one row, whose others lie 16 and 32 lanes further and in
+        // further turns.  A score that is no number has a Q that is not finite, and as
+        // patterns NaN and infinity are the largest of these: pages in 64 bits then.
+        float v = fmaxf(fmaxf(S[0], S[1]), fmaxf(S[2], S[3]));
         uint32_t e = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e = max(e, (present >> (4 * g + i)) & 1u ? __float_as_uint(Q[i]) & 0x7fffffffu : 0u);
-        e = was ? e : 0u;
-        if (per >= 2) e = max(e, (uint32_t)dpp_i<DPP_SWAP1>((int)e));
-        if (per >= 4) e = max(e, (uint32_t)dpp_i<DPP_SWAP2>((int)e));
-        if (per >= 8) e = max(e, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)e));
-        if (per >= 16) e = max(e, (uint32_t)dpp_i<DPP_MIRROR>((int)e));
-        auto w = __builtin_amdgcn_permlane16_swap(e, e, false, false);
-        e = max(w[0], w[1]);
-        w = __builtin_amdgcn_permlane32_swap(e, e, false, false);
-        e = max(w[0], w[1]);
-        off = begins ? e : max(off, e);
-        const int p = tile * 16 + 4 * g, pages = ps_pages(a.c, pos0 + r);
-        if (!ends || m % per != 0 || r >= s.n || p >= pages) continue;
+        for (int i = 0; i < 4; ++i) e = max(e, __float_as_uint(Q[i]) & 0x7fffffffu);
+        if (shift >= 3) {
+            auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+            w = __builtin_amdgcn_permlane16_swap(e, e, false, false);
+            e = max(w[0], w[1]);
+        }
+        if (shift >= 4) {
+            auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+            v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+            w = __builtin_amdgcn_permlane32_swap(e, e, false, false);
+            e = max(w[0], w[1]);
+        }
+        int column;
+        const int r = row_of(turn, 4 * g, column);
+        if (shift > 4 && column >= 16) {
+            v = fmaxf(v, best);
+            e = max(e, off);
+        }
+        best = v;
+        off = e;
+        e = there ? e : 0u;  // over the tile's pages
+        e = max(e, (uint32_t)dpp_i<DPP_SWAP1>((int)e));
+        e = max(e, (uint32_t)dpp_i<DPP_SWAP2>((int)e));
+        e = max(e, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)e));
+        e = max(e, (uint32_t)dpp_i<DPP_MIRROR>((int)e));
+        const int p = tile * 16 + m, pages = ps_pages(a.c, pos0 + r);
+        const bool writes = shift <= 4 ? column == 0 : column == a.cols - 16;
+        if (!writes || r >= s.n || tile * 16 >= pages) continue;
         const size_t row = ps_row(a, b, r, head);
-        uint32_t* const keys = a.keys + row * a.c.width + p;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p + i < pages) keys[i] = (present >> (4 * g + i)) & 1u ? ps_key(best[i]) : 0u;
-        if (g == 0) a.off[row * a.tiles + tile] = __float_as_uint(__uint_as_float(off) * PS_OFF + PS_OFF_MIN);
+        if (p < pages) a.keys[row * a.c.width + p] = there ? ps_key(v) : 0u;
+        if (m == 0) a.off[row * a.tiles + tile] = __float_as_uint(__uint_as_float(e) * PS_OFF + PS_OFF_MIN);
     }
 }
 
@@ -716,7 +711,7 @@ extern "C" int viper_hip_select_pages(const viper_kv_cache* cache, const viper_k
     a.count = count;
     a.first = first;
     a.last = last;
-    a.shift = 0;
+    a.shift = 2;
     while (a.shift <= 4 && 1 << a.shift < a.gqa) ++a.shift;
     a.cols = a.shift <= 4 ? 1 << a.shift : (a.gqa + 15) / 16 * 16;
     int d = D;
