@@ -203,11 +203,17 @@ typedef __bf16 ps_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float ps_f32x4 __attribute__((ext_vector_type(4)));
 constexpr int PS_NT = 256;
 
-// A wave takes 16 pages and all rows of its sequence.
+// A wave takes 16 pages and all rows of its sequence.  Bounds are read in whole rows of
+// 4 D bytes and turned in LDS, its 16 bytes in an order by page that spreads the banks (operands
+// loaded as they are, 64 bytes of 16 pages at a time, take 2.4 us longer over 38 MB), and
+// queries are read once for the four waves.
 template <int D>
 __global__ void __launch_bounds__(PS_NT)
 page_score_kernel(SelectArgs a) {
-    constexpr int NKB = D / 32;
+    constexpr int NKB = D / 32, PC = D / 4, QC = D / 8, NL = 16 * PC / 64, QX = QC < 16 ? QC - 1 : 15;  // PC, QC: 16 bytes of a page, a query
+    constexpr int NQ = 16 * QC < PS_NT ? 1 : 16 * QC / PS_NT;
+    __shared__ u32x4 lb[PS_NT / 64][16 * PC];
+    __shared__ u32x4 lq[2][16 * QC];
     const int tid = (int)threadIdx.x, lane = tid & 63, m = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int chunk = (int)blockIdx.x / a.c.kvh, head = (int)blockIdx.x - chunk * a.c.kvh, b = (int)blockIdx.z;
@@ -215,92 +221,130 @@ page_score_kernel(SelectArgs a) {
     const int entry = tile * 16 + m < a.c.width ? a.c.table[(size_t)b * a.c.width + tile * 16 + m] : -1;
     const KvSeq s = kv_seq(a.c, b);
     const int64_t pos0 = (int64_t)s.len - s.n;
-    if (s.n == 0 || tile * 16 >= ps_pages(a.c, (int64_t)s.len - 1)) return;
+    const int last = s.n == 0 ? 0 : ps_pages(a.c, (int64_t)s.len - 1);
+    if (chunk * (PS_NT / 64) * 16 >= last) return;
+    const bool live = tile * 16 < last;
     // a row's queries, padded with its last one, are the rows of the products, 16 to a turn
-    const int shift = a.shift, turns = (s.n * a.cols + 15) / 16;
-    auto row_of = [&](int turn, int i, int& column) {
-        const int r = shift <= 4 ? (turn * 16 + i) >> shift : turn / (a.cols / 16);
-        column = turn * 16 + i - r * a.cols;
-        return r;
+    const int shift = min(a.shift, 4), per = 1 << shift;
+    int r0 = 0, h0 = 0;  // of a turn: query i is head h0 + i % per of row r0 + i / per
+    auto advance = [&] {
+        h0 += 16;
+        if (h0 < a.cols) return;
+        h0 = 0;
+        r0 += 16 >> shift;
     };
-    u32x4 q[NKB], lo[NKB], hi[NKB];
-    auto load_q = [&](int turn) {
-        int h;
-        const int r = min(row_of(turn, m, h), s.n - 1);
-        const uint16_t* const at = a.q + (size_t)(s.row0 + r) * a.q_stride + (size_t)(head * a.gqa + min(h, a.gqa - 1)) * D + 8 * g;
+    u32x4 next[NQ];
+    auto load_q = [&] {
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) q[kb] = *(const u32x4*)(at + 32 * kb);
+        for (int i = 0; i < NQ; ++i) {
+            const int at = tid + i * PS_NT;
+            if (16 * QC < PS_NT && at >= 16 * QC) continue;
+            const int r = min(r0 + (at / QC >> shift), s.n - 1), h = min(h0 + (at / QC & (per - 1)), a.gqa - 1);
+            next[i] = *(const u32x4*)(a.q + (size_t)(s.row0 + r) * a.q_stride + (head * a.gqa + h) * D + 8 * (at % QC));
+        }
     };
-    load_q(0);
+    auto store_q = [&](u32x4* to) {
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) {
+            const int at = tid + i * PS_NT, n = at / QC;
+            if (16 * QC < PS_NT && at >= 16 * QC) continue;
+            to[n * QC + (at % QC ^ (n & QX))] = next[i];
+        }
+    };
+    load_q();
     const bool there = (unsigned)entry < (unsigned)a.c.pages;
-    {
-        const uint16_t* const at = a.bounds + ((size_t)(there ? entry : 0) * a.c.kvh + head) * (2 * D) + 8 * g;
+    u32x4 lo[NKB], hi[NKB], rows[NL];
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int n = (i * 64 + lane) / PC, c = (i * 64 + lane) % PC;
+            const int e = __shfl(there ? entry : 0, n);
+            rows[i] = *(const u32x4*)(a.bounds + ((size_t)e * a.c.kvh + head) * (2 * D) + 8 * c);
+        }
+    }
+    store_q(lq[0]);
+    __syncthreads();
+    if (live) {
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int n = (i * 64 + lane) / PC, c = (i * 64 + lane) % PC;
+            lb[wave][n * PC + (c ^ n)] = rows[i];
+        }
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int kb = 0; kb < NKB; ++kb) {
-            lo[kb] = *(const u32x4*)(at + 32 * kb);
-            hi[kb] = *(const u32x4*)(at + D + 32 * kb);
+            lo[kb] = lb[wave][m * PC + ((4 * kb + g) ^ m)];
+            hi[kb] = lb[wave][m * PC + ((QC + 4 * kb + g) ^ m)];
         }
     }
     constexpr uint32_t LEAST = 0x0d800d80u;  // 2^-100
     auto of = [](const u32x4& v) { return __builtin_bit_cast(ps_bf16x8, v); };
     float best = 0.0f;
     uint32_t off = 0;
-    for (int turn = 0; turn < turns; ++turn) {
-        const ps_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        ps_f32x4 S = zero, Q = zero;
+#pragma unroll 1
+    for (int turn = 0;; turn ^= 1) {
+        const int r = r0 + (4 * g >> shift), h = h0 + (4 * g & (per - 1));
+        advance();
+        const bool more = r0 < s.n;
+        if (more) load_q();
+        if (live) {
+            const ps_f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+            ps_f32x4 S = zero, Q = zero;
 #pragma unroll
-        for (int kb = 0; kb < NKB; ++kb) {
-            u32x4 up, dn, mag, most;  // most: the larger magnitude of either bound
+            for (int kb = 0; kb < NKB; ++kb) {
+                const u32x4 q = lq[turn][m * QC + ((4 * kb + g) ^ (m & QX))];
+                u32x4 up, dn, mag, most;  // most: the larger magnitude of either bound
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // (as integers, values with a sign are under 0)
-                up[i] = pb_max(q[kb][i], 0u);
-                dn[i] = pb_min(q[kb][i], 0u);
-                mag[i] = pb_max(q[kb][i] & 0x7fff7fffu, LEAST);
-                most[i] = pb_max(pb_max(lo[kb][i] & 0x7fff7fffu, hi[kb][i] & 0x7fff7fffu), LEAST);
+                for (int i = 0; i < 4; ++i) {  // (as integers, values with a sign are under 0)
+                    up[i] = pb_max(q[i], 0u);
+                    dn[i] = pb_min(q[i], 0u);
+                    mag[i] = pb_max(q[i] & 0x7fff7fffu, LEAST);
+                    most[i] = pb_max(pb_max(lo[kb][i] & 0x7fff7fffu, hi[kb][i] & 0x7fff7fffu), LEAST);
+                }
+                S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(up), of(hi[kb]), zero, 0, 0, 0);
+                S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(dn), of(lo[kb]), zero, 0, 0, 0);
+                Q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(mag), of(most), Q, 0, 0, 0);
             }
-            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(up), of(hi[kb]), zero, 0, 0, 0);
-            S += __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(dn), of(lo[kb]), zero, 0, 0, 0);
-            Q = __builtin_amdgcn_mfma_f32_16x16x32_bf16(of(mag), of(most), Q, 0, 0, 0);
-        }
-        if (turn + 1 < turns) load_q(turn + 1);
-        // The lane's four queries are of one row, whose others lie 16 and 32 lanes further and in
-        // further turns.  A score that is no number has a Q that is not finite, and as
-        // patterns NaN and infinity are the largest of these: pages in 64 bits then.
-        float v = fmaxf(fmaxf(S[0], S[1]), fmaxf(S[2], S[3]));
-        uint32_t e = 0;
+            // The lane's four queries are of one row, whose others lie 16 and 32 lanes further and in
+            // further turns.  A score that is no number has a Q that is not finite, and as
+            // patterns NaN and infinity are the largest of these: pages in 64 bits then.
+            float v = fmaxf(fmaxf(S[0], S[1]), fmaxf(S[2], S[3]));
+            uint32_t e = 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) e = max(e, __float_as_uint(Q[i]) & 0x7fffffffu);
-        if (shift >= 3) {
-            auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-            v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
-            w = __builtin_amdgcn_permlane16_swap(e, e, false, false);
-            e = max(w[0], w[1]);
+            for (int i = 0; i < 4; ++i) e = max(e, __float_as_uint(Q[i]) & 0x7fffffffu);
+            if (shift >= 3) {
+                auto w = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+                v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+                w = __builtin_amdgcn_permlane16_swap(e, e, false, false);
+                e = max(w[0], w[1]);
+            }
+            if (shift >= 4) {
+                auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+                v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+                w = __builtin_amdgcn_permlane32_swap(e, e, false, false);
+                e = max(w[0], w[1]);
+            }
+            if (h >= 16) {
+                v = fmaxf(v, best);
+                e = max(e, off);
+            }
+            best = v;
+            off = e;
+            e = there ? e : 0u;  // over the tile's pages
+            e = max(e, (uint32_t)dpp_i<DPP_SWAP1>((int)e));
+            e = max(e, (uint32_t)dpp_i<DPP_SWAP2>((int)e));
+            e = max(e, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)e));
+            e = max(e, (uint32_t)dpp_i<DPP_MIRROR>((int)e));
+            const int p = tile * 16 + m, pages = ps_pages(a.c, pos0 + r);
+            if ((h & 15) == 0 && (h + 16 >= a.cols) && r < s.n && tile * 16 < pages) {
+                const size_t row = ps_row(a, b, r, head);
+                if (p < pages) a.keys[row * a.c.width + p] = there ? ps_key(v) : 0u;
+                if (m == 0) a.off[row * a.tiles + tile] = __float_as_uint(__uint_as_float(e) * PS_OFF + PS_OFF_MIN);
+            }
         }
-        if (shift >= 4) {
-            auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-            v = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
-            w = __builtin_amdgcn_permlane32_swap(e, e, false, false);
-            e = max(w[0], w[1]);
-        }
-        int column;
-        const int r = row_of(turn, 4 * g, column);
-        if (shift > 4 && column >= 16) {
-            v = fmaxf(v, best);
-            e = max(e, off);
-        }
-        best = v;
-        off = e;
-        e = there ? e : 0u;  // over the tile's pages
-        e = max(e, (uint32_t)dpp_i<DPP_SWAP1>((int)e));
-        e = max(e, (uint32_t)dpp_i<DPP_SWAP2>((int)e));
-        e = max(e, (uint32_t)dpp_i<DPP_HALF_MIRROR>((int)e));
-        e = max(e, (uint32_t)dpp_i<DPP_MIRROR>((int)e));
-        const int p = tile * 16 + m, pages = ps_pages(a.c, pos0 + r);
-        const bool writes = shift <= 4 ? column == 0 : column == a.cols - 16;
-        if (!writes || r >= s.n || tile * 16 >= pages) continue;
-        const size_t row = ps_row(a, b, r, head);
-        if (p < pages) a.keys[row * a.c.width + p] = there ? ps_key(v) : 0u;
-        if (m == 0) a.off[row * a.tiles + tile] = __float_as_uint(__uint_as_float(e) * PS_OFF + PS_OFF_MIN);
+        if (!more) break;
+        store_q(lq[turn ^ 1]);
+        __syncthreads();
     }
 }
 
