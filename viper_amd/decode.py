@@ -90,6 +90,7 @@ class KVCache(_Fixed):
         self._dev = self.k.get_device()
         self._width = self.kv_heads * self.head_dim
         self._scale = 1.0 / math.sqrt(self.head_dim)
+        self._bounds = (self.num_pages, self.kv_heads, 2, self.head_dim)
         self._ref = C.addressof(self._c)
 
     @classmethod
@@ -340,7 +341,7 @@ def kv_page_bounds(cache: KVCache, batch: KVBatch, bounds, stream=None) -> Statu
     [num_pages, kv_heads, 2, head_dim]); other pages' are left as they were.  After kv_append of a batch (total_rows known)."""
     what = "viper_hip_kv_page_bounds"
     dev = cache._dev
-    if not _laid(bounds, (cache.num_pages, cache.kv_heads, 2, cache.head_dim)):
+    if bounds.shape != cache._bounds and not _laid(bounds, cache._bounds):
         return _mismatch(what, "bounds is [num_pages, kv_heads, 2, head_dim]")
     if batch.total_rows is None and batch.row_offsets is not None:
         ref = batch._rows(min(batch.batch * batch.max_rows, (1 << 31) - 1), dev)  # (an upper limit: offsets past it do not fit)
@@ -378,7 +379,7 @@ def select_pages(cache: KVCache, batch: KVBatch, q, bounds, selected, first: int
     if ref is None:
         return _mismatch(what, "the rows do not match the batch")
     count = _lists(cache, selected, rows)
-    if count is None or not _laid(bounds, (cache.num_pages, cache.kv_heads, 2, cache.head_dim)):
+    if count is None or (bounds.shape != cache._bounds and not _laid(bounds, cache._bounds)):
         return _mismatch(what, "selected is [rows, kv_heads, count], bounds [num_pages, kv_heads, 2, head_dim]")
     if not (_int32(first) and _int32(last)):
         return Status(StatusCode.INVALID_ARGUMENT, f"{what}: first and last are 32-bit")
