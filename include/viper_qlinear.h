@@ -617,7 +617,8 @@ int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper_kv_batch* 
  * (>= first + last) are.  A page's score bounds scale * q . k from above, for
  * every scale: max over the heads' q of sum_d max(q_d lo_d, q_d hi_d), summed in
  * 64 bits and rounded to fp32, NaN as +inf; pages that the table lacks have none and
- * are listed only among the first and last.  Rows at negative positions list none;
+ * are listed only among the first and last.  Bounds are as kv_page_bounds leaves
+ * them: lo <= hi, or both NaN.  Rows at negative positions list none;
  * pages past the table are not considered.  max_rows <= VIPER_QLINEAR_MAX_M, heads
  * as for viper_hip_attention_paged, count * page_size < 2^31, batch kv_heads
  * ceil(table_width / 64) < 2^24.  selected and workspace (16-byte

@@ -27,7 +27,12 @@
 // contexts (int8 at 5.3 TB/s: 395 VALU instructions a tile to widen codes against 165;
 // sequences of uneven lengths by the longest one's parts), by the latency of one load
 // chain and of the join at short ones and in 16 rows (where MFMA and softmax issue 6 of
-// the 14.4 us).
+// the 14.4 us).  FP4: 611 tokens 5.9 us, 131072 17.6 (71.3 MB, 10.6 us at 6.7 TB/s; a
+// kernel of 14.6 and a join), 32 sequences of 700 to 16384 35 (with parts of equal numbers for
+// all 43), 7 rows of 48 heads over 8 of 64 dims, 4 sequences of 2003 to 9001, 19: tiles of 4 KB in chains of table, page and
+// tile, with 4 KB to a wave in flight, spend 45 % of the waves' time on memory.  Lists of 64
+// pages of 64 tokens in bf16 8.3, of 128 pages of 32 for 64 rows in FP4 25.6 (3.6 TB/s: 8
+// tiles to a wave).
 //
 // What a row must not see cannot reach it: masked scores are replaced (not
 // added to), places of the last tile past the length are cleared in V.  So a row's
@@ -260,7 +265,8 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, si
 // unequal lengths leave most workgroups waiting for the longest sequence's, so with `share`
 // a sequence has as many as its length asks for: the least number of steps (a tile to
 // every wave) to a part with which all parts of all sequences (up to 64, a lane to each)
-// run at once.
+// run at once (FP4, 32 sequences of 700 to 16384 tokens 43 us, so 35; twice or four times
+// the parts 41 and 47).
 struct AttnShare {
     int b, split, splits, first;  // first: the sequence's part 0 among all of them
 };

@@ -17,7 +17,7 @@
 // with 2-byte stores (1-byte for int8), since 8 tokens of a dim share 16 bytes.
 // Bound by latency at a decode step's sizes (one row of 20 + 4 + 4 heads of 128: 2.7
 // us, of which 1.5 are the dispatch), by the small V stores at a batch's (512 rows of
-// 64 sequences into int8 5.9 us).
+// 64 sequences into int8 5.9 us).  FP4 caches have a kernel of their own (kv_append4_kernel).
 
 #include "kv_host.h"
 

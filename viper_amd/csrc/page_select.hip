@@ -6,8 +6,13 @@
 //
 // selection: q . k of any key of a page is at most sum_d max(q_d lo_d, q_d hi_d), the page's
 // score for a query head; the largest over the heads of a key head counts.  A page at the
-// border is in or out, so products (exact in 32 bits) are summed in 64.  Scores become
-// integers in their order; the smallest that is in is found bit by bit, by counting.
+// border is in or out, so a score is that of the sum in 64 bits.  One launch has all scores
+// as matrix products in 32 bits, with a limit to how far they may be off; a second finds the
+// border among them and computes in 64 bits only the pages too near to it.
+//
+// Measured (20 heads over 4 key heads of 128 dims): 64 of 2048 pages for one row 8.6 us
+// (scores 4.4, selection 5.2: latency); 128 of up to 2032 for 4 rows of 16 sequences 21.2
+// (13.0 and 8.4; 38 MB of bounds, 5.7 us at 6.7 TB/s); all scores in 64 bits took 48.
 
 #include "kv_host.h"
 
@@ -41,7 +46,9 @@ constexpr int DPP_ROR8 = 0x128;  // lane i <- i ^ 8 within 16
 // meet in LDS) with the tile's 16-byte loads.  The least and, complemented, the largest of a
 // lane's token are R registers; each step of the way over the 16 lanes of other tokens
 // halves them, a lane keeping the half that one bit of its number says.  3 prompts of
-// 20000 tokens in pages of 32, int8: 4 pages to a workgroup of one wave for each 32 dims took 11.5 us.
+// 20000 tokens in pages of 32, int8, take 9.1 us (16.5 MB, 2.5 us at 6.7 TB/s: 400 VALU
+// instructions a wave are 5 us of issue), one decode row of 16 sequences 3.3; 4 pages to a workgroup of one wave for
+// each 32 dims took 11.5.
 template <int D, int KT>
 __global__ void __launch_bounds__(PB_NT)
 page_bounds_kernel(BoundsArgs a) {
@@ -203,10 +210,14 @@ typedef __bf16 ps_bf16x8 __attribute__((ext_vector_type(8)));
 typedef float ps_f32x4 __attribute__((ext_vector_type(4)));
 constexpr int PS_NT = 256;
 
-// A wave takes 16 pages and all rows of its sequence.  Bounds are read in whole rows of
-// 4 D bytes and turned in LDS, its 16 bytes in an order by page that spreads the banks (operands
-// loaded as they are, 64 bytes of 16 pages at a time, take 2.4 us longer over 38 MB), and
-// queries are read once for the four waves.
+// A wave takes 16 pages and all rows of its sequence.  Queries are the rows of the products, so
+// that the heads of a row meet in a lane's registers (as columns 2.5 us longer in the batch above).
+// Bounds are read in whole rows of 4 D bytes and turned in LDS, its 16 bytes in an order by
+// page that spreads the banks (operands loaded as they are, 64 bytes of 16 pages at a time, take
+// 2.4 us longer over 38 MB), and queries are read once for the four waves.  Of the batch's 13
+// us 2.3 are an empty dispatch, 5.5 the loads and 5 the products' and sums' issue, which few
+// loads cover, as all waves start together (two tiles to a wave, or fewer waves that go on to
+// further tiles, were no faster).
 template <int D>
 __global__ void __launch_bounds__(PS_NT)
 page_score_kernel(SelectArgs a) {

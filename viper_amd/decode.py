@@ -10,6 +10,12 @@ no call could take raise ``ValueError``.
     ws = torch.zeros(attention_workspace_bytes(cache, batch, heads), dtype=torch.uint8, device="cuda")
     kv_append(cache, batch, k, v, q=q, q_out=q, rope_theta=1e6)
     attention_paged(cache, batch, q, out, workspace=ws)
+
+Over long contexts a row may look at some pages of each sequence alone, those whose keys promise the largest scores:
+
+    kv_page_bounds(cache, batch, bounds)                     # after each kv_append: bf16 [num_pages, kv_heads, 2, head_dim]
+    select_pages(cache, batch, q, bounds, selected, workspace=select_ws)  # int32 [rows, kv_heads, count]
+    attention_selected(cache, batch, q, selected, out, workspace=selected_ws)
 """
 from __future__ import annotations
 
