@@ -202,3 +202,33 @@ def test_as_many_pages_as_a_workgroup_holds_and_one_more(n):
             for r in range(2):
                 x = R.bf16_val(q[r]).astype(np.float64).reshape(heads, D)
                 assert back(sel)[r, 0].tolist() == P.select(x, f, table[0], n, page, length - 2 + r, 1, 2, count), (length, count, r)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5, 8, 9, 16, 17, 32, 33, 40, 64])
+def test_every_head_of_a_key_head_counts(D, G):
+    """Rows of up to 64 heads to a key head (queries of several turns of 16, padded or not): each head alone decides about pages of its own."""
+    page, kvh, n, rows = 32, 2, 70, [16, 0, 5, 1]
+    rng = np.random.default_rng(D + G)
+    lens = [n * page - 3, 40, 33 * page, 17 * page + 1]
+    table = np.stack([rng.permutation(n) for _ in lens]).astype(np.int32)
+    near = np.sort(rng.standard_normal((n, kvh, 2, D)), 2)
+    q = 0.05 * rng.standard_normal((sum(rows), kvh, G, D))
+    for i in range(sum(rows)):  # the head that looks along the page's own dimension
+        h = i % G
+        q[i, :, h, (7 * h) % D] = 4.0
+        q[i, 1, (h + G // 2) % G, (11 * h + 3) % D] = -3.0
+    near, q = R.bf16_bits(near), R.bf16_bits(q.reshape(sum(rows), kvh * G * D))
+    offs = offsets(rows)
+    g = va.KVCache.empty(va.KVType.BF16, n, page, kvh, D)
+    batch = va.KVBatch(dev(table), dev(np.array(lens, np.int32)), 16, dev(offs), sum(rows))
+    f = R.bf16_val(near).astype(np.float64)
+    count = 12
+    sel = dev(np.zeros((sum(rows), kvh, count), np.int32))
+    ws = ws_of(va.select_workspace_bytes(g, batch, kvh * G, count))
+    assert va.select_pages(g, batch, dev(q), dev(near), sel, first=1, last=2, workspace=ws).ok()
+    got = back(sel)
+    for b, r, p in R.row_map(lens, 16, offs):
+        x = R.bf16_val(q[r]).astype(np.float64).reshape(kvh, G, D)
+        for h in range(kvh):
+            assert got[r, h].tolist() == P.select(x[h], f[:, h], table[b], n, page, p, 1, 2, count), (b, r, p, h)
