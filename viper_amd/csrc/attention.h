@@ -31,8 +31,8 @@
 // kernel of 14.6 and a join), 32 sequences of 700 to 16384 35 (with parts of equal numbers for
 // all 43), 7 rows of 48 heads over 8 of 64 dims, 4 sequences of 2003 to 9001, 19: tiles of 4 KB in chains of table, page and
 // tile, with 4 KB to a wave in flight, spend 45 % of the waves' time on memory.  Lists of 64
-// pages of 64 tokens in bf16 8.3, of 128 pages of 32 for 64 rows in FP4 25.6 (3.6 TB/s: 8
-// tiles to a wave).
+// pages of 64 tokens in bf16 8.3, of 128 pages of 32 for 41 rows in FP4 24.6 (91 MB;
+// twice the pages 41, 5.8 TB/s; two to six parts to a row make no difference).
 //
 // What a row must not see cannot reach it: masked scores are replaced (not
 // added to), places of the last tile past the length are cleared in V.  So a row's
@@ -173,13 +173,13 @@ __device__ __forceinline__ void row_again(const AttnArgs& a, int b, int head, si
     constexpr int TILES = NT / KV_TILE, G = NT / D;  // tiles of a chunk of tokens; groups of threads over its octets
     constexpr bool I8 = KT == VIPER_KV_INT8, F4 = KT == VIPER_KV_FP4;
     const int tid = (int)threadIdx.x;
-    const Sight sight{a.window, a.sinks};
+    const Sight sight{SEL ? 0 : a.window, SEL ? 0 : a.sinks};
     const int64_t cap = ((int64_t)a.c.width << a.c.tpl) * KV_TILE;
     float* w = lds;                // [NT] weights of a chunk of tokens, -1: not seen
     float* acc = w + NT;           // [NT]
     int* pages = (int*)(acc + NT);  // [TILES]
     // chunks between the first tokens and the window are skipped
-    auto between = [&](int64_t j0, int n) { return a.window != 0 && j0 >= a.sinks && j0 + n - 1 <= (int64_t)p - a.window; };
+    auto between = [&](int64_t j0, int n) { return !SEL && a.window != 0 && j0 >= a.sinks && j0 + n - 1 <= (int64_t)p - a.window; };
     // tokens are walked in order, or (SEL) in the list's, where number j lies in tile turned(j / 32)
     const AttnList list(a, row, head, p);
     auto turned = [&](int64_t vt) { return SEL ? list.tile_at((int)vt) : (int)vt; };
@@ -339,7 +339,7 @@ __device__ __forceinline__ AttnSeq attn_seq(const AttnArgs& a, KvSeq sq, int qg,
     s.pos0 = s.len - sq.n;
     // the tiles that some row sees: those of the first tokens, then the window's
     s.lo_t = s.nsink = 0;
-    if (a.window != 0) {
+    if (!SEL && a.window != 0) {
         const int from = max(0, s.pos0 + 1 > a.window ? s.pos0 + 1 - a.window : 0);
         // (a length past the table has no more tiles than it)
         s.nsink = (min(min(a.sinks, from), cap) + KV_TILE - 1) / KV_TILE;
@@ -603,7 +603,7 @@ attn_kernel(AttnArgs a) {
             load_k(next);
             const int j0 = tile * KV_TILE, jl = j0 + 8 * g;
             const bool whole = (!SEL || tile >= 0) && j0 + KV_TILE - 1 <= pos0 &&
-                               (a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
+                               (SEL || a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
             at_bf16x8 ph[QT], pl[QT];
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
@@ -614,7 +614,7 @@ attn_kernel(AttnArgs a) {
                     vs[e] = __uint_as_float(vsc[e >> 2][e & 3]);
                 }
                 if (!whole) {
-                    const Sight sight{a.window, a.sinks};
+                    const Sight sight{SEL ? 0 : a.window, SEL ? 0 : a.sinks};
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const bool in = (!SEL || tile >= 0) && sight.sees(jl + e, pos[qt]);
@@ -775,7 +775,7 @@ attn_kernel(AttnArgs a) {
             // scores, by token of the lane's eight; tiles that some row does not see whole are masked
             const int j0 = tile * KV_TILE, jl = j0 + 8 * g;
             const bool whole = (!SEL || tile >= 0) && j0 + KV_TILE - 1 <= pos0 &&
-                               (a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
+                               (SEL || a.window == 0 || j0 > len - 1 - a.window || j0 + KV_TILE <= a.sinks);
             at_bf16x8 ph[QT], pl[QT];
 #pragma unroll
             for (int qt = 0; qt < QT; ++qt) {
@@ -786,7 +786,7 @@ attn_kernel(AttnArgs a) {
                 }
                 uint32_t seen = 0xffu;
                 if (!whole) {
-                    const Sight sight{a.window, a.sinks};
+                    const Sight sight{SEL ? 0 : a.window, SEL ? 0 : a.sinks};
                     seen = 0;
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
@@ -821,12 +821,13 @@ attn_kernel(AttnArgs a) {
                 ph[qt] = __builtin_bit_cast(at_bf16x8, h);
                 pl[qt] = __builtin_bit_cast(at_bf16x8, r);
             }
-            if (!I8 && (j0 + KV_TILE > len || (SEL && tile < 0))) {  // places past the length hold anything
+            const int upto = SEL && tile < 0 ? INT32_MIN : len;
+            if (!I8 && j0 + KV_TILE > upto) {  // places past the length hold anything
 #pragma unroll
                 for (int i = 0; i < NV; ++i) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        vr[i][e] &= SEL && tile < 0 ? 0u : (jl + 2 * e < len ? 0xffffu : 0u) | (jl + 2 * e + 1 < len ? 0xffff0000u : 0u);
+                        vr[i][e] &= (jl + 2 * e < upto ? 0xffffu : 0u) | (jl + 2 * e + 1 < upto ? 0xffff0000u : 0u);
                 }
             }
             if constexpr (I8) {
