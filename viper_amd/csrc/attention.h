@@ -32,7 +32,7 @@
 // all 43), 7 rows of 48 heads over 8 of 64 dims, 4 sequences of 2003 to 9001, 19: tiles of 4 KB in chains of table, page and
 // tile, with 4 KB to a wave in flight, spend 45 % of the waves' time on memory.  Lists of 64
 // pages of 64 tokens in bf16 8.3, of 128 pages of 32 for 41 rows in FP4 24.6 (91 MB;
-// twice the pages 41, 5.8 TB/s; two to six parts to a row make no difference).
+// twice the pages 41, 5.8 TB/s; two to five parts to a row make no difference).
 //
 // What a row must not see cannot reach it: masked scores are replaced (not
 // added to), places of the last tile past the length are cleared in V.  So a row's
