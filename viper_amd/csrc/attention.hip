@@ -30,6 +30,7 @@ constexpr int AT_WAVES = 8, AT_SHORT = 4096 / KV_TILE, AT_APART = 80000;
 struct AttnPlan {
     int qt, qgroups, waves, splits, lrows;
     int shared;  // parts of all sequences together where they are shared out by length, 0: not
+    bool two;      // workgroups of 8 waves to a CU
     size_t bytes;  // of workspace; 0: one part
 };
 
@@ -46,9 +47,10 @@ static AttnPlan attn_plan(const viper_kv_cache* c, int rows, int64_t units, int6
     if (tiles <= AT_SHORT) p.waves = 4;
     int64_t s = 1;
     p.shared = 0;
+    p.two = false;
     if (base <= AT_CNT) {
-        const bool two = units > 1 && at_two(c->head_dim, c->kv_type != VIPER_KV_BF16, p.qt);
-        const int64_t wgs = (int64_t)device_cus() * AT_WAVES * (two ? 2 : 1) / p.waves;
+        p.two = units > 1 && at_two(c->head_dim, c->kv_type != VIPER_KV_BF16, p.qt);
+        const int64_t wgs = (int64_t)device_cus() * AT_WAVES * (p.two ? 2 : 1) / p.waves;
         s = (wgs + base - 1) / base;
         const int64_t fit = (tiles + p.waves - 1) / p.waves;
         if (share && units > 1 && units <= 64 && s > 1 && fit > 1) {
@@ -132,6 +134,15 @@ static int attn_call(const viper_kv_cache* cache, const viper_kv_batch* batch, c
     if (fn.attn == nullptr) return VIPER_INTERNAL;
     a.by_gqa = (65536u + (unsigned)a.gqa - 1) / (unsigned)a.gqa;
     a.apart = p.splits > 1 && (int64_t)p.splits * p.lrows * D * 4 >= AT_APART;
+    // Over lists, and over FP4 caches where parts are not shared out: from 16 parts on, from 8 where two
+    // workgroups share a CU and 128 join.  FP4, 20 heads over 4 of 128 dims, lists of 64 tiles (16 parts) of
+    // 1 / 4 / 16 rows 7.7 / 9.9 / 15.3 us joined below and 7.4 / 7.7 / 10.4 apart, of 32 tiles (8 parts) 6.9 / 8.0 / 9.6
+    // and 7.3 / 7.5 / 8.3, of 16 tiles (4 parts) 6.4 / 6.9 / 7.5 and 7.1 / 7.3 / 7.4 (bf16, 8 parts of 16
+    // rows over 128 tiles 24.6 and 25.1); shared out parts of 4 sequences of 1024 tokens 7.7 and 8.9.
+    if (sel != nullptr || (cache->kv_type == VIPER_KV_FP4 && !a.share)) {
+        const int64_t joined = (int64_t)p.splits * batch->batch * rows * cache->kv_heads * p.qgroups;
+        a.apart |= p.splits >= 16 || (p.two && p.splits >= 8 && joined >= 128);
+    }
     void* args[] = {&a};
     const dim3 grid((unsigned)(a.splits * rows), (unsigned)(cache->kv_heads * p.qgroups), a.share ? 1u : (unsigned)batch->batch);
     (void)hipLaunchKernel(fn.attn, grid, dim3((unsigned)p.waves * 64), args, at_lds_bytes(D, p.qt, p.waves, p.lrows),
