@@ -270,3 +270,10 @@ def test_a_stack_on_a_4_bit_cache():
         o, bound = R.attention(c, np.arange(4)[None, :], [70], 1, None, q, 8, 64 ** -0.5, 40, 3)
         check(out, o, bound, [70], 1, None, l)
     assert torch.isfinite(s.logits.float()).all()
+
+
+@pytest.mark.parametrize("D,kvh,heads", [(64, 1, 3), (128, 4, 20), (256, 2, 6)])
+@pytest.mark.parametrize("at", range(8))
+def test_one_row_at_every_place_of_an_octet(D, kvh, heads, at):
+    """Rows alone in their octet of tokens: at each place their angles are in LDS by themselves (nothing else is written there)."""
+    test_append_and_read(D, 64, kvh, heads, [8 * i + at + 1 for i in range(0, 120, 3)], None, 1, 10000.0)

@@ -247,17 +247,18 @@ kv_append4_kernel(AppendArgs a) {
     }
     if constexpr (ROPE) {
         double cv = 0.0, sv = 0.0;
-        if (tid < D) {  // the upper half: one step
+        const bool several = t1 - t0 > 1;
+        if (tid < (several ? D : D / 2)) {  // the upper half: one step
             const int d = tid % (D / 2);
             const double f = exp2(-(double)d * (2.0 / D) * a.log2_theta);
-            if (tid < D / 2 || t1 - t0 > 1) sincos(tid < D / 2 ? (double)(lo + t0) * f : f, &sv, &cv);
-            if (tid >= D / 2) {
+            sincos(tid < D / 2 ? (double)(lo + t0) * f : f, &sv, &cv);
+            if (tid >= D / 2) {  // (in the last row's place until the barriers; a row alone may be that one)
                 cs[7][d] = cv;
                 sn[7][d] = sv;
             }
         }
         double c1 = 0.0, s1 = 0.0;
-        if (t1 - t0 > 1) {
+        if (several) {
             __syncthreads();
             if (tid < D / 2) {
                 c1 = cs[7][tid];
