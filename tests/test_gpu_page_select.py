@@ -399,3 +399,24 @@ def test_arguments():
     some = va.KVBatch(batch.block_table, batch.seq_lens, 3, torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda"))
     assert va.kv_page_bounds(g, some, near).ok()
     assert va.select_pages(g, some, q, near, sel, workspace=ws_of(va.select_workspace_bytes(g, some, 8, 4))).ok()
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_bounds_where_rows_begin_past_the_first(given):
+    """Row tensors with rows before the first sequence's: the rows count as kv_append takes them, whether the batch says how many
+    the tensors hold or not."""
+    D, page, kvh, lens, offs = 64, 32, 2, [40, 7], np.array([5, 6, 8], np.int32)
+    rng = np.random.default_rng(2)
+    table, pages = table_for(rng, lens, page)
+    c = F.make_cache("int8", pages, page, kvh, D, rng)
+    g = F.gpu_cache(c, va, dev)
+    batch = va.KVBatch(dev(table), dev(np.array(lens, np.int32)), 2, dev(offs), 8 if given else None)
+    rows = dev(R.bf16_bits(rng.standard_normal((8, kvh * D))))
+    assert va.kv_append(g, batch, rows, rows).ok()
+    c.k, c.ks = back(g.k).ravel(), back(g.k_scales).ravel()
+    out = dev(np.full((pages, kvh, 2, D), SENT))
+    assert va.kv_page_bounds(g, batch, out).ok()
+    want = np.broadcast_to(R.bf16_val(SENT).astype(np.float64), (pages, kvh, 2, D)).copy()
+    P.bounds(c, table, lens, 2, offs, want)
+    np.testing.assert_array_equal(R.bf16_val(back(out)), want)
+    assert np.any(want != R.bf16_val(SENT))

@@ -350,7 +350,7 @@ def kv_page_bounds(cache: KVCache, batch: KVBatch, bounds, stream=None) -> Statu
     if bounds.shape != cache._bounds and not _laid(bounds, cache._bounds):
         return _mismatch(what, "bounds is [num_pages, kv_heads, 2, head_dim]")
     if batch.total_rows is None and batch.row_offsets is not None:
-        ref = batch._rows(min(batch.batch * batch.max_rows, (1 << 31) - 1), dev)  # (an upper limit: offsets past it do not fit)
+        ref = batch._rows((1 << 31) - 1, dev)  # (no row tensor limits the offsets, which may begin past 0)
     else:
         ref = batch._rows(batch.total_rows, dev)
     return _call(lib().viper_hip_kv_page_bounds, what, dev, stream, cache._ref, ref, _flat(bounds, _BF16, dev))
