@@ -94,3 +94,20 @@ def test_tensors():
         va.KVCache(va.KVType.BF16, pool, pool, 64, 4, 128)  # (host memory: no cache to call with)
     assert P.select(np.ones((1, 2)), np.zeros((9, 2, 2)), [3, -1, 5, 6, 8, 7], 9, 32, 191, 1, 1, 4) == [0, 2, 3, 5]
     assert i32(1).dtype == torch.int32
+
+
+@pytest.mark.parametrize("kind", [0, 1, 4])
+def test_bounds_over_any_part_of_the_cache_are_refused(kind):
+    """Keys, values and the scales of either: their first and last bytes, and none that lie right beside."""
+    token = 8 * 4 * 64  # pages, key heads, tokens of a page
+    size = dict(k=token * {0: 256, 1: 128, 4: 64}[kind])
+    size["v"] = size["k"]
+    if kind:
+        size["k_scales"], size["v_scales"] = token * 4, token * 4  # (FP4: 4 exponents of a byte)
+    bounds = 8 * 4 * 2 * 128 * 2
+    none = batch(total_rows=0, row_offsets=FAKE)  # (refused all the same, and no launch)
+    for name, n in size.items():
+        place = {x: (16 + i) * BIG for i, x in enumerate(size)}
+        for at, want in ((0, INVALID), (n - 16, INVALID), (16 - bounds, INVALID), (n, OK), (-bounds, OK)):
+            c = cache(kv_type=kind, **{**place, name: 2 * BIG - at})
+            assert calls(c, none, bounds=2 * BIG)[0] == want, (name, at)

@@ -710,8 +710,8 @@ extern "C" int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper
                         (cache->kv_type == VIPER_KV_FP4 ? 2 : 1);
     const size_t rows = (size_t)cache->num_pages * cache->kv_heads * cache->page_size;
     const size_t scales = cache->kv_type == VIPER_KV_FP4 ? rows * (cache->head_dim / 32) : rows * 4;
-    if (ranges_meet(bounds_bf16, bounds_bytes(cache), cache->k, keys) ||
-        (cache->k_scales != nullptr && ranges_meet(bounds_bf16, bounds_bytes(cache), cache->k_scales, scales)))
+    auto over = [&](const void* p, size_t n) { return p != nullptr && ranges_meet(bounds_bf16, bounds_bytes(cache), p, n); };
+    if (over(cache->k, keys) || over(cache->v, keys) || over(cache->k_scales, scales) || over(cache->v_scales, rows * 4))
         return VIPER_INVALID_ARGUMENT;
     if (batch->total_rows == 0) return VIPER_OK;
     BoundsArgs a;
