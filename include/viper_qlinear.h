@@ -525,7 +525,7 @@ typedef struct viper_kv_cache {
     int32_t num_pages;
     void* k; /* the pools, 16-byte aligned */
     void* v;
-    void* k_scales;  /* int8 (fp32) and FP4 (uint8) only, 16-byte aligned */
+    float* k_scales; /* int8 and FP4 (the uint8 exponents' address) only, 16-byte aligned */
     float* v_scales;
 } viper_kv_cache;
 

@@ -1,5 +1,7 @@
 """The 4-bit cache without a GPU: the tile orders are permutations, the reference's rounding, the cache's arguments."""
 import ctypes as C
+import os
+import subprocess
 
 import numpy as np
 import pytest
@@ -60,3 +62,16 @@ def test_tensors_of_an_fp4_cache():
             make(**kw)
     with pytest.raises(ValueError, match="GPU|device|CUDA"):  # all fits, but for where it is
         make()
+
+
+@pytest.mark.parametrize("compiler,flags", [("gcc", ["-std=c99", "-x", "c"]), ("g++", ["-std=c++17", "-x", "c++"])])
+def test_scales_in_c(compiler, flags):
+    """The scales of a cache description are read as floats in C and C++ (int8), and exponents go in by their address (FP4)."""
+    include = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
+    source = """#include "viper_qlinear.h"
+        float first(const viper_kv_cache* c) { const float* s = c->k_scales; return s[0] + c->k_scales[1] + c->v_scales[1]; }
+        void scales(viper_kv_cache* c, float* k, float* v) { c->k_scales = k; c->v_scales = v; }
+        void exponents(viper_kv_cache* c, unsigned char* k) { c->kv_type = VIPER_KV_FP4; c->k_scales = (float*)k; }"""
+    p = subprocess.run([compiler, *flags, "-Wall", "-Wextra", "-pedantic", "-Werror", "-fsyntax-only", "-I", include, "-"], input=source,
+                       capture_output=True, text=True)
+    assert p.returncode == 0, p.stderr

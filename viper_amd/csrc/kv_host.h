@@ -37,7 +37,7 @@ inline KvArgs kv_args(const viper_kv_cache* c, const viper_kv_batch* b) {
     a.offs = b->row_offsets;
     a.k = c->k;
     a.v = c->v;
-    a.ks = (float*)c->k_scales;
+    a.ks = c->k_scales;
     a.vs = c->v_scales;
     a.batch = b->batch;
     a.max_rows = b->max_rows;
