@@ -75,3 +75,17 @@ def test_scales_in_c(compiler, flags):
     p = subprocess.run([compiler, *flags, "-Wall", "-Wextra", "-pedantic", "-Werror", "-fsyntax-only", "-I", include, "-"], input=source,
                        capture_output=True, text=True)
     assert p.returncode == 0, p.stderr
+
+
+@pytest.mark.parametrize("D,page", [(64, 32), (128, 64), (256, 256)])
+def test_exponents_have_the_shape_of_their_tiles(D, page):
+    """Tiles of head_dim bytes, whose order within is the header's; the same bytes by rows, and no other shape."""
+    u8 = lambda *s: torch.zeros(s, dtype=torch.uint8)
+    pool, vs = u8(3, 4, page // 32, 16 * D), torch.zeros((3, 4, page), dtype=torch.float32)
+    make = lambda ks: va.KVCache(va.KVType.FP4, pool, pool, page, 4, D, ks, vs)
+    for ks in (u8(3, 4, page // 32, D), u8(3, 4, page, D // 32), u8(12 * page * D // 32)):
+        with pytest.raises(ValueError, match="GPU|device|CUDA"):  # all fits, but for where it is
+            make(ks)
+    for ks in (u8(3, 4, D, page // 32 + 1), u8(4, 3, page // 32, D), u8(3, 2, 2 * page // 32, D), u8(3, 4, page // 32, D // 2)):
+        with pytest.raises(ValueError, match="exponent"):
+            make(ks)

@@ -277,3 +277,18 @@ def test_a_stack_on_a_4_bit_cache():
 def test_one_row_at_every_place_of_an_octet(D, kvh, heads, at):
     """Rows alone in their octet of tokens: at each place their angles are in LDS by themselves (nothing else is written there)."""
     test_append_and_read(D, 64, kvh, heads, [8 * i + at + 1 for i in range(0, 120, 3)], None, 1, 10000.0)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_exponents_of_an_empty_cache_are_tiles(D):
+    """k_scales [num_pages, kv_heads, tile, head_dim]: a row's bytes lie in its tile where the header says, and nowhere else."""
+    page, kvh, t = 64, 2, 45
+    g = va.KVCache.empty(va.KVType.FP4, 3, page, kvh, D)
+    assert tuple(g.k_scales.shape) == (3, kvh, 2, D) and bool((g.k_scales == 2).all())
+    x = np.zeros((1, kvh, D), np.float32)
+    x[0, 1] = 2.0 ** (np.arange(D) // 32 * 3)
+    row = dev(R.bf16_bits(x))
+    assert va.kv_append(g, va.KVBatch(dev(np.array([[2]], np.int32)), dev(np.array([t + 1], np.int32))), row, row).ok()
+    want = np.full((3, kvh, 2, D), 2, np.uint8)
+    want[2, 1, t // 32, F.exp_byte(t % 32, np.arange(D // 32), D)] = F.quantize_k(x[0, 1].astype(np.float64))[1]
+    np.testing.assert_array_equal(back(g.k_scales), want)

@@ -59,8 +59,10 @@ class _CBatch(C.Structure):
 class KVCache(_Fixed):
     """Pages of keys and values of one layer: ``k`` and ``v`` bf16 or int8 tensors of num_pages * kv_heads * page_size *
     head_dim elements (their order within a page: include/viper_qlinear.h), ``k_scales`` and ``v_scales`` fp32
-    [num_pages, kv_heads, page_size] for int8.  FP4: two elements to a byte of ``k`` and ``v`` (uint8), ``k_scales`` uint8
-    [num_pages, kv_heads, page_size, head_dim / 32], the exponents of blocks of 32 dimensions, ``v_scales`` as for int8."""
+    [num_pages, kv_heads, page_size] for int8.  FP4: two elements to a byte of ``k`` and ``v`` (uint8), ``v_scales`` as for int8,
+    ``k_scales`` uint8 [num_pages, kv_heads, page_size / 32, head_dim], a tile's exponents of its 32 tokens' blocks of 32 dimensions
+    in an order of their own (the header's; as many bytes of the shape [num_pages, kv_heads, page_size, head_dim / 32] are taken
+    too, and lie in the same order, not by token and block)."""
     kv_type: KVType
     k: Any
     v: Any
@@ -87,9 +89,10 @@ class KVCache(_Fixed):
         rows = (self.num_pages, self.kv_heads, self.page_size)
         if self.k_scales is not None and not _laid(self.v_scales, rows):
             raise ValueError("KVCache: one scale for each token and head, [num_pages, kv_heads, page_size]")
-        if self.k_scales is not None and not (_laid(self.k_scales, (*rows, self.head_dim // 32)) if f4 else _laid(self.k_scales, rows)):
-            raise ValueError("KVCache: one scale for each token and head (FP4 keys: and 32 dimensions), [num_pages, kv_heads, "
-                             "page_size] (head_dim / 32)")
+        shapes = ((*rows[:2], self.page_size // 32, self.head_dim), (*rows, self.head_dim // 32)) if f4 else (rows,)
+        if self.k_scales is not None and not any(_laid(self.k_scales, s) for s in shapes):
+            raise ValueError("KVCache: one scale for each token and head, [num_pages, kv_heads, page_size] (FP4 keys: one exponent for "
+                             "each token, head and 32 dimensions, [num_pages, kv_heads, page_size / 32, head_dim])")
         _one_device(self.k, self.v, self.k_scales, self.v_scales)
         self._c = _CCache(int(self.kv_type), self.kv_heads, self.head_dim, self.page_size, self.num_pages, ptr(self.k, size),
                           ptr(self.v, size), ptr(self.k_scales, 1 if f4 else 4), ptr(self.v_scales, 4))
@@ -112,7 +115,7 @@ class KVCache(_Fixed):
         if kv_type != KVType.BF16:
             vs = torch.zeros(rows, dtype=torch.float32, device=device)
             # (every exponent's least: blocks of zeros)
-            ks = torch.full((*rows, head_dim // 32), 2, dtype=torch.uint8, device=device) if f4 else torch.zeros_like(vs)
+            ks = torch.full((*shape[:3], head_dim), 2, dtype=torch.uint8, device=device) if f4 else torch.zeros_like(vs)
         return cls(kv_type, pool(), pool(), page_size, kv_heads, head_dim, ks, vs)
 
 
