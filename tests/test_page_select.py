@@ -111,3 +111,13 @@ def test_bounds_over_any_part_of_the_cache_are_refused(kind):
         for at, want in ((0, INVALID), (n - 16, INVALID), (16 - bounds, INVALID), (n, OK), (-bounds, OK)):
             c = cache(kv_type=kind, **{**place, name: 2 * BIG - at})
             assert calls(c, none, bounds=2 * BIG)[0] == want, (name, at)
+
+
+@pytest.mark.parametrize("bad,says", [(dict(select=4), "context"), (dict(context=64, select=4, sinks=3), "sinks"),
+                                      (dict(context=64, select=4, window=9), "window"), (dict(context=64, select=2), "keep"),
+                                      (dict(context=64, select=-1), "keep"), (dict(context=64, select=4, keep_last=0), "keep"),
+                                      (dict(context=64, select=4, keep_first=-1), "keep")])
+def test_a_stack_refuses_a_selection_that_it_could_not_follow(bad, says):
+    from viper_amd.stack import Stack
+    with pytest.raises(ValueError, match=says):  # (before it lays anything out)
+        Stack(torch, hidden=512, inter=1024, n_heads=8, n_kv_heads=2, head_dim=64, layers=1, passes=1, vocab=64, **bad)

@@ -36,7 +36,7 @@ each step, a captured step's replays included; past `capacity` tokens results
 are NaN.  With `select` > 0 the new token attends over that many pages of each
 slot's cache alone: the first `keep_first`, the last `keep_last` and those whose
 keys' bounds promise most (kv_page_bounds, select_pages and attention_selected in
-place of attention_paged).
+place of attention_paged); it takes neither `window` nor `sinks`.
 """
 import ctypes as C
 import math
@@ -51,6 +51,13 @@ class Stack:
     def __init__(self, torch, hidden=2560, inter=10240, n_heads=20, n_kv_heads=4, head_dim=128,
                  layers=22, passes=2, vocab=166144, seed=0x5EED0003, eps=1e-6, context=0, kv_type=_d.KVType.BF16, page_size=64,
                  rope_theta=10000.0, window=0, sinks=0, select=0, keep_first=1, keep_last=2):
+        if select:  # (what a selection cannot follow is refused, not left out)
+            if not context:
+                raise ValueError("Stack: a selection is of a context's pages (context > 0)")
+            if window or sinks:
+                raise ValueError("Stack: select and window or sinks exclude each other (keep_first and keep_last stay visible)")
+            if keep_first < 0 or keep_last < 1 or select < keep_first + keep_last:
+                raise ValueError("Stack: select lists keep_first (>= 0) and keep_last (>= 1) pages at least")
         self.torch = torch
         self.H, self.I = hidden, inter
         self.nQ, self.nKV = n_heads * head_dim, n_kv_heads * head_dim
@@ -140,8 +147,6 @@ class Stack:
             nws = _d.attention_workspace_bytes(self.kv[0], self.rows, n_heads)
             self.select, self.keep = select, dict(first=keep_first, last=keep_last)
             if select:
-                if window:
-                    raise ValueError("Stack: select and window exclude each other")
                 nws = _d.attention_selected_workspace_bytes(self.kv[0], self.rows, n_heads, select)
                 self.bounds = [torch.zeros((pages, n_kv_heads, 2, head_dim), dtype=torch.bfloat16, device="cuda")
                                for _ in range(layers * passes)]
