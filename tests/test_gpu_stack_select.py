@@ -82,3 +82,34 @@ def test_all_pages_listed_is_the_whole_context():
 def test_a_window_excludes_a_selection():
     with pytest.raises(ValueError, match="window"):
         Stack(torch, **SMALL, context=64, page_size=32, window=10, select=2)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "fp4"])
+def test_attention_over_all_pages_listed_is_the_whole_contexts(kind):
+    """Slot 0 of a stack whose lists hold every page and of one without lists (its inputs are the same at each step): the lists,
+    and both attentions within the derived bound of one plain result."""
+    kw = dict(context=96, page_size=32, kv_type=va.KVType[kind.upper()])
+    a, b = Stack(torch, **SMALL, **kw, select=3, keep_last=1), Stack(torch, **SMALL, **kw)
+    seen = {}
+    for name, s in (("listed", a), ("whole", b)):
+        def attend(l, name=name, s=s, plain=s.attend):
+            plain(l)
+            if l == 0:
+                seen[name] = bits(s.q), bits(s.attn)
+        s.attend = attend
+    for n in range(1, 97):
+        a.step_fused(), b.step_fused()
+        held_pages = -(-n // 32)
+        assert a.selected.cpu().numpy()[0].tolist() == [list(range(held_pages)) + [-1] * (3 - held_pages)] * 2
+        if n not in (1, 2, 31, 32, 33, 64, 65, 95, 96):
+            continue
+        np.testing.assert_array_equal(seen["listed"][0], seen["whole"][0])
+        c = F.Cache4(3, 32, 2, 64) if kind == "fp4" else R.Cache(kind == "int8", 3, 32, 2, 64)
+        g = a.kv[0]
+        c.k, c.v = (back(t if kind != "bf16" else t.view(torch.int16)).ravel() for t in (g.k, g.v))
+        if kind != "bf16":
+            c.ks, c.vs = back(g.k_scales).ravel(), back(g.v_scales).ravel()
+        o, bound = R.attention(c, np.arange(3)[None, :], [n], 1, None, seen["whole"][0], 8, 64 ** -0.5)
+        assert np.abs(o[0]).max() > 0
+        for name in seen:
+            check(seen[name][1], o, bound, [n], 1, None, (name, n))
