@@ -232,3 +232,121 @@ def test_every_head_of_a_key_head_counts(D, G):
         x = R.bf16_val(q[r]).astype(np.float64).reshape(kvh, G, D)
         for h in range(kvh):
             assert got[r, h].tolist() == P.select(x[h], f[:, h], table[b], n, page, p, 1, 2, count), (b, r, p, h)
+
+
+def busy(stream, a, b):
+    """Copies of 600 GB in all on a stream (over a tenth of a second) on a stream, which the host is well ahead of."""
+    with torch.cuda.stream(stream):
+        for _ in range(300):
+            a.copy_(b)
+
+
+@pytest.mark.parametrize("how", ["argument", "number", "current"])
+@pytest.mark.parametrize("kind", ["fp4", "bf16"])
+def test_each_call_waits_for_the_work_before_it_on_its_stream(kind, how):
+    """Inputs change on a side stream behind a delay, then the call: a launch of it on any other stream (the second of the selection,
+    and of attentions that join apart, among them) would still see the former inputs, or what the former call left of them."""
+    D, page, kvh, heads, n, count = 128, 64, 2, 10, 20000, 64
+    rng = np.random.default_rng(7)
+    table, pages = table_for(rng, [n], page)
+    lens = dev(np.array([n], np.int32))
+    fill, one = va.KVBatch(dev(table), lens, 300), va.KVBatch(dev(table), lens)
+    caches = [F.gpu_cache(F.make_cache(kind, pages, page, kvh, D, rng), va, dev) for _ in range(2)]
+    g = F.gpu_cache(F.make_cache(kind, pages, page, kvh, D, rng), va, dev)
+    pools = [t for t in ("k", "v", "k_scales", "v_scales") if getattr(g, t) is not None]
+    rows = [dev(R.bf16_bits(rng.standard_normal((300, kvh * D)))) for _ in range(2)]
+    qs = [dev(R.bf16_bits(rng.standard_normal((1, heads * D)))) for _ in range(2)]
+    near = dev(R.bf16_bits(np.sort(rng.standard_normal((pages, kvh, 2, D)), 2)))
+    lists = [torch.stack([torch.randperm(n // page, device="cuda")[:count] for _ in range(kvh)])[None].to(torch.int32) for _ in range(2)]
+    row, q, sel = rows[0].clone(), qs[0].clone(), lists[0].clone()
+    box = lambda *s, dt=torch.int16: torch.zeros(s, dtype=dt, device="cuda")
+    bounds, chosen, out, whole, ko, vo = (box(pages, kvh, 2, D), box(1, kvh, count, dt=torch.int32), box(1, heads * D), box(1, heads * D),
+                                          box(300, kvh, D), box(300, kvh, D))
+    ws = [ws_of(va.select_workspace_bytes(g, one, heads, count)), ws_of(va.attention_selected_workspace_bytes(g, one, heads, count)),
+          workspace(g, one, heads)]
+    content = [[getattr(c, t) for t in pools] for c in caches]
+    held = [getattr(g, t) for t in pools]
+    steps = [  # name, inputs, what they hold before and after, outputs, call
+        ("append", [row], [[x] for x in rows], held, lambda st: va.kv_append(g, fill, row, row, stream=st)),
+        ("read", held, content, [ko, vo], lambda st: va.kv_read(g, fill, ko, vo, stream=st)),
+        ("bounds", held, content, [bounds], lambda st: va.kv_page_bounds(g, fill, bounds, stream=st)),
+        ("select", [q], [[x] for x in qs], [chosen], lambda st: va.select_pages(g, one, q, near, chosen, workspace=ws[0], stream=st)),
+        ("lists", [sel], [[x] for x in lists], [out], lambda st: va.attention_selected(g, one, q, sel, out, workspace=ws[1], stream=st)),
+        ("queries", [q], [[x] for x in qs], [out], lambda st: va.attention_selected(g, one, q, sel, out, workspace=ws[1], stream=st)),
+        ("whole", [q], [[x] for x in qs], [whole], lambda st: va.attention_paged(g, one, q, whole, workspace=ws[2], stream=st))]
+    side = torch.cuda.Stream()
+    given = {"argument": side, "number": side.cuda_stream, "current": None}[how]
+    big = [torch.zeros(1 << 30, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    for name, inputs, (old, new), outputs, call in steps:
+        print("stream", kind, how, name, flush=True)
+
+        def now(values):
+            for t, x in zip(inputs, values):
+                t.copy_(x)
+
+        start = [t.clone() for t in outputs]
+        now(new)
+        assert call(None).ok()
+        want = [t.clone() for t in outputs]
+        for t, x in zip(outputs, start):
+            t.copy_(x)
+        now(old)
+        assert call(None).ok()
+        assert not all(torch.equal(t, x) for t, x in zip(outputs, want))
+        torch.cuda.synchronize()
+        busy(side, *big)
+        with torch.cuda.stream(side):
+            now(new)
+            if how == "current":
+                assert call(None).ok()
+        if how != "current":
+            assert call(given).ok()
+        assert not side.query()  # (the delay still runs: nothing before the call has)
+        with torch.cuda.stream(side):
+            got = [t.clone() for t in outputs]
+        side.synchronize()
+        for t, x in zip(got, want):
+            assert torch.equal(t.view(torch.uint8), x.view(torch.uint8)), name
+
+
+def test_chains_on_several_streams_at_once():
+    """Four chains, each of tensors of its own, all queued before the first is waited for, on the default stream and three others."""
+    D, page, kvh, heads, n, count = 128, 64, 2, 10, 9000, 40
+    rng = np.random.default_rng(8)
+    table, pages = table_for(rng, [n], page)
+    lens = dev(np.array([n], np.int32))
+    fill, one = va.KVBatch(dev(table), lens, n), va.KVBatch(dev(table), lens)
+    rows = [dev(R.bf16_bits(rng.standard_normal((n, kvh * D)))) for _ in range(4)]
+    qs = [dev(R.bf16_bits(rng.standard_normal((1, heads * D)))) for _ in range(4)]
+
+    def tensors():
+        g = va.KVCache.empty(va.KVType.FP4, pages, page, kvh, D)
+        return (g, torch.zeros((pages, kvh, 2, D), dtype=torch.int16, device="cuda"),
+                torch.zeros((1, kvh, count), dtype=torch.int32, device="cuda"), dev(np.zeros((1, heads * D), np.uint16)),
+                ws_of(va.select_workspace_bytes(g, one, heads, count)), ws_of(va.attention_selected_workspace_bytes(g, one, heads, count)))
+
+    def calls(i, t, stream):
+        g, near, sel, out, w0, w1 = t
+        return (lambda: va.kv_append(g, fill, rows[i], rows[i], stream=stream), lambda: va.kv_page_bounds(g, fill, near, stream=stream),
+                lambda: va.select_pages(g, one, qs[i], near, sel, workspace=w0, stream=stream),
+                lambda: va.attention_selected(g, one, qs[i], sel, out, workspace=w1, stream=stream))
+
+    want = []
+    for i in range(4):  # one after the other
+        t = tensors()
+        for call in calls(i, t, None):
+            assert call().ok()
+        torch.cuda.synchronize()
+        want.append([x.clone() for x in t[1:4]])
+    streams = [None] + [torch.cuda.Stream() for _ in range(3)]
+    for _ in range(5):
+        runs = [tensors() for _ in range(4)]
+        chains = [calls(i, t, s) for i, (t, s) in enumerate(zip(runs, streams))]
+        torch.cuda.synchronize()
+        for step in zip(*chains):
+            for call in step:
+                assert call().ok()
+        torch.cuda.synchronize()
+        for t, w in zip(runs, want):
+            for a, b in zip(t[1:4], w):
+                assert torch.equal(a, b)
