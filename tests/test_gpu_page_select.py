@@ -420,3 +420,37 @@ def test_bounds_where_rows_begin_past_the_first(given):
     P.bounds(c, table, lens, 2, offs, want)
     np.testing.assert_array_equal(R.bf16_val(back(out)), want)
     assert np.any(want != R.bf16_val(SENT))
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page", [32, 128])
+@pytest.mark.parametrize("kind", ["int8", "fp4"])
+def test_bounds_of_scales_that_are_not_finite(kind, page, D):
+    """A block of keys that is not finite (FP4: exponent 255) makes its 32 dimensions' bounds NaN, a scale of NaN or an infinity
+    (int8) what kv_read makes of it; places past the sequence hold anything."""
+    n, kvh = 2 * page + 21, 2
+    rng = np.random.default_rng(D + page)
+    c = F.make_cache(kind, 4, page, kvh, D, rng)
+    table = np.array([[2, 0, 3]], np.int32)
+    for t, head, block in ((5, 0, 0), (page + 3, 1, D // 32 - 1), (page + 9, 0, 1), (2 * page + 20, 1, 0)):
+        tile = (int(table[0, t // page]) * kvh + head) * (page // 32) + t % page // 32
+        if kind == "fp4":
+            c.ks[tile * D + F.exp_byte(t % 32, block, D)] = 255
+        else:
+            c.ks[tile * 32 + t % 32] = np.nan if block == 0 else np.inf
+    past = 2 * page + 21
+    tile = (3 * kvh + 0) * (page // 32) + past % page // 32
+    if kind == "fp4":
+        c.ks[tile * D + F.exp_byte(past % 32, np.arange(D // 32), D)] = 255
+    else:
+        c.ks[tile * 32 + past % 32] = np.nan
+    g = F.gpu_cache(c, va, dev)
+    out = dev(np.full((4, kvh, 2, D), SENT))
+    assert va.kv_page_bounds(g, va.KVBatch(dev(table), dev(np.array([n], np.int32)), n), out).ok()
+    want = np.broadcast_to(R.bf16_val(SENT).astype(np.float64), (4, kvh, 2, D)).copy()
+    with np.errstate(all="ignore"):
+        P.bounds(c, table, [n], n, None, want)
+    np.testing.assert_array_equal(R.bf16_val(back(out)), want)
+    assert np.isnan(want[2, 0]).any() and np.isnan(want[3, 1]).any() and np.isfinite(want[3, 0]).all()
+    if kind == "fp4":
+        assert np.isnan(want[2, 0, :, :32]).all() and np.isfinite(want[2, 0, :, 32:]).all()
