@@ -614,11 +614,14 @@ int viper_hip_kv_page_bounds(const viper_kv_cache* cache, const viper_kv_batch* 
  * (token j lies on page j / page_size), in order, then -1.  Of its pages 0 ..
  * p / page_size the first `first` and the last `last` (>= 1) are listed; of the
  * others those with the largest scores (of equal ones the first) until `count`
- * (>= first + last) are.  A page's score bounds scale * q . k from above, for
- * every scale: max over the heads' q of sum_d max(q_d lo_d, q_d hi_d), summed in
- * 64 bits and rounded to fp32, NaN as +inf; pages that the table lacks have none and
- * are listed only among the first and last.  Bounds are as kv_page_bounds leaves
- * them: lo <= hi, or both NaN.  Rows at negative positions list none;
+ * (>= first + last) are.  A page's score is max over the heads' q of
+ * sum_d max(q_d lo_d, q_d hi_d), summed in 64 bits and rounded to fp32, NaN as
+ * +inf; pages that the table lacks have none and are listed only among the first and
+ * last.  Bounds are as kv_page_bounds leaves them: lo <= hi, or both NaN.  So, but for
+ * that rounding, no key k of the page that is held in bf16 or FP4 has a larger q . k.
+ * Bounds of int8 keys are of code * scale rounded to bf16, as kv_read gives it, and
+ * attention takes it unrounded: its q . k may be larger by up to 2^-8 sum_d |q_d k_d|.
+ * Rows at negative positions list none;
  * pages past the table are not considered.  max_rows <= VIPER_QLINEAR_MAX_M, heads
  * as for viper_hip_attention_paged, count * page_size < 2^31, batch kv_heads
  * ceil(table_width / 64) < 2^24.  selected and workspace (16-byte

@@ -235,7 +235,7 @@ def test_every_head_of_a_key_head_counts(D, G):
 
 
 def busy(stream, a, b):
-    """Copies of 600 GB in all on a stream (over a tenth of a second) on a stream, which the host is well ahead of."""
+    """Copies of 600 GB in all (over a tenth of a second) on a stream, which the host is well ahead of."""
     with torch.cuda.stream(stream):
         for _ in range(300):
             a.copy_(b)

@@ -2,6 +2,8 @@
 import numpy as np
 import pytest
 
+import decode_ref as R
+import fp4_ref as F
 import pages_ref as P
 import viper_amd as va
 from test_decode_refusals import BAD_BATCH, BAD_CACHE, FAKE, INVALID, OK, batch, cache, ref
@@ -121,3 +123,28 @@ def test_a_stack_refuses_a_selection_that_it_could_not_follow(bad, says):
     from viper_amd.stack import Stack
     with pytest.raises(ValueError, match=says):  # (before it lays anything out)
         Stack(torch, hidden=512, inter=1024, n_heads=8, n_kv_heads=2, head_dim=64, layers=1, passes=1, vocab=64, **bad)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "int8", "fp4"])
+def test_scores_bound_the_keys_of_their_pages(kind):
+    """A page's score, unrounded, against q . k of each of its keys as attention takes them: at least that for bf16 and FP4; int8
+    keys are bounded after a rounding to bf16 (half a step, 2^-8 of the value), and some do lie above."""
+    D, page, pages = 64, 32, 40
+    rng = np.random.default_rng(9)
+    c = F.make_cache(kind, pages, page, 1, D, rng)
+    near = np.zeros((pages, 1, 2, D))
+    table = [np.arange(pages)]
+    P.bounds(c, table, [pages * page], pages * page, None, near)
+    k = c.rows(table[0], np.arange(pages * page), 0, True).reshape(pages, page, D)
+    q = R.bf16_val(R.bf16_bits(rng.standard_normal((500, D)))).astype(np.float64)
+    q = np.concatenate([q, np.sign(k[:, 0]), np.sign(k[:, 1])])  # (along a key's own signs: nearest to the bound)
+    over = -np.inf
+    for p in range(pages):
+        score = np.maximum(q * near[p, 0, 0], q * near[p, 0, 1]).sum(1)
+        dot, size = q @ k[p].T, np.abs(q) @ np.abs(k[p]).T
+        slack = 2.0 ** -8 * size if kind == "int8" else 0.0
+        assert np.all(dot <= score[:, None] + slack + D * 2.0 ** -52 * size)  # (sums in 64 bits)
+        one = q * k[p, 0]  # of a page that holds one key alone
+        r = R.bf16_val(R.bf16_bits(k[p, 0].astype(np.float32))).astype(np.float64)
+        over = max(over, (one.sum(1) - (q * r).sum(1)).max())
+    assert (over > 1e-6) == (kind == "int8")

@@ -5,7 +5,10 @@
 // a time, where NaN lies past the infinities and so is not lost.
 //
 // selection: q . k of any key of a page is at most sum_d max(q_d lo_d, q_d hi_d), the page's
-// score for a query head; the largest over the heads of a key head counts.  A page at the
+// score for a query head; the largest over the heads of a key head counts.  (Keys as kv_read
+// gives them: int8 keys are bounded after their rounding to bf16, which attention does not
+// make, so there q . k may be larger by 2^-8 sum_d |q_d k_d|: a page that close to the border
+// may be taken for a lesser one, and what is listed is the same on every run.)  A page at the
 // border is in or out, so a score is that of the sum in 64 bits.  One launch has all scores
 // as matrix products in 32 bits, with a limit to how far they may be off; a second finds the
 // border among them and computes in 64 bits only the pages too near to it.
