@@ -31,8 +31,10 @@
 // kernel of 14.6 and a join), 32 sequences of 700 to 16384 35 (with parts of equal numbers for
 // all 43), 7 rows of 48 heads over 8 of 64 dims, 4 sequences of 2003 to 9001, 19: tiles of 4 KB in chains of table, page and
 // tile, with 4 KB to a wave in flight, spend 45 % of the waves' time on memory.  Lists of 64
-// pages of 64 tokens in bf16 8.3, of 128 pages of 32 for 41 rows in FP4 24.6 (91 MB;
-// twice the pages 41, 5.8 TB/s; two to five parts to a row make no difference).
+// pages of 64 tokens in bf16 8.3, int8 8.1; of 128 pages of 32 for 41 rows in FP4 24.6 (91 MB;
+// twice the pages 41, 5.8 TB/s; two to five parts to a row make no difference), int8 40.6, bf16
+// 62.5.  Rows read their lists' pages each for itself: four rows of 16 sequences with one list a
+// sequence 25.1 in FP4 (30.9 with a list a row), int8 43.2 (53.8), bf16 93.1 (87.7).
 //
 // What a row must not see cannot reach it: masked scores are replaced (not
 // added to), places of the last tile past the length are cleared in V.  So a row's

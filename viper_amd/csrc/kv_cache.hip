@@ -194,12 +194,13 @@ kv_append_kernel(AppendArgs a) {
 // FP4: two tokens of a value share a byte and eight a word, so a workgroup takes the
 // rows of one octet of tokens (one row of a decode step, eight of a prompt) and stores its
 // words whole, those of an octet that the call does not fill with what they held of the
-// other tokens (flipping their bits by atomics took 8.6 us for one row, this 3.7).
+// other tokens (flipping their bits by atomics took 8.6 us for one row, this 3.5).
 // The angles of all rows are in LDS before the first: those of the first row and of one
 // step by sincos, each further row's by the sum of angles (4 products of 64 bits).  A
 // row's values are in flight while the one before is rounded.  9700 rows of 20 + 4 + 4 heads
-// of 128 in 35 us (124 MB): not more rows in flight, nor whole tiles to one XCD made a
-// difference; 235 VALU instructions a wave and row, two thirds of them the rotation's.
+// of 128 in 33.5 us (124 MB): 13 are VALU issue, two thirds of it the rotation's, and waves wait
+// 57 % of their time, four to a SIMD (101 registers; 1220 octets are a round of 1024 workgroups and
+// a fifth of another).  Not more rows in flight, nor whole tiles to one XCD made a difference.
 template <int D, bool ROPE>
 __global__ void __launch_bounds__(KA_NT)
 kv_append4_kernel(AppendArgs a) {

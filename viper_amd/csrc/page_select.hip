@@ -15,7 +15,9 @@
 //
 // Measured (20 heads over 4 key heads of 128 dims): 64 of 2048 pages for one row 8.6 us
 // (scores 4.4, selection 5.2: latency); 128 of up to 2032 for 4 rows of 16 sequences 21.2
-// (13.0 and 8.4; 38 MB of bounds, 5.7 us at 6.7 TB/s); all scores in 64 bits took 48.
+// (13.0 and 8.4; 38 MB of bounds, 5.7 us at 6.7 TB/s); all scores in 64 bits took 48.  A row
+// and key head with a score that is no finite number (a NaN key), or with more than 64 pages
+// in doubt (equal ones), has all pages scored in 64 bits by its one workgroup: 1.05 ms and 1.15.
 
 #include "kv_host.h"
 
@@ -49,9 +51,9 @@ constexpr int DPP_ROR8 = 0x128;  // lane i <- i ^ 8 within 16
 // meet in LDS) with the tile's 16-byte loads.  The least and, complemented, the largest of a
 // lane's token are R registers; each step of the way over the 16 lanes of other tokens
 // halves them, a lane keeping the half that one bit of its number says.  3 prompts of
-// 20000 tokens in pages of 32, int8, take 9.1 us (16.5 MB, 2.5 us at 6.7 TB/s: 400 VALU
-// instructions a wave are 5 us of issue), one decode row of 16 sequences 3.3; 4 pages to a workgroup of one wave for
-// each 32 dims took 11.5.
+// 20000 tokens in pages of 32, int8, take 9.1 us (16.5 MB, 2.5 us at 6.7 TB/s: 820 VALU
+// instructions in each of the 3500 waves that have a page are 5 us of issue), one decode row
+// of 16 sequences 3.3; 4 pages to a workgroup of one wave for each 32 dims took 11.5.
 template <int D, int KT>
 __global__ void __launch_bounds__(PB_NT)
 page_bounds_kernel(BoundsArgs a) {
